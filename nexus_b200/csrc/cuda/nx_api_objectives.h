@@ -1,0 +1,66 @@
+// C ABI of the operators that fine-tune a language model on rewards and preferences: log-probabilities of given tokens, clipped
+// policy loss, preference loss, global gradient norm over many tensors.  Conventions as in nx_api.h.
+#pragma once
+#include "nx_api.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+// Logits of `rows` tokens: row r starts at logits + (r / per) * stride_outer + (r % per) * stride_inner elements (any alignment of the
+// element) and has `width` elements, of which the first `vocab` are the vocabulary.  targets [rows]: int32 or int64; a row whose target is
+// `ignore_index` is not read, one whose target lies outside the vocabulary gives NaN and a gradient of zeros.
+typedef struct NxTokenRows {
+  const void* logits;
+  const void* targets;
+  int64_t rows, per, stride_outer, stride_inner, ignore_index;
+  int32_t dtype;         // NX_BF16, NX_F16 or NX_F32
+  int32_t targets_wide;  // targets are int64
+  int32_t vocab, width;
+  float inv_temp;        // the logits are multiplied by it
+  int32_t pad_;
+} NxTokenRows;
+
+// logp [rows] = log-probability of the target (0 where ignored); stats [rows] pairs: the largest logit, and log2 of the sum of
+// exp((logit - largest) * inv_temp).
+int nx_token_logprobs(const NxTokenRows* rows, float* logp, float* stats, nx_stream_t stream);
+// grad = coef (delta_target - p) * inv_temp in the layout and type of the logits (zeros in ignored rows and behind the vocabulary);
+// coef of row r: coef[r / coef_per] * *factor (factor: device scalar, may be null)
+int nx_token_logprobs_grad(const NxTokenRows* rows, const float* stats, const float* coef, int64_t coef_per, const float* factor,
+                           void* grad, nx_stream_t stream);
+
+enum NxPolicyKl { NX_KL_K1 = 0, NX_KL_K2 = 1, NX_KL_K3 = 2 };
+enum NxPolicyMean { NX_MEAN_TOKEN = 0, NX_MEAN_SEQUENCE = 1, NX_MEAN_NONE = 2 };
+typedef struct NxPolicyArgs {
+  const float* old_logp;    // [rows]
+  const float* ref_logp;    // [rows], may be null (no KL term)
+  const float* advantages;  // advantage of row r: advantages[r / adv_per]
+  int64_t adv_per;
+  int64_t seq_len;          // tokens of a sequence: row r belongs to sequence r / seq_len
+  float clip_low, clip_high, kl_coef, entropy_coef, scale;
+  int32_t kl, mean;
+  int32_t write_grad;
+} NxPolicyArgs;
+// Clipped policy loss with KL and entropy terms.  logp, kl, entropy, row_loss: [rows]; totals: two doubles, counts: [rows / seq_len],
+// both scratch; loss: one float;
+// grad (write_grad): d loss / d logits in the layout and type of the logits.
+int nx_policy_loss(const NxTokenRows* rows, const NxPolicyArgs* args, double* totals, int32_t* counts, float* logp, float* kl, float* entropy,
+                   float* row_loss, float* loss, void* grad, nx_stream_t stream);
+// x *= *factor in place, n elements; nothing is read or written where the factor is 1
+int nx_scale_unless_one(void* x, const float* factor, int dtype, int64_t n, nx_stream_t stream);
+
+enum NxPreferenceKind { NX_PREF_SIGMOID = 0, NX_PREF_HINGE = 1, NX_PREF_IPO = 2 };
+typedef struct NxPreferenceArgs {
+  const float* logp;       // [2 * pairs, seq_len] per token, chosen sequences first
+  const void* targets;     // [2 * pairs, seq_len]
+  const float* ref_logp;   // [2 * pairs], may be null
+  int64_t pairs, seq_len, ignore_index;
+  int32_t targets_wide, kind, average;
+  float beta, smoothing, target_margin;
+} NxPreferenceArgs;
+// seq_logp [2 * pairs], margin [pairs], coef [2 * pairs] = d loss / d logp of each counted token, loss: one float
+int nx_preference_loss(const NxPreferenceArgs* args, float* seq_logp, float* margin, float* coef, float* loss, nx_stream_t stream);
+
+#ifdef __cplusplus
+}
+#endif

@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "nx_api_kernels.h"
+#include "row_vec.cuh"
 
 #include <algorithm>
 #include <cstdio>
@@ -167,53 +168,6 @@ __global__ void ce_row_kernel(LT* __restrict__ logits, const int32_t* __restrict
   }
   for (int64_t c = vocab + threadIdx.x; c < ld; c += blockDim.x) Num<LT>::store(lr + c, 0.0f);
 }
-
-// 16-byte vector access to a logits row: 8 bf16 or 4 fp32 per load.
-template <typename LT>
-struct RowVec;
-template <>
-struct RowVec<__nv_bfloat16> {
-  static constexpr int kN = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) { unpack(*reinterpret_cast<const uint4*>(p), v); }
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
-      v[2 * i] = __low2float(h);
-      v[2 * i + 1] = __high2float(h);
-    }
-  }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-// 2^x; results below the smallest normal number are zeros (beside a maximum of 1 they are far below the last bit of the sum)
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <>
-struct RowVec<float> {
-  static constexpr int kN = 4;
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  }
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
-    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
 
 // Vectorised variant of ce_row_kernel: rows are 16-byte aligned (ld a multiple of the vector width).
 // Pass 1 streams the row from HBM (online max / sum-exp in the log2 domain); pass 2 re-reads it

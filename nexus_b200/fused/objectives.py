@@ -1,0 +1,303 @@
+"""Operators that fine-tune a language model on rewards and preferences: log-probabilities of given tokens, the clipped policy loss
+with KL and entropy terms, the preference loss over pairs, and the global gradient norm over many tensors with clipping.
+
+On CUDA logits (BF16, FP16, FP32) every operator runs hand-written sm_100a kernels (``csrc/cuda/token_objectives.cu``); elsewhere the
+same mathematics runs as plain PyTorch, which is also what the GPU tests compare against.  All of them are reached as
+``fused.ops.<name>``, beside the cross-entropy.
+
+With x = logits / temperature over the vocabulary: logp_t = x_t - logsumexp(x), H = -sum p log p.  A target equal to `ignore_index`
+takes its token out of everything (prompts, padding): its results and gradients are zeros and its logits are never read, whatever they
+hold.  A target outside the vocabulary gives NaN and a gradient of zeros.  Statistics are FP32; sums over tokens FP64."""
+from __future__ import annotations
+
+import math
+from typing import List, NamedTuple, Optional, Sequence
+
+import torch
+from torch.autograd.function import once_differentiable
+
+_KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+class PolicyLoss(NamedTuple):
+    """What `policy_loss` returns: the loss (differentiable with respect to the logits) and, per token and detached, the new
+    log-probability, the KL estimate against the reference and the entropy (zeros where a token does not count)."""
+    loss: torch.Tensor
+    logp: torch.Tensor
+    kl: torch.Tensor
+    entropy: torch.Tensor
+
+
+class PreferenceLoss(NamedTuple):
+    """What `preference_loss` returns: the loss (differentiable with respect to the logits) and, detached, the log-probability of each
+    sequence [2 * pairs] and the margin of each pair (log-ratio of the chosen sequence minus that of the rejected one)."""
+    loss: torch.Tensor
+    logp: torch.Tensor
+    margin: torch.Tensor
+
+
+def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature: float) -> int:
+    if not torch.is_floating_point(logits) or logits.dim() < 1:
+        raise ValueError(f"{name}: logits must be a floating-point tensor [..., vocabulary]")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: targets must be int32 or int64, got {targets.dtype}")
+    if targets.shape != logits.shape[:-1]:
+        raise ValueError(f"{name}: targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
+    if targets.device != logits.device:
+        raise ValueError(f"{name}: targets on {targets.device}, logits on {logits.device}")
+    _check_temperature(name, temperature)
+    V = logits.shape[-1] if vocab is None else int(vocab)
+    if not 1 <= V <= logits.shape[-1]:
+        raise ValueError(f"{name}: vocab must be between 1 and {logits.shape[-1]}, got {V}")
+    if logits.shape[-1] >= 2 ** 31 or targets.numel() >= 2 ** 31:
+        raise ValueError(f"{name}: at most 2^31 - 1 rows and columns")
+    return V
+
+
+def _check_temperature(name: str, temperature: float) -> None:
+    if not (math.isfinite(temperature) and temperature > 0.0):
+        raise ValueError(f"{name}: temperature must be positive, got {temperature}")
+
+
+def _check_values(name: str, what: str, t, shapes, device) -> torch.Tensor:
+    """A tensor of constants of the loss in FP32: log-probabilities, advantages."""
+    if not torch.is_tensor(t) or not torch.is_floating_point(t):
+        raise ValueError(f"{name}: {what} must be a floating-point tensor")
+    if tuple(t.shape) not in shapes:
+        raise ValueError(f"{name}: {what} must have the shape {' or '.join(map(str, shapes))}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name}: {what} on {t.device}, logits on {device}")
+    return t.detach().float().contiguous()
+
+
+def _kernels(t: torch.Tensor) -> bool:
+    if not t.is_cuda or t.dtype not in _KERNEL_TYPES:
+        return False
+    from ..ops import _cuda as K
+    K.lib()  # raises loudly when the library is missing on a GPU machine
+    return True
+
+
+def _token_parts(logits, targets, ignore_index, temperature, V):
+    """Plain form: (counted, log-probabilities of all tokens [N, V], log-probability of the target [N]); FP32, or FP64 for FP64."""
+    x = logits.reshape(-1, logits.shape[-1])[:, :V]
+    x = (x if x.dtype == torch.float64 else x.float()) / temperature
+    t = targets.reshape(-1).long()
+    keep = t != ignore_index
+    x = torch.where(keep[:, None], x, torch.zeros((), dtype=x.dtype, device=x.device))
+    lp = torch.log_softmax(x, -1)
+    inside = (t >= 0) & (t < V)
+    logp = lp.gather(1, torch.where(inside, t, 0)[:, None])[:, 0]
+    logp = torch.where(inside, logp, torch.full((), math.nan, dtype=lp.dtype, device=lp.device))
+    return keep, lp, torch.where(keep, logp, torch.zeros((), dtype=lp.dtype, device=lp.device))
+
+
+# ------------------------------------------------------------------------------------- log-probabilities of given tokens
+class _TokenLogprobs(torch.autograd.Function):
+    """One read of the logits forward (largest logit and sum per row are kept), one read and one write backward."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature):
+        from ..ops import _objectives as O
+        with torch.cuda.device(logits.device):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            logp, stats = O.token_logprobs(rows, logits.device)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.cfg = (vocab, ignore_index, temperature)
+        return logp.view(targets.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp):
+        from ..ops import _objectives as O
+        logits, targets, stats = ctx.saved_tensors
+        vocab, ignore_index, temperature = ctx.cfg
+        with torch.cuda.device(logits.device):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            coef = dlogp.float().contiguous()
+            grad = O.empty_grad(logits)
+            O.token_logprobs_grad(rows, stats, coef, 1, None, grad)
+        return grad, None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
+                   vocab: Optional[int] = None) -> torch.Tensor:
+    """FP32 log-probability of ``targets`` [...] under ``softmax(logits / temperature)``, logits [..., V(+pad)]; zero where the target is
+    `ignore_index`.  Differentiable (once) with respect to the logits; any row strides, the innermost one 1 (others are copied)."""
+    V = _check_logits("token_logprobs", logits, targets, vocab, temperature)
+    if targets.numel() and _kernels(logits):
+        return _TokenLogprobs.apply(logits, targets, V, ignore_index, float(temperature))
+    return _token_parts(logits, targets, ignore_index, temperature, V)[2].view(targets.shape)
+
+
+# ---------------------------------------------------------------------------------------------------------- policy loss
+class _PolicyLoss(torch.autograd.Function):
+    """Loss and gradient from one pass; the backward pass multiplies the gradient where the loss's own is not 1."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature, args, constants, want_grad):
+        from ..ops import _objectives as O
+        with torch.cuda.device(logits.device):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            grad = O.empty_grad(logits) if want_grad else None
+            out = O.policy_loss(rows, args, logits.device, grad)
+        ctx.save_for_backward(grad)
+        loss, logp, kl, entropy = (t.view(targets.shape) if i else t for i, t in enumerate(out))
+        ctx.mark_non_differentiable(logp, kl, entropy)
+        return loss, logp, kl, entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, *_):
+        from ..ops import _objectives as O
+        (grad,) = ctx.saved_tensors
+        # a graph that is kept may be walked again, and then needs the gradient as it was
+        if torch._C._autograd._get_current_graph_task_keep_graph():
+            return ((grad.float() * dloss.float()).to(grad.dtype), *(None,) * 7)
+        with torch.cuda.device(grad.device):
+            O.scale_unless_one_(_memory_of(grad), dloss.float())
+        return (grad, *(None,) * 7)
+
+
+def _memory_of(t: torch.Tensor) -> torch.Tensor:
+    """The elements between the first and the last of a tensor as a vector."""
+    if t.is_contiguous():
+        return t.view(-1)
+    return t.as_strided((1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())),), (1,))
+
+
+def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
+                ref_logp: Optional[torch.Tensor] = None, clip_low: float = 0.2, clip_high: Optional[float] = None, kl_coef: float = 0.0,
+                kl: str = "k3", entropy_coef: float = 0.0, temperature: float = 1.0, reduction: str = "token", scale: float = 1.0,
+                ignore_index: int = -100, vocab: Optional[int] = None) -> PolicyLoss:
+    """Clipped policy loss of sampled tokens, from logits [B, T, V(+pad)] and their targets [B, T].
+
+    Per token, with r = exp(logp - old_logp) and A its advantage: ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef KL -
+    entropy_coef H``; KL is the estimate of the divergence from the reference (``ref_logp``) with d = ref_logp - logp: ``"k1"`` -d, ``"k2"``
+    d^2 / 2, ``"k3"`` exp(d) - d - 1.  ``advantages`` [B, T], or [B] for one per sequence.  ``reduction``: ``"token"`` the mean over all tokens
+    that count, ``"sequence"`` the mean over sequences (with such tokens) of the means over their tokens, ``"sum"``; times ``scale``.
+    ``old_logp``, ``ref_logp`` and the advantages are constants.
+
+    The gradient is made together with the loss, in one read of the logits; where the gradient of the loss itself is not 1 it is
+    multiplied afterwards, so the factor of an accumulated micro-batch is better given as ``scale``."""
+    name = "policy_loss"
+    V = _check_logits(name, logits, targets, vocab, temperature)
+    if targets.dim() != 2:
+        raise ValueError(f"{name}: logits must be [B, T, V] and targets [B, T]")
+    B, T = targets.shape
+    clip_high = clip_low if clip_high is None else clip_high
+    if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0 and math.isfinite(clip_high)):
+        raise ValueError(f"{name}: needs 0 <= clip_low <= 1 and clip_high >= 0")
+    if kl not in ("k1", "k2", "k3"):
+        raise ValueError(f"{name}: kl must be 'k1', 'k2' or 'k3'")
+    if reduction not in ("token", "sequence", "sum"):
+        raise ValueError(f"{name}: reduction must be 'token', 'sequence' or 'sum'")
+    if not all(math.isfinite(v) for v in (kl_coef, entropy_coef, scale)):
+        raise ValueError(f"{name}: kl_coef, entropy_coef and scale must be finite")
+    if kl_coef != 0.0 and ref_logp is None:
+        raise ValueError(f"{name}: a KL term needs ref_logp")
+    old = _check_values(name, "old_logp", old_logp, [(B, T)], logits.device)
+    adv = _check_values(name, "advantages", advantages, [(B, T), (B,)], logits.device)
+    ref = None if ref_logp is None else _check_values(name, "ref_logp", ref_logp, [(B, T)], logits.device)
+    if targets.numel() and _kernels(logits):
+        from ..ops import _objectives as O
+        a = O.PolicyArgs()
+        a.old_logp, a.advantages, a.ref_logp = old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr()
+        a.adv_per, a.seq_len = (T if adv.dim() == 1 else 1), T
+        a.clip_low, a.clip_high, a.kl_coef, a.entropy_coef, a.scale = clip_low, clip_high, kl_coef, entropy_coef, scale
+        a.kl, a.mean = O.KL[kl], O.MEAN[reduction]
+        want = torch.is_grad_enabled() and logits.requires_grad
+        return PolicyLoss(*_PolicyLoss.apply(logits, targets, V, ignore_index, float(temperature), a, (old, adv, ref), want))
+    keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
+    zero = torch.zeros((), dtype=lp.dtype, device=lp.device)
+    p = lp.exp()
+    ent = torch.where(keep, -torch.where(p > 0, p * lp, zero).sum(-1), zero)
+    old, adv = old.to(lp.dtype).reshape(-1), (adv if adv.dim() == 2 else adv[:, None].expand(B, T)).to(lp.dtype).reshape(-1)
+    ratio = torch.exp(logp - old)
+    gain = torch.minimum(ratio * adv, ratio.clamp(1.0 - clip_low, 1.0 + clip_high) * adv)
+    div = torch.zeros_like(logp)
+    if ref is not None:
+        d = ref.to(lp.dtype).reshape(-1) - logp
+        div = {"k1": -d, "k2": 0.5 * d * d, "k3": torch.expm1(d) - d}[kl]
+    per = torch.where(keep, kl_coef * div - gain - entropy_coef * ent, zero)
+    counts = keep.view(B, T).sum(-1)
+    if reduction == "token":
+        per = per / counts.sum().clamp(min=1)
+    elif reduction == "sequence":
+        per = per.view(B, T) / (counts.clamp(min=1)[:, None] * (counts > 0).sum().clamp(min=1))
+    loss = (per.double().sum() * scale).to(lp.dtype)
+    return PolicyLoss(loss, logp.detach().view(B, T), torch.where(keep, div, zero).detach().view(B, T), ent.detach().view(B, T))
+
+
+# ------------------------------------------------------------------------------------------------------ preference loss
+class _PreferenceLoss(torch.autograd.Function):
+    """Forward: one read of the logits, then the pairs' losses and slopes; backward: one read and one write."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature, ref, kind, average, beta, smoothing, target_margin):
+        from ..ops import _objectives as O
+        pairs = targets.shape[0] // 2
+        with torch.cuda.device(logits.device):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            logp, stats = O.token_logprobs(rows, logits.device)
+            loss, seq, margin, coef = O.preference_loss(logp, targets, ref, pairs, ignore_index, kind=kind, average=average, beta=beta,
+                                                        smoothing=smoothing, target_margin=target_margin)
+        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.cfg = (vocab, ignore_index, temperature)
+        ctx.mark_non_differentiable(seq, margin)
+        return loss, seq, margin
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, *_):
+        from ..ops import _objectives as O
+        logits, targets, stats, coef = ctx.saved_tensors
+        vocab, ignore_index, temperature = ctx.cfg
+        with torch.cuda.device(logits.device):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            grad = O.empty_grad(logits)
+            O.token_logprobs_grad(rows, stats, coef, targets.shape[1], dloss.float(), grad)
+        return (grad, *(None,) * 10)
+
+
+def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, beta: float = 0.1,
+                    kind: str = "sigmoid", label_smoothing: float = 0.0, target_margin: float = 0.0, average: bool = False,
+                    temperature: float = 1.0, ignore_index: int = -100, vocab: Optional[int] = None) -> PreferenceLoss:
+    """Preference loss over pairs of sequences: logits [2 P, T, V(+pad)] and targets [2 P, T], the P chosen sequences first, then the P
+    rejected ones in the same order (padding and prompts marked by `ignore_index`).
+
+    A sequence's log-probability is the sum over its tokens (their mean with ``average``), its log-ratio that minus ``ref_logp`` [2 P]
+    (none: without a reference), and with h the chosen log-ratio minus the rejected one and z = beta h - target_margin a pair's loss is
+    ``"sigmoid"``: -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z); ``"hinge"``: max(0, 1 - z); ``"ipo"``:
+    (h - 1 / (2 beta))^2.  The loss is the mean over the pairs."""
+    name = "preference_loss"
+    V = _check_logits(name, logits, targets, vocab, temperature)
+    if targets.dim() != 2 or targets.shape[0] < 2 or targets.shape[0] % 2:
+        raise ValueError(f"{name}: logits must be [2 P, T, V] and targets [2 P, T] with P >= 1 chosen sequences before P rejected ones")
+    if kind not in ("sigmoid", "hinge", "ipo"):
+        raise ValueError(f"{name}: kind must be 'sigmoid', 'hinge' or 'ipo'")
+    if not (math.isfinite(beta) and beta > 0.0):
+        raise ValueError(f"{name}: beta must be positive, got {beta}")
+    if not 0.0 <= label_smoothing < 0.5 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError(f"{name}: label_smoothing must be in [0, 0.5), and belongs to the sigmoid loss")
+    if not math.isfinite(target_margin) or (target_margin and kind == "ipo"):
+        raise ValueError(f"{name}: target_margin must be finite, and does not belong to the ipo loss")
+    pairs = targets.shape[0] // 2
+    ref = None if ref_logp is None else _check_values(name, "ref_logp", ref_logp, [(2 * pairs,)], logits.device)
+    if targets.numel() and _kernels(logits):
+        return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, V, ignore_index, float(temperature), ref, kind, bool(average),
+                                                     float(beta), float(label_smoothing), float(target_margin)))
+    keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
+    seq = logp.double().view(targets.shape).sum(-1)
+    if average:
+        seq = seq / keep.view(targets.shape).sum(-1).clamp(min=1)
+    ratio = seq if ref is None else seq - ref.double()
+    h = ratio[:pairs] - ratio[pairs:]
+    z = beta * h - target_margin
+    if kind == "sigmoid":
+        each = -torch.nn.functional.logsigmoid(z) + label_smoothing * z
+    elif kind == "hinge":
+        each = (1.0 - z).clamp(min=0.0)
+    else:
+        each = (h - 0.5 / beta) ** 2
+    return PreferenceLoss(each.mean().to(lp.dtype), seq.detach().to(lp.dtype), h.detach().to(lp.dtype))

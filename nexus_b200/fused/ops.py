@@ -612,3 +612,7 @@ def adamw_multi_tensor(params: Sequence[torch.Tensor], grads: Sequence[torch.Ten
             denom = (vi * float(inv2)).sqrt_().add_(float(np.float32(eps)))
             p.sub_((mi * float(inv1)) * float(lr_i) / denom)
     return norm
+
+
+# ------------------------------------------------------------------- fine-tuning on rewards and preferences
+from .objectives import PolicyLoss, PreferenceLoss, policy_loss, preference_loss, token_logprobs  # noqa: E402,F401

@@ -1,0 +1,135 @@
+"""ctypes bindings of the kernels that fine-tune a language model on rewards and preferences (``nx_api_objectives.h``): log-probabilities
+of given tokens, clipped policy loss, preference loss.  Workspaces are allocated per call: calls on several streams and captured graphs
+share nothing."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _cuda as K
+
+KL = {"k1": 0, "k2": 1, "k3": 2}
+MEAN = {"token": 0, "sequence": 1, "sum": 2}
+PREFERENCE = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+
+
+class TokenRows(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("targets", C.c_void_p), ("rows", C.c_int64), ("per", C.c_int64), ("stride_outer", C.c_int64),
+                ("stride_inner", C.c_int64), ("ignore_index", C.c_int64), ("dtype", C.c_int32), ("targets_wide", C.c_int32),
+                ("vocab", C.c_int32), ("width", C.c_int32), ("inv_temp", C.c_float), ("pad_", C.c_int32)]
+
+
+class PolicyArgs(C.Structure):
+    _fields_ = [("old_logp", C.c_void_p), ("ref_logp", C.c_void_p), ("advantages", C.c_void_p), ("adv_per", C.c_int64),
+                ("seq_len", C.c_int64), ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float),
+                ("entropy_coef", C.c_float), ("scale", C.c_float), ("kl", C.c_int32), ("mean", C.c_int32), ("write_grad", C.c_int32)]
+
+
+class PreferenceArgs(C.Structure):
+    _fields_ = [("logp", C.c_void_p), ("targets", C.c_void_p), ("ref_logp", C.c_void_p), ("pairs", C.c_int64), ("seq_len", C.c_int64),
+                ("ignore_index", C.c_int64), ("targets_wide", C.c_int32), ("kind", C.c_int32), ("average", C.c_int32), ("beta", C.c_float),
+                ("smoothing", C.c_float), ("target_margin", C.c_float)]
+
+
+def row_layout(x: torch.Tensor) -> Optional[Tuple[int, int, int]]:
+    """(rows of an inner run, stride between runs, stride inside a run) of the rows of x [..., W] in elements; None where the rows are not
+    of that form, overlap, or lie so far apart that a gradient of the same layout would waste more than it saves."""
+    W = x.shape[-1]
+    if x.numel() == 0 or (W > 1 and x.stride(-1) != 1):
+        return None
+    dims = []
+    for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
+        if size == 1:
+            continue
+        if dims and dims[-1][1] == size * stride:
+            dims[-1] = (dims[-1][0] * size, stride)
+        else:
+            dims.append((size, stride))
+    if len(dims) > 2:
+        return None
+    (no, so), (ni, si) = ([(1, 0)] * (2 - len(dims)) + dims)
+    if (ni > 1 and si < W) or (no > 1 and so < W):
+        return None
+    if no > 1 and ni > 1 and so < ni * si and si < no * so:
+        return None
+    if (no - 1) * so + (ni - 1) * si + W > 2 * no * ni * W:
+        return None
+    return ni, so, si
+
+
+def prepare_rows(logits: torch.Tensor, targets: torch.Tensor, vocab: int, ignore_index: int, inv_temp: float):
+    """(logits that the kernels read, their description).  The returned tensors must outlive the calls."""
+    lay = row_layout(logits)
+    if lay is None:
+        logits = logits.contiguous()
+        lay = (max(1, logits.numel() // max(1, logits.shape[-1])), 0, logits.shape[-1])
+    targets = targets.contiguous()
+    r = TokenRows()
+    r.logits, r.targets, r.rows = logits.data_ptr(), targets.data_ptr(), targets.numel()
+    r.per, r.stride_outer, r.stride_inner = lay
+    r.ignore_index, r.dtype, r.targets_wide = ignore_index, K._DT[logits.dtype], int(targets.dtype == torch.int64)
+    r.vocab, r.width, r.inv_temp = vocab, logits.shape[-1], inv_temp
+    return logits, targets, r
+
+
+def empty_grad(logits: torch.Tensor) -> torch.Tensor:
+    """A tensor of the layout of `logits` (as `prepare_rows` returned it) that starts at the same place of a 16-byte line."""
+    off = logits.data_ptr() % 16 // logits.element_size()
+    if logits.is_contiguous() and off == 0:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    extent = 1 + sum((n - 1) * s for n, s in zip(logits.shape, logits.stride()))
+    buf = torch.empty(extent + off, dtype=logits.dtype, device=logits.device)
+    return buf.as_strided(logits.shape, logits.stride(), off)
+
+
+def token_logprobs(rows: TokenRows, device):
+    """FP32 (logp [rows], stats [rows, 2])."""
+    logp = torch.empty(rows.rows, dtype=torch.float32, device=device)
+    stats = torch.empty((rows.rows, 2), dtype=torch.float32, device=device)
+    K._check(K.lib().nx_token_logprobs(C.byref(rows), K._p(logp), K._p(stats), K._stream()), "nx_token_logprobs")
+    return logp, stats
+
+
+def token_logprobs_grad(rows: TokenRows, stats, coef, coef_per: int, factor, grad) -> None:
+    K._check(K.lib().nx_token_logprobs_grad(C.byref(rows), K._p(stats), K._p(coef), C.c_int64(coef_per), K._p(factor), K._p(grad),
+                                            K._stream()), "nx_token_logprobs_grad")
+
+
+def policy_loss(rows: TokenRows, args: PolicyArgs, device, grad):
+    """FP32 (loss, logp, kl, entropy); `grad` (or None) is written."""
+    n = rows.rows
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    per_row = torch.empty((4, n), dtype=torch.float32, device=device)
+    sequences = n // args.seq_len
+    totals = torch.empty(2 + (sequences + 1) // 2, dtype=torch.float64, device=device)
+    args.write_grad = int(grad is not None)
+    K._check(K.lib().nx_policy_loss(C.byref(rows), C.byref(args), K._p(totals), C.c_void_p(totals.data_ptr() + 16), K._p(per_row[0]),
+                                    K._p(per_row[1]), K._p(per_row[2]), K._p(per_row[3]), K._p(loss), K._p(grad), K._stream()),
+             "nx_policy_loss")
+    return loss, per_row[0], per_row[1], per_row[2]
+
+
+def scale_unless_one_(x: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
+    """x *= factor in place (x dense, factor one FP32 value on the device); where the factor is 1, nothing is read or written."""
+    K._check(K.lib().nx_scale_unless_one(K._p(x), K._p(factor), C.c_int(K._DT[x.dtype]), C.c_int64(x.numel()), K._stream()),
+             "nx_scale_unless_one")
+    return x
+
+
+def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, kind: str, average: bool, beta: float, smoothing: float,
+                    target_margin: float):
+    """FP32 (loss, logp of the sequences [2 * pairs], margin [pairs], coef [2 * pairs])."""
+    dev = logp.device
+    a = PreferenceArgs()
+    a.logp, a.targets, a.pairs, a.seq_len = logp.data_ptr(), targets.data_ptr(), pairs, targets.numel() // (2 * pairs)
+    a.ref_logp = None if ref_logp is None else ref_logp.data_ptr()
+    a.ignore_index, a.targets_wide, a.kind, a.average = ignore_index, int(targets.dtype == torch.int64), PREFERENCE[kind], int(average)
+    a.beta, a.smoothing, a.target_margin = beta, smoothing, target_margin
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    out = torch.empty(5 * pairs, dtype=torch.float32, device=dev)
+    seq_logp, margin, coef = out[: 2 * pairs], out[2 * pairs: 3 * pairs], out[3 * pairs:]
+    K._check(K.lib().nx_preference_loss(C.byref(a), K._p(seq_logp), K._p(margin), K._p(coef), K._p(loss), K._stream()),
+             "nx_preference_loss")
+    return loss, seq_logp, margin, coef

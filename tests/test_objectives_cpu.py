@@ -1,0 +1,86 @@
+"""The plain forms of the objectives (gradients against differences in 64 bits) and what the entry points refuse."""
+import math
+
+import pytest
+import torch
+
+from nexus_b200.fused import ops as F
+
+
+def inputs(B=4, T=5, W=17, V=15):
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(B, T, W, dtype=torch.float64, generator=g, requires_grad=True)
+    t = torch.randint(0, V, (B, T), generator=g)
+    t[0, :2] = -100
+    t[B - 1] = -100
+    const = [torch.randn(B, T, generator=g) * 0.1 - 3 for _ in range(2)]
+    return x, t, *const, torch.randn(B, generator=g)
+
+
+def test_gradients_against_differences():
+    x, t, old, ref, adv = inputs()
+    assert torch.autograd.gradcheck(lambda x: F.token_logprobs(x, t, vocab=15, temperature=0.7), x)
+    for reduction in ("token", "sequence", "sum"):
+        for kl in ("k1", "k2", "k3"):
+            assert torch.autograd.gradcheck(lambda x: F.policy_loss(x, t, old, adv, ref, kl_coef=0.1, kl=kl, entropy_coef=0.02,
+                                                                    reduction=reduction, vocab=15).loss, x)
+    for kind in ("sigmoid", "hinge", "ipo"):
+        assert torch.autograd.gradcheck(lambda x: F.preference_loss(x, t, adv, kind=kind, average=True, vocab=15).loss, x)
+
+
+def test_policy_clips():
+    """Advantage of each sign at ratios inside and outside the borders: value and slope by hand."""
+    V = 4
+    x = torch.zeros(1, 6, V, dtype=torch.float64, requires_grad=True)
+    t = torch.zeros(1, 6, dtype=torch.long)
+    ratios = torch.tensor([[0.5, 1.0, 1.5, 0.5, 1.0, 1.5]], dtype=torch.float64)
+    adv = torch.tensor([[1.0, 1.0, 1.0, -1.0, -1.0, -1.0]])
+    old = math.log(0.25) - torch.log(ratios)
+    r = F.policy_loss(x, t, old.double(), adv, clip_low=0.2, clip_high=0.3, reduction="sum")
+    assert float(r.loss.detach()) == pytest.approx(-0.5 - 1.0 - 1.3 + 0.8 + 1.0 + 1.5, abs=1e-6)
+    r.loss.backward()
+    slope = x.grad[0, :, 0] / 0.75
+    assert slope.tolist() == pytest.approx([-0.5, -1.0, 0.0, 0.0, 1.0, 1.5], abs=1e-6)
+
+
+def test_ignored_and_bad_targets():
+    x = torch.randn(2, 3, 8)
+    x[0, 0] = math.nan
+    x.requires_grad_(True)
+    t = torch.tensor([[-100, 1, 2], [8, -1, 3]])
+    logp = F.token_logprobs(x, t)
+    assert float(logp[0, 0].detach()) == 0.0 and torch.isnan(logp).tolist() == [[False] * 3, [True, True, False]]
+    logp.sum().backward()
+    assert bool((x.grad[0, 0] == 0).all()) and bool((x.grad[1, :2] == 0).all())
+    assert math.isnan(float(F.policy_loss(x, t, torch.zeros(2, 3), torch.ones(2)).loss.detach()))
+
+
+def test_refusals():
+    x, t, old, ref, adv = inputs()
+    lp, pol, pref = F.token_logprobs, F.policy_loss, F.preference_loss
+    bad = [
+        lambda: lp(x.long(), t), lambda: lp(x, t.float()), lambda: lp(x, t[:, :-1]), lambda: lp(x, t, vocab=18), lambda: lp(x, t, vocab=0),
+        lambda: lp(x, t, temperature=0.0), lambda: lp(x, t, temperature=math.inf), lambda: lp(x, t, temperature=-1.0),
+        lambda: pol(x[0], t[0], old[0], adv), lambda: pol(x, t, old[:, :-1], adv), lambda: pol(x, t, old, adv[:-1]), lambda: pol(x, t, old, 1.0),
+        lambda: pol(x, t, old.long(), adv), lambda: pol(x, t, old, adv, kl_coef=0.1), lambda: pol(x, t, old, adv, ref[:1], kl_coef=0.1),
+        lambda: pol(x, t, old, adv, ref, kl="kl"), lambda: pol(x, t, old, adv, reduction="mean"), lambda: pol(x, t, old, adv, clip_low=-0.1),
+        lambda: pol(x, t, old, adv, clip_low=1.1), lambda: pol(x, t, old, adv, clip_high=math.inf), lambda: pol(x, t, old, adv, scale=math.nan),
+        lambda: pref(x[:3], t[:3]), lambda: pref(x[0], t[0]), lambda: pref(x, t, adv[:2]), lambda: pref(x, t, kind="dpo"), lambda: pref(x, t, beta=0.0),
+        lambda: pref(x, t, label_smoothing=0.5), lambda: pref(x, t, kind="hinge", label_smoothing=0.1), lambda: pref(x, t, kind="ipo", target_margin=1.0),
+        lambda: pref(x[:0], t[:0]),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_row_layouts():
+    """The rows of these views are read where they are; the others are copied first."""
+    from nexus_b200.ops._objectives import row_layout
+    x = torch.empty(4, 6, 64)
+    assert row_layout(x) == (24, 0, 64)
+    assert row_layout(x[:, 1:]) == (5, 384, 64) and row_layout(x[..., :50]) == (24, 0, 64)
+    assert row_layout(x.transpose(0, 1)) == (4, 64, 384)
+    assert row_layout(x[0, 0])[0] == 1 and row_layout(x.view(4, 3, 2, 64)[:, :, 1]) == (12, 0, 128)
+    for copied in (x[..., ::2], x[:, :1].expand(4, 6, 64), x[:, -1:], x[..., :20], x.view(4, 3, 2, 64)[:, :2, :1], torch.empty(0, 3, 4)):
+        assert row_layout(copied) is None
