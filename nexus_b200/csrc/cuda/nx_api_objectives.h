@@ -61,6 +61,20 @@ typedef struct NxPreferenceArgs {
 // seq_logp [2 * pairs], margin [pairs], coef [2 * pairs] = d loss / d logp of each counted token, loss: one float
 int nx_preference_loss(const NxPreferenceArgs* args, float* seq_logp, float* margin, float* coef, float* loss, nx_stream_t stream);
 
+// Gradients of `tensors` tensors (host arrays): count elements at src, of NxDType `type & 15`; the clipped ones go to dst, of type `type >> 4`
+// (dst null: in place, both types the same).
+typedef struct NxGradTable {
+  const void* const* src;
+  void* const* dst;
+  const int64_t* count;
+  const uint8_t* type;
+  int64_t tensors;
+} NxGradTable;
+int64_t nx_grad_clip_partials(int64_t tensors);  // doubles of scratch
+// out[0] = sum of squares; (float*)(out + 1) = norm = sqrt of it.  clip: the gradients times min(1, max_norm / (norm + 1e-6)); where the norm
+// is not finite they stay (dst: are copied) as they are.  Sums in a fixed order.
+int nx_grad_clip(const NxGradTable* table, double max_norm, int clip, double* partial, double* out, nx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -301,3 +301,157 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optio
     else:
         each = (h - 0.5 / beta) ** 2
     return PreferenceLoss(each.mean().to(lp.dtype), seq.detach().to(lp.dtype), h.detach().to(lp.dtype))
+
+
+# --------------------------------------------------------------------------------------------- gradients of many tensors
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill their memory without gaps or overlap, in whatever order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _spans(ts) -> List[tuple]:
+    return [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts]
+
+
+def _grad_list(name: str, grads, out):
+    """The tensors that count, without None, empty ones and repetitions; with `out`, the tensors their clipped values go to."""
+    grads = list(grads) if not torch.is_tensor(grads) else [grads]
+    if out is not None:
+        out = list(out) if not torch.is_tensor(out) else [out]
+        if len(out) != len(grads):
+            raise ValueError(f"{name}: {len(grads)} gradients and {len(out)} outputs")
+        pairs = [(g, o) for g, o in zip(grads, out) if g is not None]
+        grads, out = [g for g, _ in pairs], [o for _, o in pairs]
+    else:
+        grads = [g for g in grads if g is not None]
+    for t in grads if out is None else grads + out:
+        if not torch.is_tensor(t) or t.layout != torch.strided or not t.is_floating_point():
+            raise ValueError(f"{name}: takes dense floating-point tensors")
+        if t.device != grads[0].device:
+            raise ValueError(f"{name}: tensors on {t.device} and {grads[0].device}")
+    if out is not None:
+        for g, o in zip(grads, out):
+            if g.shape != o.shape:
+                raise ValueError(f"{name}: output {tuple(o.shape)} of a gradient {tuple(g.shape)}")
+    return grads, out
+
+
+def _separate(name: str, grads, out):
+    """Drops tensors listed twice (tied weights: they count and are clipped once); refuses other overlaps of memory."""
+    loose = {i for i, g in enumerate(grads) if not _dense(g)}  # views with gaps may interleave: only repetitions are looked for
+    seen, twice = {}, set()
+    for i in loose:
+        g = grads[i]
+        if seen.setdefault((g.data_ptr(), g.shape, g.stride(), g.dtype), i) != i:
+            twice.add(i)
+    spans = _spans(grads)
+    order = sorted((i for i in range(len(spans)) if i not in loose), key=spans.__getitem__)
+    for a, b in zip(order, order[1:]):
+        if spans[b][0] < spans[a][1]:
+            if spans[a] != spans[b] or grads[a].stride() != grads[b].stride() or grads[a].dtype != grads[b].dtype:
+                raise ValueError(f"{name}: two gradients share a part of their memory")
+            twice.add(b)
+    if out is not None:
+        if twice:
+            raise ValueError(f"{name}: a gradient is listed twice, with an output each")
+        every = sorted([(s, 0, i) for i, s in enumerate(spans) if i not in loose] + [(s, 1, i) for i, s in enumerate(_spans(out)) if _dense(out[i])])
+        for (s, ka, ia), (u, kb, ib) in zip(every, every[1:]):
+            if u[0] < s[1] and not (ka != kb and ia == ib and s == u and grads[ia].dtype == out[ia].dtype):
+                raise ValueError(f"{name}: an output shares memory with another tensor")
+    if twice:
+        grads = [g for i, g in enumerate(grads) if i not in twice]
+    return grads
+
+
+def _square_sum_plain(grads) -> float:
+    sq = 0.0
+    for g in grads:
+        sq += float(g.double().pow(2).sum())
+    return sq
+
+
+def _kernel_list(grads) -> bool:
+    return bool(grads) and all(g.dtype in _KERNEL_TYPES for g in grads) and _kernels(grads[0])
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    return t if _dense(t) else t.contiguous()
+
+
+def grad_square_sum(grads: Sequence[Optional[torch.Tensor]]) -> float:
+    """Sum of squares of all elements in FP64, on the host (one synchronisation): the square of the global gradient norm."""
+    grads, _ = _grad_list("grad_square_sum", grads, None)
+    if not _kernel_list(grads):
+        return _square_sum_plain(grads)
+    from ..ops import _objectives as O
+    with torch.cuda.device(grads[0].device):
+        ts = [_packed(g) for g in grads if g.numel()]
+        return float(O.grad_clip(ts, None)[0]) if ts else 0.0
+
+
+def clip_grads(name: str, grads, max_norm: float, out=None):
+    """`clip_grad_norm_` with the FP64 sum of squares beside the FP32 norm."""
+    if not max_norm >= 0.0:
+        raise ValueError(f"{name}: max_norm must not be negative, got {max_norm}")
+    grads, out = _grad_list(name, grads, out)
+    if not grads:
+        return torch.zeros((), dtype=torch.float64), torch.zeros((), dtype=torch.float32)
+    with torch.no_grad():
+        every = [t for t in (grads if out is None else grads + out) if t.numel()]
+        for t in every:
+            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise ValueError(f"{name}: a tensor whose elements share memory (expanded) cannot be clipped")
+        if out is not None:
+            kept = [(g, o) for g, o in zip(grads, out) if g.numel()]
+            full, outs = [g for g, _ in kept], [o for _, o in kept]
+        else:
+            full, outs = [g for g in grads if g.numel()], None
+        if not full:
+            return tuple(torch.zeros((), dtype=dt, device=grads[0].device) for dt in (torch.float64, torch.float32))
+        full = _separate(name, full, outs)
+        if _kernel_list(full) and (outs is None or all(o.dtype in _KERNEL_TYPES for o in outs)):
+            from ..ops import _objectives as O
+            with torch.cuda.device(full[0].device):
+                src = [_packed(g) for g in full]
+                if outs is None:
+                    norms = O.grad_clip(src, max_norm)
+                    torch.autograd.graph.increment_version(src)
+                    for g, s in zip(full, src):
+                        if s is not g:
+                            g.copy_(s)
+                    return norms
+                # element order of the memory: an output of another order than its gradient is written through a copy of that order
+                dst = [o if o.stride() == s.stride() else torch.empty_like(s, dtype=o.dtype) for o, s in zip(outs, src)]
+                norms = O.grad_clip(src, max_norm, dst)
+                torch.autograd.graph.increment_version(dst)
+                for o, d in zip(outs, dst):
+                    if d is not o:
+                        o.copy_(d)
+                return norms
+        sq = _square_sum_plain(full)
+        norm = math.sqrt(sq)
+        coef = min(1.0, max_norm / (norm + 1e-6)) if math.isfinite(norm) else 1.0
+        for i, g in enumerate(full):
+            if outs is not None:
+                outs[i].copy_(g if coef == 1.0 else g * coef)
+            elif coef != 1.0:
+                g.mul_(coef)
+        return torch.tensor(sq, dtype=torch.float64), torch.tensor(norm, dtype=torch.float32, device=full[0].device)
+
+
+def clip_grad_norm_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Clips gradients by their global norm |g| = sqrt(sum of the squares of all elements): every one times
+    ``min(1, max_norm / (|g| + 1e-6))``, in place, or written to the tensors ``out`` (of the same shapes; their type may be another).
+    Returns |g| as an FP32 scalar on the tensors' device, without a synchronisation; where it is not finite the gradients stay as they are
+    (and are copied to ``out``), for the caller to skip the step.
+
+    ``grads``: BF16, FP16 and FP32 tensors of one device in any mixture; None is left out, a tensor listed twice counts and is clipped once.
+    Two launches per 256 tensors; nothing is written in place where the norm is small enough."""
+    return clip_grads("clip_grad_norm_", grads, max_norm, out)[1]

@@ -582,9 +582,7 @@ def adamw_multi_tensor(params: Sequence[torch.Tensor], grads: Sequence[torch.Ten
     Returns the global gradient norm.  ``grad_sq_sum`` overrides the local square sum (sharded callers).
     """
     if grad_sq_sum is None:
-        sq = 0.0
-        for g in grads:
-            sq += float(g.double().pow(2).sum())
+        sq = grad_square_sum(grads)
     else:
         sq = grad_sq_sum
     norm = math.sqrt(sq)
@@ -615,4 +613,5 @@ def adamw_multi_tensor(params: Sequence[torch.Tensor], grads: Sequence[torch.Ten
 
 
 # ------------------------------------------------------------------- fine-tuning on rewards and preferences
-from .objectives import PolicyLoss, PreferenceLoss, policy_loss, preference_loss, token_logprobs  # noqa: E402,F401
+from .objectives import (PolicyLoss, PreferenceLoss, clip_grad_norm_, grad_square_sum, policy_loss, preference_loss,  # noqa: E402,F401
+                         token_logprobs)

@@ -4,6 +4,7 @@ share nothing."""
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from typing import Optional, Tuple
 
 import torch
@@ -133,3 +134,32 @@ def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, k
     K._check(K.lib().nx_preference_loss(C.byref(a), K._p(seq_logp), K._p(margin), K._p(coef), K._p(loss), K._stream()),
              "nx_preference_loss")
     return loss, seq_logp, margin, coef
+
+
+# ---------------------------------------------------------------------------------------------------- gradients of many tensors
+class GradTable(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("count", C.c_void_p), ("type", C.c_void_p), ("tensors", C.c_int64)]
+
+
+def grad_clip(grads, max_norm: Optional[float], out=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(FP64 sum of squares, FP32 norm) of dense, non-empty tensors; with `max_norm` they are clipped, in place or into `out`."""
+    n = len(grads)
+    src = array("Q", map(torch.Tensor.data_ptr, grads))
+    count = array("q", map(torch.Tensor.numel, grads))
+    if out is None:
+        types = bytes([17 * K._DT[t.dtype] for t in grads])
+        dst = None
+    else:
+        types = bytes([K._DT[t.dtype] | K._DT[o.dtype] << 4 for t, o in zip(grads, out)])
+        dst = array("Q", map(torch.Tensor.data_ptr, out))
+    L = K.lib()
+    parts = int(L.nx_grad_clip_partials(C.c_int64(n)))
+    buf = torch.empty(2 + parts, dtype=torch.float64, device=grads[0].device)
+    a = GradTable()
+    a.src, a.count, a.tensors = src.buffer_info()[0], count.buffer_info()[0], n
+    a.dst = None if dst is None else dst.buffer_info()[0]
+    a.type = C.cast(C.c_char_p(types), C.c_void_p).value
+    at = buf.data_ptr()
+    K._check(L.nx_grad_clip(C.byref(a), C.c_double(0.0 if max_norm is None else max_norm), C.c_int(int(max_norm is not None)),
+                            C.c_void_p(at + 16), C.c_void_p(at), K._stream()), "nx_grad_clip")
+    return buf[0], buf[1:2].view(torch.float32)[0]

@@ -17,6 +17,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 import numpy as np
 import torch
 
+from ..fused.objectives import clip_grads, grad_square_sum
 from ..loss import CrossEntropy
 from ..metrics import Accuracy
 from ..optim import SGD, AdamW
@@ -134,18 +135,17 @@ class Trainer:
         inv = 1.0 / (window * (self.scaler.scale if self.scaler else 1.0))
         for p in params:
             p.grad.mul_(inv)
-        sq = sum(float(p.grad.double().pow(2).sum()) for p in params)
+        grads = [p.grad for p in params]
+        if self.clip > 0:      # gradients whose norm is not finite stay as they are: the step is skipped below
+            sq = float(clip_grads("Trainer", grads, self.clip)[0])
+        else:
+            sq = grad_square_sum(grads)
         if not math.isfinite(sq):
             if self.scaler:
                 self.scaler.on_overflow()
             self.skipped_steps += 1
             self.optimizer.zero_grad()
             return
-        if self.clip > 0:
-            coef = min(1.0, self.clip / (math.sqrt(sq) + 1e-6))
-            if coef < 1.0:
-                for p in params:
-                    p.grad.mul_(coef)
         if self.step_schedule is not None:
             self.optimizer.lr = self.base_lr * self.step_schedule.factor(self.global_step)
         self.optimizer.step()

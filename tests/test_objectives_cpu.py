@@ -84,3 +84,35 @@ def test_row_layouts():
     assert row_layout(x[0, 0])[0] == 1 and row_layout(x.view(4, 3, 2, 64)[:, :, 1]) == (12, 0, 128)
     for copied in (x[..., ::2], x[:, :1].expand(4, 6, 64), x[:, -1:], x[..., :20], x.view(4, 3, 2, 64)[:, :2, :1], torch.empty(0, 3, 4)):
         assert row_layout(copied) is None
+
+
+def test_clip_on_the_host():
+    g = torch.Generator().manual_seed(3)
+    make = lambda: [torch.randn(n, generator=g) for n in (1, 7, 40)] + [torch.randn(5, 6, generator=g).t(), torch.randn(3, 8, generator=g)[:, :5]]  # noqa: E731
+    gs = make()
+    want = math.sqrt(sum(float(t.double().pow(2).sum()) for t in gs))
+    keep = [t.clone() for t in gs]
+    assert F.grad_square_sum(gs) == pytest.approx(want * want, rel=1e-14)
+    norm = F.clip_grad_norm_(gs + [None, torch.zeros(0)], 1.5)
+    assert norm.dtype == torch.float32 and float(norm) == pytest.approx(want, rel=2 ** -24)
+    for a, b in zip(gs, keep):
+        assert torch.allclose(a, b * (1.5 / (want + 1e-6)), rtol=2 ** -22, atol=0)
+    outs = [torch.empty(t.shape, dtype=torch.bfloat16) for t in keep]
+    F.clip_grad_norm_(keep, 1e9, out=outs)
+    assert all(torch.equal(o, k.bfloat16()) for o, k in zip(outs, keep))
+    bad = [torch.tensor([1.0, math.inf]), torch.tensor([2.0])]
+    assert math.isinf(float(F.clip_grad_norm_(bad, 1.0))) and bad[1].item() == 2.0
+    tied = torch.ones(4)
+    assert float(F.clip_grad_norm_([tied, tied], 1.0)) == 2.0 and float(tied[0]) == pytest.approx(0.5, rel=1e-5)
+    assert float(F.clip_grad_norm_([], 1.0)) == 0.0 and float(F.clip_grad_norm_([torch.zeros(0)], 1.0)) == 0.0
+
+
+def test_clip_refusals():
+    a, b = torch.ones(6), torch.ones(6)
+    for call in (lambda: F.clip_grad_norm_([a], -1.0), lambda: F.clip_grad_norm_([a], math.nan), lambda: F.clip_grad_norm_([a.long()], 1.0),
+                 lambda: F.clip_grad_norm_([a], 1.0, out=[b, b]), lambda: F.clip_grad_norm_([a], 1.0, out=[torch.ones(5)]),
+                 lambda: F.clip_grad_norm_([a[:4], a[2:]], 1.0), lambda: F.clip_grad_norm_([torch.ones(1).expand(4)], 1.0),
+                 lambda: F.clip_grad_norm_([a, b], 1.0, out=[b, torch.ones(6)]), lambda: F.clip_grad_norm_([a, b], 1.0, out=[torch.ones(6)] + [a]),
+                 lambda: F.clip_grad_norm_([a, a], 1.0, out=[torch.ones(6), torch.ones(6)]), lambda: F.clip_grad_norm_([a.to_sparse()], 1.0)):
+        with pytest.raises(ValueError):
+            call()
