@@ -1,0 +1,817 @@
+// Log-probabilities of given tokens from hidden states and the weight of a language model's head, and their gradients, without the logits in
+// memory:
+//
+//   x = h W^T * inv_temp,   logp_r = x_rt - logsumexp_v x_rv,   G_rv = c_r inv_temp (delta_vt - p_rv),   dh = G W,   dW = G^T h
+//
+// Four products on one persistent CTA-pair kernel (tcgen05, 256 x 256 tiles over two SMs, operands by TMA, two accumulators in tensor memory):
+//   stats   h W^T, whose epilogue leaves the largest logit and the sum of exponentials of each row and 128 columns (8 bytes instead of 512)
+//           and the target's logit; a join over the vocabulary follows
+//   grad    h W^T again, whose epilogue turns the logits into G in 16 bits: the gradient costs one product more than with stored logits, and
+//           G of a bounded number of rows is all that is ever in memory
+//   dh, dW  G W and G^T h
+// Rows whose target does not count are left out before the first product: the others are brought together in order (their number stays on the
+// device and bounds every loop), so that prompts and padding cost no tensor-core time.  A tile is 256 rows: without a gradient, up to that
+// many rows stay where they are (with one they would put 0 * h of a row that does not count into dW, and h may hold anything there).
+//
+// G is rounded to the operands' type, as the tensor cores take it.  FP16 has no room for c p below 2^-24: G is multiplied by the power of two
+// that takes the largest |c| to at most 2^15, and the products by its inverse.
+#include "common.cuh"
+#include "nx_api_objectives.h"
+#include "sm100_ptx.cuh"
+#include "tensor_map.h"
+
+#include <algorithm>
+
+namespace {
+using namespace nx;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kBM = 128, kTile = 256, kBK = 64;
+constexpr int kThreads = 320;  // warp 0: TMA, warp 1: MMA, warps 2..9: epilogue (two per quarter of the tensor memory's lanes)
+constexpr int kOperandBytes = 128 * kBK * 2, kStageBytes = 2 * kOperandBytes, kStages = 5, kSlots = 4;
+constexpr int kStoreBytes = 8 * kSlots * 2048;
+constexpr int kSmemBytes = kStages * kStageBytes + kStoreBytes + 256;
+constexpr int kTmemCols = 512;
+
+enum Mode { kStats = 0, kGrad = 1, kInputGrad = 2, kWeightGrad = 3 };
+
+struct Params {
+  int64_t rows;             // of the whole call
+  int64_t row0, cap;        // this launch: rows [row0, row0 + cap) of those that count
+  const int32_t* count;     // how many count (null: all)
+  const int32_t* index;     // where the r-th of them is (null: r)
+  const void* targets;
+  int64_t ignore;
+  int targets_wide;
+  int vocab, width;         // columns of the logits; columns of h
+  int group;                // stats, grad: row tiles that pass over the vocabulary together
+  int slices, blocks_per_slice;  // input gradient: pieces of the vocabulary
+  float inv_temp;
+  float2* part;             // stats: [2 * column tiles][part_ld]
+  int64_t part_ld;
+  float* tlogit;
+  const float2* stats;      // grad
+  const float* coef;
+  const float* scale;       // FP16: {2^e, 2^-e}; null: 1
+  void* out;                // input gradient: rows of pitch out_ld; weight gradient in FP32
+  float* partial;           // input gradient of several slices: [slice][cap][width]
+  int64_t out_ld;
+  int add;                  // weight gradient: add to the FP32 rows
+  int* status;
+};
+
+__device__ __forceinline__ int64_t live_rows(const Params& p) {
+  const int64_t n = (p.count != nullptr ? static_cast<int64_t>(*p.count) : p.rows) - p.row0;
+  return n < 0 ? 0 : (n < p.cap ? n : p.cap);
+}
+__device__ __forceinline__ int64_t place(const Params& p, int64_t row) { return p.index != nullptr ? p.index[p.row0 + row] : p.row0 + row; }
+__device__ __forceinline__ int64_t target_of(const void* targets, int wide, int64_t at) {
+  return wide ? reinterpret_cast<const int64_t*>(targets)[at] : static_cast<int64_t>(reinterpret_cast<const int32_t*>(targets)[at]);
+}
+
+struct Unit {
+  int m0, n0, kb_begin, kb_end, slice;
+};
+struct Extent {
+  int tiles_m, tiles_n, kb, units;
+};
+template <int MODE>
+__device__ __forceinline__ Extent extent(const Params& p, int live) {
+  Extent e;
+  if (MODE == kStats || MODE == kGrad) {
+    e.tiles_m = (live + kTile - 1) / kTile;
+    e.tiles_n = (p.vocab + kTile - 1) / kTile;
+    e.kb = (p.width + kBK - 1) / kBK;
+  } else if (MODE == kInputGrad) {
+    e.tiles_m = (live + kTile - 1) / kTile;
+    e.tiles_n = (p.width + kTile - 1) / kTile;
+    e.kb = (p.vocab + kBK - 1) / kBK;
+  } else {
+    e.tiles_m = (p.vocab + kTile - 1) / kTile;
+    e.tiles_n = (p.width + kTile - 1) / kTile;
+    e.kb = (live + kBK - 1) / kBK;
+  }
+  e.units = e.tiles_m * e.tiles_n * (MODE == kInputGrad ? p.slices : 1);
+  return e;
+}
+template <int MODE>
+__device__ __forceinline__ Unit unit_at(const Params& p, const Extent& e, int u) {
+  Unit w;
+  int tm, tn;
+  w.slice = 0;
+  w.kb_begin = 0;
+  w.kb_end = e.kb;
+  if (MODE == kStats || MODE == kGrad) {
+    // a group of row tiles stays in L2 while the weight passes by once
+    const int per = p.group * e.tiles_n, g = u / per, in = u - g * per;
+    const int rows = min(p.group, e.tiles_m - g * p.group);
+    tn = in / rows;
+    tm = g * p.group + in - tn * rows;
+  } else {
+    tn = u % e.tiles_n;
+    u /= e.tiles_n;
+    tm = u % e.tiles_m;
+    if (MODE == kInputGrad) {
+      w.slice = u / e.tiles_m;
+      w.kb_begin = w.slice * p.blocks_per_slice;
+      w.kb_end = min(e.kb, w.kb_begin + p.blocks_per_slice);
+    }
+  }
+  w.m0 = tm * kTile;
+  w.n0 = tn * kTile;
+  return w;
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF) return pack_bf16x2(a, b);
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+// one row of a [32][32] staging tile in the 64-byte swizzle of its tensor map
+template <bool BF>
+__device__ __forceinline__ void stage_row(uint8_t* buf, int r, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 q;
+    q.x = pack2<BF>(v[8 * i], v[8 * i + 1]);
+    q.y = pack2<BF>(v[8 * i + 2], v[8 * i + 3]);
+    q.z = pack2<BF>(v[8 * i + 4], v[8 * i + 5]);
+    q.w = pack2<BF>(v[8 * i + 6], v[8 * i + 7]);
+    *reinterpret_cast<uint4*>(buf + r * 64 + ((i ^ ((r >> 1) & 3)) << 4)) = q;
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int MODE, bool BF>
+__global__ void __launch_bounds__(kThreads, 1)
+head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
+            const Params p, const uint32_t idesc) {
+  constexpr bool kAmn = MODE == kWeightGrad, kBmn = MODE == kInputGrad || MODE == kWeightGrad;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzle needs it; the same in both CTAs
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, kStatusBadArgument);
+    return;
+  }
+  uint8_t* const store_base = smem + kStages * kStageBytes;
+  uint64_t* const full_bar = reinterpret_cast<uint64_t*>(store_base + kStoreBytes);
+  uint64_t* const empty_bar = full_bar + kStages;
+  uint64_t* const tfull_bar = empty_bar + kStages;
+  uint64_t* const tempty_bar = tfull_bar + 2;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta_rank = cluster_ctarank();
+  const int unit_first = static_cast<int>(blockIdx.x >> 1), unit_step = static_cast<int>(gridDim.x >> 1);
+  const int m_off = static_cast<int>(cta_rank) * kBM;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 16);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  cluster_sync_all();
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int live = static_cast<int>(live_rows(p));
+  Extent e = extent<MODE>(p, live);
+  if (MODE == kWeightGrad && p.add && live == 0) e.units = 0;  // nothing to add
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = unit_first; u < e.units && ok; u += unit_step) {
+        const Unit w = unit_at<MODE>(p, e, u);
+        const int m0 = w.m0 + m_off, bn0 = w.n0 + static_cast<int>(cta_rank) * 128;
+        for (int kb = w.kb_begin; kb < w.kb_end; ++kb) {
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            atomicCAS(p.status, 0, kStatusTimeoutProducer);
+            break;
+          }
+          uint8_t* sa = smem + stage * kStageBytes;
+          uint8_t* sb = sa + kOperandBytes;
+          const int k0 = kb * kBK;
+          // both CTAs' bytes are counted on the even CTA's barrier
+          if (cta_rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
+          const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          if constexpr (!kAmn) {
+            tma_load_3d_pair(sa, &map_a, bar, k0, m0, 0);
+          } else {
+            tma_load_3d_pair(sa, &map_a, bar, m0, k0, 0);
+            tma_load_3d_pair(sa + 64 * kBK * 2, &map_a, bar, m0 + 64, k0, 0);
+          }
+          if constexpr (!kBmn) {
+            tma_load_3d_pair(sb, &map_b, bar, k0, bn0, 0);
+          } else {
+            tma_load_3d_pair(sb, &map_b, bar, bn0, k0, 0);
+            tma_load_3d_pair(sb + 64 * kBK * 2, &map_b, bar, bn0 + 64, k0, 0);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // The even CTA's commits also arrive on this CTA's barriers: every stage filled here has been released before the CTA leaves.
+      for (int s = 0; s < kStages && ok; ++s) {
+        ok = mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag);
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (cta_rank == 0) {
+      const bool leader = elect_one();
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int u = unit_first; u < e.units && ok; u += unit_step) {
+        const Unit w = unit_at<MODE>(p, e, u);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u, abort_flag))) {
+          if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kTile);
+        for (int kb = w.kb_begin; kb < w.kb_end; ++kb) {
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[stage], phase, abort_flag))) {
+            ok = false;
+            if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t sa = smem_u32(smem + stage * kStageBytes), sb = sa + kOperandBytes;
+          const uint64_t da0 = make_smem_desc_sw128(sa, kAmn ? 64 * kBK * 2 : 16, 1024);
+          const uint64_t db0 = make_smem_desc_sw128(sb, kBmn ? 64 * kBK * 2 : 16, 1024);
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < kBK / 16; ++ks)
+              umma_f16_ss_pair(tmem_d, da0 + static_cast<uint64_t>(kAmn ? ks * 128 : ks * 2), db0 + static_cast<uint64_t>(kBmn ? ks * 128 : ks * 2),
+                               idesc, (kb > w.kb_begin || ks > 0) ? 1u : 0u);
+            umma_commit_pair(&empty_bar[stage], 3);
+          }
+          __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (leader) umma_commit_pair(&tfull_bar[acc], 3);
+        __syncwarp();
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* const st = store_base + (warp - 2) * (kSlots * 2048);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    const float k2 = p.inv_temp * kLog2e;
+    const float up = (MODE == kGrad && p.scale != nullptr) ? p.scale[0] : 1.0f;
+    const float down = ((MODE == kInputGrad || MODE == kWeightGrad) && p.scale != nullptr) ? p.scale[1] : 1.0f;
+    const int n_end = (MODE == kStats || MODE == kGrad) ? p.vocab : p.width;
+    for (int u = unit_first; u < e.units; u += unit_step) {
+      const Unit w = unit_at<MODE>(p, e, u);
+      const int row0 = w.m0 + m_off + quarter * 32, row = row0 + lane;
+      const int c0 = w.n0 + half * 128;  // this warp's columns: four chunks of 32
+      // what the rows need, under the tile's MMAs
+      int64_t at = 0;
+      int tcol = -1;
+      float2 mine = make_float2(0.0f, 0.0f);
+      float c = 0.0f;
+      bool counts = false;
+      if (MODE != kWeightGrad && row < live) {
+        at = place(p, row);
+        if (MODE == kStats || MODE == kGrad) {
+          const int64_t tg = target_of(p.targets, p.targets_wide, at);
+          counts = tg != p.ignore && tg >= 0 && tg < p.vocab;
+          tcol = counts ? static_cast<int>(tg) : -1;
+          if (MODE == kGrad && counts) {
+            mine = p.stats[p.row0 + row];
+            c = p.coef[at] * p.inv_temp * up;
+          }
+        }
+      }
+      const bool got = mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag);
+      if (!__all_sync(0xffffffffu, got)) {
+        if (lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kTile + half * 128);
+      float top = -INFINITY, sum = 0.0f;
+      const int chunks = c0 >= n_end ? 0 : min(4, (n_end - c0 + 31) / 32);
+      uint32_t r[32];
+      if (chunks > 0) tmem_ld_32x32b_x32(taddr, r);
+      auto release = [&] {  // everything this warp needs from the accumulator is in registers
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), 0));
+      };
+      if ((MODE == kGrad || MODE == kWeightGrad) && chunks > 0) {
+        if (lane == 0) tma_store_wait_read<0>();  // the staging tiles are free once the last group has been read
+        __syncwarp();
+      }
+#pragma unroll 1
+      for (int i = 0; i < chunks; ++i) {
+        const int col0 = c0 + i * 32;
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        if (i + 1 < chunks) tmem_ld_32x32b_x32(taddr + (i + 1) * 32, r);
+        else release();
+        const int valid = min(32, n_end - col0);
+        if constexpr (MODE == kStats) {
+          if (valid < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j >= valid) v[j] = -INFINITY;
+          }
+          const int off = tcol - col0;
+          if (__any_sync(0xffffffffu, off >= 0 && off < 32)) {
+            if (off >= 0 && off < 32) {
+              float t = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == off) t = v[j];
+              p.tlogit[row] = t;
+            }
+          }
+          float cm[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int j = 4; j < 32; ++j) cm[j & 3] = fmaxf(cm[j & 3], v[j]);
+          const float m = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3]));
+          if (m > top) {
+            if (top != -INFINITY) sum *= ex2((top - m) * k2);
+            top = m;
+          }
+          const float base = top == -INFINITY ? 0.0f : top;
+          float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s4[j & 3] += ex2((v[j] - base) * k2);
+          sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        } else if constexpr (MODE == kGrad) {
+          // rows that do not count, those behind the last one among them, are zeros whatever the product left there
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float g = -c * ex2(fmaf(v[j] - mine.x, k2, -mine.y));
+            if (col0 + j == tcol) g += c;
+            v[j] = counts ? g : 0.0f;
+          }
+          stage_row<BF>(st + i * 2048, lane, v);
+        } else if constexpr (MODE == kInputGrad) {
+          if (row < live) {
+            if (p.slices > 1) {
+              float* o = p.partial + (static_cast<int64_t>(w.slice) * p.cap + row) * p.width + col0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (4 * j < valid) *reinterpret_cast<float4*>(o + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+              uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + at * p.out_ld + col0;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (8 * j < valid) {
+                  uint4 q;
+                  q.x = pack2<BF>(v[8 * j] * down, v[8 * j + 1] * down);
+                  q.y = pack2<BF>(v[8 * j + 2] * down, v[8 * j + 3] * down);
+                  q.z = pack2<BF>(v[8 * j + 4] * down, v[8 * j + 5] * down);
+                  q.w = pack2<BF>(v[8 * j + 6] * down, v[8 * j + 7] * down);
+                  *reinterpret_cast<uint4*>(o + 8 * j) = q;
+                }
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = e.kb > 0 ? v[j] * down : 0.0f;  // no row counts: the accumulator was never written
+          if (p.partial != nullptr) {  // FP32 rows that several launches add up in
+            if (row < p.vocab) {
+              float* o = p.partial + static_cast<int64_t>(row) * p.width + col0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                if (4 * j < valid) {
+                  float4 q = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                  if (p.add) {
+                    const float4 was = *reinterpret_cast<const float4*>(o + 4 * j);
+                    q.x += was.x; q.y += was.y; q.z += was.z; q.w += was.w;
+                  }
+                  *reinterpret_cast<float4*>(o + 4 * j) = q;
+                }
+              }
+            }
+          } else {
+            stage_row<BF>(st + i * 2048, lane, v);
+          }
+        }
+      }
+      if (chunks == 0) release();
+      if constexpr (MODE == kStats) {
+        if (row < live && chunks > 0) p.part[static_cast<int64_t>(w.n0 / 128 + half) * p.part_ld + row] = make_float2(top, sum);
+      } else if constexpr (MODE == kGrad || MODE == kWeightGrad) {
+        if (chunks > 0 && (MODE == kGrad || p.partial == nullptr)) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          const int row_end = MODE == kGrad ? static_cast<int>(p.cap) : p.vocab;
+          if (lane == 0 && row0 < row_end) {
+            for (int i = 0; i < chunks; ++i) tma_store_3d(&map_out, st + i * 2048, c0 + 32 * i, row0, 0);
+            tma_store_commit();
+          }
+        }
+      }
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if ((MODE == kGrad || MODE == kWeightGrad) && lane == 0) tma_store_wait_all();  // the staging tiles die with the CTA
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0) {  // a wait ran out: copies still in flight land before the shared memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(2000);
+    __syncthreads();
+  }
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ around the products
+// index[0 .. count) = the rows whose target counts, in order; the others' logp is written.  One block: a thread takes a run of rows.
+constexpr int kPickThreads = 1024;
+__global__ void __launch_bounds__(kPickThreads) pick_rows_kernel(const void* __restrict__ targets, int wide, int64_t rows, int64_t ignore, int vocab,
+                                                                 int32_t* __restrict__ index, int32_t* __restrict__ count, float* __restrict__ logp) {
+  __shared__ int warp_total[32];
+  pdl_dependency();
+  pdl_trigger();
+  const int64_t per = (rows + kPickThreads - 1) / kPickThreads, first = threadIdx.x * per, end = min(rows, first + per);
+  int mine = 0;
+  for (int64_t r = first; r < end; ++r) {
+    const int64_t t = target_of(targets, wide, r);
+    const bool in = t >= 0 && t < vocab;
+    if (t != ignore && in) ++mine;
+    else logp[r] = t == ignore ? 0.0f : NAN;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_total[warp] = upto;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int i = 0; i < 32; ++i) {
+    if (i < warp) before += warp_total[i];
+    all += warp_total[i];
+  }
+  int at = before + upto - mine;
+  for (int64_t r = first; r < end; ++r) {
+    const int64_t t = target_of(targets, wide, r);
+    if (t != ignore && t >= 0 && t < vocab) index[at++] = static_cast<int32_t>(r);
+  }
+  if (threadIdx.x == 0) *count = all;
+}
+
+// Row r of `out` = row index[r] of `h` for r < count, zeros up to the next multiple of 64 (the reduction of the weight gradient reads them)
+__global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* __restrict__ h, int64_t ld, const int32_t* __restrict__ index,
+                                                          const int32_t* __restrict__ count, uint4* __restrict__ out, int pieces, int64_t rows) {
+  pdl_dependency();
+  pdl_trigger();
+  const int64_t n = *count, end = min((n + 63) / 64 * 64, rows);
+  for (int64_t r = blockIdx.x; r < end; r += gridDim.x) {
+    const uint4* src = r < n ? h + index[r] * ld : nullptr;
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) out[r * pieces + i] = src != nullptr ? src[i] : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Joins the column tiles' maxima and sums of a row: 32 rows per block, a warp per share of the tiles.
+__global__ void __launch_bounds__(1024) join_kernel(const Params p, int parts, float* __restrict__ logp, float2* __restrict__ stats) {
+  __shared__ float2 share[32][33];
+  pdl_dependency();
+  pdl_trigger();
+  const int64_t live = live_rows(p), row = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (static_cast<int64_t>(blockIdx.x) * 32 >= live) return;
+  const float k2 = p.inv_temp * kLog2e;
+  float top = -INFINITY, sum = 0.0f;
+  auto take = [&](const float2 v) {
+    if (v.x > top) {
+      if (top != -INFINITY) sum *= ex2((top - v.x) * k2);
+      top = v.x;
+    }
+    // a part of nothing but -inf has the sum 0 (or NaN)
+    sum += v.x == -INFINITY ? v.y : v.y * ex2((v.x - top) * k2);
+  };
+  if (row < live)
+    for (int i = warp; i < parts; i += 32) take(p.part[i * p.part_ld + row]);
+  share[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  const int r = warp;  // now a warp takes a row, a lane a share
+  const float2 v = share[lane][r];
+  const float m = warp_max(v.x);
+  const float s = warp_sum(v.x == -INFINITY ? v.y : v.y * ex2((v.x - m) * k2));
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + r;
+  if (lane == 0 && mine < live) {
+    const int64_t at = place(p, mine);
+    const int64_t tg = target_of(p.targets, p.targets_wide, at);
+    if (tg == p.ignore || tg < 0 || tg >= p.vocab) {
+      logp[at] = tg == p.ignore ? 0.0f : NAN;
+      return;
+    }
+    logp[at] = (p.tlogit[mine] - m) * p.inv_temp - logf(s);
+    stats[mine] = make_float2(m, log2f(s));
+  }
+}
+
+// scale = {2^e, 2^-e} with the largest |coef * inv_temp| * 2^e of the rows that count in [2^14, 2^15); one where none is positive and finite
+__global__ void __launch_bounds__(1024) coef_scale_kernel(const float* __restrict__ coef, const void* __restrict__ targets, int wide, int64_t ignore,
+                                                          int64_t n, float inv_temp, float* __restrict__ scale) {
+  __shared__ float scratch[32];
+  pdl_dependency();
+  pdl_trigger();
+  float top = 0.0f;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const float v = fabsf(coef[i]) * inv_temp;
+    if (v <= 3.0e38f && target_of(targets, wide, i) != ignore) top = fmaxf(top, v);
+  }
+  top = block_max(top, scratch);
+  if (threadIdx.x == 0) {
+    int e = 0;
+    if (top > 0.0f) {
+      frexpf(top, &e);
+      e = 15 - e;
+      e = max(-100, min(100, e));
+    }
+    scale[0] = ldexpf(1.0f, e);
+    scale[1] = ldexpf(1.0f, -e);
+  }
+}
+
+template <bool BF>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+}
+
+// Rows of dh = sum of the slices in order, times the inverse scale
+template <bool BF>
+__global__ void __launch_bounds__(128) slices_kernel(const Params p) {
+  pdl_dependency();
+  pdl_trigger();
+  const int64_t live = live_rows(p);
+  const float down = p.scale != nullptr ? p.scale[1] : 1.0f;
+  for (int64_t r = blockIdx.x; r < live; r += gridDim.x) {
+    uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + place(p, r) * p.out_ld;
+    for (int i = threadIdx.x * 8; i < p.width; i += blockDim.x * 8) {
+      float v[8] = {};
+      for (int s = 0; s < p.slices; ++s) {
+        const float4* q = reinterpret_cast<const float4*>(p.partial + (static_cast<int64_t>(s) * p.cap + r) * p.width + i);
+        const float4 a = q[0], b = q[1];
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= down;
+      *reinterpret_cast<uint4*>(o + i) = pack8<BF>(v);
+    }
+  }
+}
+
+// Rows of dh whose target does not count (or lies outside the vocabulary): zeros
+__global__ void __launch_bounds__(128) clear_rows_kernel(const void* __restrict__ targets, int wide, int64_t rows, int64_t ignore, int vocab,
+                                                         uint4* __restrict__ out, int64_t ld, int pieces) {
+  pdl_dependency();
+  pdl_trigger();
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int64_t t = target_of(targets, wide, r);
+    if (t != ignore && t >= 0 && t < vocab) continue;
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) out[r * ld + i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <bool BF>
+__global__ void __launch_bounds__(256) narrow_kernel(const float* __restrict__ x, uint4* __restrict__ out, int64_t pieces) {
+  pdl_dependency();
+  pdl_trigger();
+  NX_GRID_STRIDE(i, pieces) {
+    const float4 a = reinterpret_cast<const float4*>(x)[2 * i], b = reinterpret_cast<const float4*>(x)[2 * i + 1];
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    out[i] = pack8<BF>(v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+template <int MODE, bool BF>
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Params& p, int64_t units, cudaStream_t st) {
+  auto kern = head_kernel<MODE, BF>;
+  NX_ALLOW_SMEM(kern, kSmemBytes);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(units, kNumSmsB200 / 2)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const uint32_t fmt = BF ? kFmtBF16 : kFmtF16;
+  const uint32_t idesc = make_idesc(fmt, fmt, MODE == kWeightGrad, MODE == kInputGrad || MODE == kWeightGrad, kTile, kTile);
+  if (cudaLaunchKernelEx(&cfg, kern, a, b, out, p, idesc) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return -2;
+  }
+  return 0;
+}
+
+int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
+
+// K-major operand of [rows][k], or MN-major of [k][mn]; 128-byte swizzle
+int map_k(CUtensorMap* m, const NxHeadArgs* a, const void* base, int64_t k, int64_t rows, int64_t ld) {
+  const CUtensorMapDataType dt = a->dtype == NX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return make_tensor_map_3d(m, dt, 2, base, k, rows, 1, ld, 0, kBK, 128);
+}
+int map_mn(CUtensorMap* m, const NxHeadArgs* a, const void* base, int64_t mn, int64_t k, int64_t ld) {
+  const CUtensorMapDataType dt = a->dtype == NX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return make_tensor_map_3d(m, dt, 2, base, mn, k, 1, ld, 0, 64, kBK);
+}
+int map_store(CUtensorMap* m, const NxHeadArgs* a, const void* base, int64_t cols, int64_t rows, int64_t ld) {
+  const CUtensorMapDataType dt = a->dtype == NX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return make_tensor_map_3d(m, dt, 2, base, cols, rows, 1, ld, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+bool args_ok(const NxHeadArgs* a) {
+  auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  return a != nullptr && (a->dtype == NX_BF16 || a->dtype == NX_F16) && a->rows > 0 && a->rows <= (1 << 30) && a->width > 0 && a->width % 8 == 0 &&
+         a->vocab > 0 && a->vocab <= (1 << 30) && a->hidden != nullptr && a->weight != nullptr && a->targets != nullptr && !off(a->hidden) &&
+         !off(a->weight) && a->ld_hidden % 8 == 0 && a->ld_weight % 8 == 0 && a->ld_hidden >= a->width && a->ld_weight >= a->width &&
+         a->stats != nullptr && a->status != nullptr && (a->index == nullptr) == (a->count == nullptr) &&
+         (a->index == nullptr) == (a->gathered == nullptr) && !off(a->gathered);
+}
+
+Params base_params(const NxHeadArgs* a) {
+  Params p{};
+  p.rows = a->rows;
+  p.cap = a->rows;
+  p.count = a->count;
+  p.index = a->index;
+  p.targets = a->targets;
+  p.targets_wide = a->targets_wide;
+  p.ignore = a->ignore_index;
+  p.vocab = a->vocab;
+  p.width = a->width;
+  p.inv_temp = a->inv_temp;
+  p.stats = reinterpret_cast<const float2*>(a->stats);
+  p.status = a->status;
+  p.slices = 1;
+  // row tiles whose part of h is about 40 MB pass over the vocabulary together
+  p.group = static_cast<int>(std::max<int64_t>(1, (40ll << 20) / (static_cast<int64_t>(kTile) * a->width * 2)));
+  return p;
+}
+
+int gather(const NxHeadArgs* a, cudaStream_t st) {
+  const int pieces = a->width / 8;
+  NX_PDL(gather_rows_kernel, static_cast<unsigned>(std::min<int64_t>(a->rows, kNumSmsB200 * 8)), 256, 0, st,
+         reinterpret_cast<const uint4*>(a->hidden), a->ld_hidden / 8, a->index, a->count, reinterpret_cast<uint4*>(a->gathered), pieces,
+         (a->rows + 63) / 64 * 64);
+  return 0;
+}
+}  // namespace
+
+#define NX_HEAD(MODE_, ...) (a->dtype == NX_BF16 ? launch<MODE_, true>(__VA_ARGS__) : launch<MODE_, false>(__VA_ARGS__))
+
+extern "C" int64_t nx_head_parts(int32_t vocab) { return 2 * tiles(vocab); }
+
+extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* part, float* tlogit, nx_stream_t stream) {
+  if (!args_ok(a) || logp == nullptr || part == nullptr || tlogit == nullptr) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc;
+  if (a->index != nullptr) {
+    NX_PDL(pick_rows_kernel, 1, kPickThreads, 0, st, a->targets, a->targets_wide, a->rows, a->ignore_index, a->vocab, a->index, a->count, logp);
+    if ((rc = gather(a, st)) != 0) return rc;
+  }
+  const void* h = a->index != nullptr ? a->gathered : a->hidden;
+  const int64_t ldh = a->index != nullptr ? a->width : a->ld_hidden;
+  CUtensorMap ma, mb;
+  if ((rc = map_k(&ma, a, h, a->width, a->rows, ldh)) != 0 || (rc = map_k(&mb, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0) return rc;
+  Params p = base_params(a);
+  p.part = reinterpret_cast<float2*>(part);
+  p.part_ld = a->rows;
+  p.tlogit = tlogit;
+  if ((rc = NX_HEAD(kStats, ma, mb, ma, p, tiles(a->rows) * tiles(a->vocab), st)) != 0) return rc;
+  // the last column tile may have no second half
+  const int parts = static_cast<int>((a->vocab + 127) / 128);
+  NX_PDL(join_kernel, static_cast<unsigned>((a->rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
+  return 0;
+}
+
+extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, nx_stream_t stream) {
+  if (!args_ok(a) || g == nullptr || g->coef == nullptr || g->logit_grad == nullptr || g->chunk < kTile || g->chunk % kTile != 0 ||
+      g->ld_logit_grad < a->vocab || g->ld_logit_grad % 64 != 0 || (reinterpret_cast<uintptr_t>(g->logit_grad) & 15) != 0 ||
+      (a->dtype == NX_F16 && g->scale == nullptr) || g->slices < 1 || (g->slices > 1 && g->slice_sums == nullptr) ||
+      (reinterpret_cast<uintptr_t>(g->d_hidden) & 15) != 0 || (reinterpret_cast<uintptr_t>(g->d_weight) & 15) != 0 ||
+      (g->d_weight != nullptr && g->chunk < a->rows && g->weight_sums == nullptr))
+    return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc;
+  const bool half = a->dtype == NX_F16;
+  if (half) NX_PDL(coef_scale_kernel, 1, 1024, 0, st, g->coef, a->targets, a->targets_wide, a->ignore_index, a->rows, a->inv_temp, g->scale);
+  if (a->index != nullptr && (rc = gather(a, st)) != 0) return rc;
+  const void* h = a->index != nullptr ? a->gathered : a->hidden;
+  const int64_t ldh = a->index != nullptr ? a->width : a->ld_hidden;
+  if (g->d_hidden != nullptr)
+    NX_PDL(clear_rows_kernel, static_cast<unsigned>(std::min<int64_t>(a->rows, kNumSmsB200 * 16)), 128, 0, st, a->targets, a->targets_wide, a->rows,
+           a->ignore_index, a->vocab, reinterpret_cast<uint4*>(g->d_hidden), static_cast<int64_t>(a->width / 8), a->width / 8);
+  const bool sums = g->d_weight != nullptr && g->chunk < a->rows;  // several launches add up in FP32
+  CUtensorMap w_k, w_mn, g_k, g_mn, g_out, dw_out;
+  const int64_t ldg = g->ld_logit_grad;
+  if ((rc = map_k(&w_k, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0 || (rc = map_mn(&w_mn, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0 ||
+      (rc = map_k(&g_k, a, g->logit_grad, a->vocab, g->chunk, ldg)) != 0 || (rc = map_mn(&g_mn, a, g->logit_grad, a->vocab, g->chunk, ldg)) != 0 ||
+      (rc = map_store(&g_out, a, g->logit_grad, a->vocab, g->chunk, ldg)) != 0)
+    return rc;
+  dw_out = g_out;
+  if (g->d_weight != nullptr && !sums && (rc = map_store(&dw_out, a, g->d_weight, a->width, a->vocab, a->width)) != 0) return rc;
+  for (int64_t row0 = 0; row0 < a->rows; row0 += g->chunk) {
+    Params p = base_params(a);
+    p.row0 = row0;
+    p.cap = g->chunk;
+    p.coef = g->coef;
+    p.scale = half ? g->scale : nullptr;
+    const int64_t here = std::min(g->chunk, a->rows - row0);
+    CUtensorMap h_k, h_mn;
+    const uint16_t* hp = static_cast<const uint16_t*>(h) + row0 * ldh;
+    if ((rc = map_k(&h_k, a, hp, a->width, here, ldh)) != 0 || (rc = map_mn(&h_mn, a, hp, a->width, here, ldh)) != 0) return rc;
+    if ((rc = NX_HEAD(kGrad, h_k, w_k, g_out, p, tiles(here) * tiles(a->vocab), st)) != 0) return rc;
+    if (g->d_hidden != nullptr) {
+      p.out = g->d_hidden;
+      p.out_ld = a->width;
+      const int64_t blocks = (a->vocab + kBK - 1) / kBK;
+      p.blocks_per_slice = static_cast<int>((blocks + g->slices - 1) / g->slices);
+      p.slices = static_cast<int>((blocks + p.blocks_per_slice - 1) / p.blocks_per_slice);
+      p.partial = p.slices > 1 ? g->slice_sums : nullptr;
+      if ((rc = NX_HEAD(kInputGrad, g_k, w_mn, g_out, p, tiles(here) * tiles(a->width) * p.slices, st)) != 0) return rc;
+      if (p.slices > 1) {
+        const unsigned blocks_out = static_cast<unsigned>(std::min<int64_t>(here, kNumSmsB200 * 16));
+        if (half) NX_PDL((slices_kernel<false>), blocks_out, 128, 0, st, p);
+        else NX_PDL((slices_kernel<true>), blocks_out, 128, 0, st, p);
+      }
+    }
+    if (g->d_weight != nullptr) {
+      p.slices = 1;
+      p.partial = sums ? g->weight_sums : nullptr;
+      p.add = row0 > 0;
+      if ((rc = NX_HEAD(kWeightGrad, g_mn, h_mn, dw_out, p, tiles(a->vocab) * tiles(a->width), st)) != 0) return rc;
+    }
+  }
+  if (sums) {
+    const int64_t pieces = static_cast<int64_t>(a->vocab) * a->width / 8;
+    if (half) NX_PDL((narrow_kernel<false>), blocks_for(pieces, 256), 256, 0, st, g->weight_sums, static_cast<uint4*>(g->d_weight), pieces);
+    else NX_PDL((narrow_kernel<true>), blocks_for(pieces, 256), 256, 0, st, g->weight_sums, static_cast<uint4*>(g->d_weight), pieces);
+  }
+  return 0;
+}

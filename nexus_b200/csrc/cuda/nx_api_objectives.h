@@ -61,6 +61,40 @@ typedef struct NxPreferenceArgs {
 // seq_logp [2 * pairs], margin [pairs], coef [2 * pairs] = d loss / d logp of each counted token, loss: one float
 int nx_preference_loss(const NxPreferenceArgs* args, float* seq_logp, float* margin, float* coef, float* loss, nx_stream_t stream);
 
+// Log-probabilities of `targets` [rows] under softmax(hidden weight^T * inv_temp), hidden [rows, width] of pitch ld_hidden, weight
+// [vocab, width] of pitch ld_weight, BF16 or FP16 (16-byte bases; width and pitches multiples of 8).  `index` [rows], `count` [1] and `gathered`
+// [rows rounded up to 64, width], all three or none: the rows that count are brought together before the products (the forward call fills index
+// and count, both calls fill `gathered`).  stats [rows] pairs, written by the forward call, read by the gradient.
+typedef struct NxHeadArgs {
+  const void* hidden;
+  const void* weight;
+  const void* targets;
+  int32_t* index;
+  int32_t* count;
+  void* gathered;
+  float* stats;
+  int* status;  // receives a non-zero nx::StatusCode when a wait timed out
+  int64_t rows, ld_hidden, ld_weight, ignore_index;
+  int32_t vocab, width, dtype, targets_wide;
+  float inv_temp;
+  int32_t pad_;
+} NxHeadArgs;
+int64_t nx_head_parts(int32_t vocab);  // `part` holds this many pairs of floats per row
+// logp [rows] (0 where ignored, NaN where the target lies outside the vocabulary); part, tlogit [rows]: scratch
+int nx_head_logprobs(const NxHeadArgs* args, float* logp, float* part, float* tlogit, nx_stream_t stream);
+typedef struct NxHeadGrad {
+  const float* coef;       // [rows] gradient of logp
+  void* logit_grad;        // scratch [chunk, ld_logit_grad] of the operands' type: rows are taken `chunk` (a multiple of 256) at a time
+  int64_t chunk, ld_logit_grad;  // ld a multiple of 64
+  float* scale;            // two floats of scratch (FP16)
+  void* d_hidden;          // [rows, width], may be null
+  void* d_weight;          // [vocab, width], may be null
+  float* slice_sums;       // slices > 1: scratch [slices, chunk, width]: the vocabulary is cut to fill the machine
+  float* weight_sums;      // chunk < rows: scratch [vocab, width]
+  int32_t slices, pad_;
+} NxHeadGrad;
+int nx_head_logprobs_grad(const NxHeadArgs* args, const NxHeadGrad* grad, nx_stream_t stream);
+
 // Gradients of `tensors` tensors (host arrays): count elements at src, of NxDType `type & 15`; the clipped ones go to dst, of type `type >> 4`
 // (dst null: in place, both types the same).
 typedef struct NxGradTable {

@@ -130,6 +130,61 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: in
     return _token_parts(logits, targets, ignore_index, temperature, V)[2].view(targets.shape)
 
 
+class _LinearLogprobs(torch.autograd.Function):
+    """The logits exist a tile at a time, in tensor memory; the backward pass makes them again."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, vocab, ignore_index, temperature, want_grad):
+        from ..ops import _objectives as O
+        with torch.cuda.device(hidden.device):
+            h, w, t = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight), targets.contiguous()
+            logp, stats, index = O.head_logprobs(h, w, t, vocab, ignore_index, 1.0 / temperature, want_grad)
+        if want_grad:
+            ctx.save_for_backward(hidden, weight, t, stats, index)
+        ctx.cfg = (vocab, ignore_index, temperature)
+        return logp.view(targets.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp):
+        from ..ops import _objectives as O
+        hidden, weight, t, stats, index = ctx.saved_tensors
+        vocab, ignore_index, temperature = ctx.cfg
+        with torch.cuda.device(hidden.device):
+            h, w = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight)
+            dh, dw = O.head_logprobs_grad(h, w, t, vocab, ignore_index, 1.0 / temperature, stats, index, dlogp.float().contiguous(),
+                                          ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None, None
+
+
+def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
+                    vocab: Optional[int] = None) -> torch.Tensor:
+    """`token_logprobs` of the logits ``hidden @ weight.T`` without the logits in memory: hidden [..., d], weight [V(+pad), d] of one type,
+    targets [...].  Differentiable (once) with respect to both; the backward pass holds the gradient of at most 2^29 logits (or of 256 rows) at
+    a time.  The kernels take BF16 and FP16 with d a multiple of 8 (logits in FP32, rounded nowhere; their gradient rounded to the type for
+    its products); other types and sizes go through the logits."""
+    name = "linear_logprobs"
+    if not torch.is_floating_point(hidden) or hidden.dim() < 1 or weight.dim() != 2 or weight.dtype != hidden.dtype:
+        raise ValueError(f"{name}: hidden [..., d] and weight [V, d] must be floating-point tensors of one type")
+    if weight.shape[1] != hidden.shape[-1]:
+        raise ValueError(f"{name}: hidden has {hidden.shape[-1]} columns, weight {weight.shape[1]}")
+    if weight.device != hidden.device or targets.device != hidden.device:
+        raise ValueError(f"{name}: hidden on {hidden.device}, weight on {weight.device}, targets on {targets.device}")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: targets must be int32 or int64, got {targets.dtype}")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"{name}: targets {tuple(targets.shape)} do not match hidden {tuple(hidden.shape)}")
+    _check_temperature(name, temperature)
+    V = weight.shape[0] if vocab is None else int(vocab)
+    if not 1 <= V <= weight.shape[0]:
+        raise ValueError(f"{name}: vocab must be between 1 and {weight.shape[0]}, got {V}")
+    d, n = hidden.shape[-1], targets.numel()
+    if n and d and d % 8 == 0 and hidden.dtype != torch.float32 and max(n, V) <= 1 << 30 and _kernels(hidden):
+        want = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+        return _LinearLogprobs.apply(hidden, weight, targets, V, ignore_index, float(temperature), want)
+    return token_logprobs(torch.nn.functional.linear(hidden, weight), targets, ignore_index, temperature, V)
+
+
 # ---------------------------------------------------------------------------------------------------------- policy loss
 class _PolicyLoss(torch.autograd.Function):
     """Loss and gradient from one pass; the backward pass multiplies the gradient where the loss's own is not 1."""

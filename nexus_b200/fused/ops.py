@@ -613,5 +613,5 @@ def adamw_multi_tensor(params: Sequence[torch.Tensor], grads: Sequence[torch.Ten
 
 
 # ------------------------------------------------------------------- fine-tuning on rewards and preferences
-from .objectives import (PolicyLoss, PreferenceLoss, clip_grad_norm_, grad_square_sum, policy_loss, preference_loss,  # noqa: E402,F401
-                         token_logprobs)
+from .objectives import (PolicyLoss, PreferenceLoss, clip_grad_norm_, grad_square_sum, linear_logprobs, policy_loss,  # noqa: E402,F401
+                         preference_loss, token_logprobs)

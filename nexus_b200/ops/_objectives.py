@@ -136,6 +136,105 @@ def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, k
     return loss, seq_logp, margin, coef
 
 
+# ------------------------------------------------------------------------------------------- log-probabilities from hidden states
+class HeadArgs(C.Structure):
+    _fields_ = [("hidden", C.c_void_p), ("weight", C.c_void_p), ("targets", C.c_void_p), ("index", C.c_void_p), ("count", C.c_void_p),
+                ("gathered", C.c_void_p), ("stats", C.c_void_p), ("status", C.c_void_p), ("rows", C.c_int64), ("ld_hidden", C.c_int64),
+                ("ld_weight", C.c_int64), ("ignore_index", C.c_int64), ("vocab", C.c_int32), ("width", C.c_int32), ("dtype", C.c_int32),
+                ("targets_wide", C.c_int32), ("inv_temp", C.c_float), ("pad_", C.c_int32)]
+
+
+class HeadGrad(C.Structure):
+    _fields_ = [("coef", C.c_void_p), ("logit_grad", C.c_void_p), ("chunk", C.c_int64), ("ld_logit_grad", C.c_int64), ("scale", C.c_void_p),
+                ("d_hidden", C.c_void_p), ("d_weight", C.c_void_p), ("slice_sums", C.c_void_p), ("weight_sums", C.c_void_p),
+                ("slices", C.c_int32), ("pad_", C.c_int32)]
+
+
+HEAD_TILE = 256
+HEAD_GRAD_ELEMENTS = 1 << 29     # of the logits' gradient at a time: 1 GiB
+
+
+def head_rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix as the tensor maps take it: contiguous rows on 16-byte boundaries; copied if it is not one."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _head_args(hidden, weight, targets, index, stats, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
+    a = HeadArgs()
+    a.hidden, a.weight, a.targets, a.stats = hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr()
+    a.status = K.status_word(hidden.device).data_ptr()
+    a.rows, a.width = hidden.shape
+    a.ld_hidden, a.ld_weight, a.ignore_index, a.vocab = hidden.stride(0), weight.stride(0), ignore_index, vocab
+    a.dtype, a.targets_wide, a.inv_temp = K._DT[hidden.dtype], int(targets.dtype == torch.int64), inv_temp
+    if index is not None:
+        a.index, a.count = index.data_ptr(), index.data_ptr() + 4 * a.rows
+    return a
+
+
+def _gathered(hidden) -> torch.Tensor:
+    return torch.empty(((hidden.shape[0] + 63) // 64 * 64, hidden.shape[1]), dtype=hidden.dtype, device=hidden.device)
+
+
+def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, want_grad: bool):
+    """FP32 logp [rows] for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient needs: (stats, index
+    of the rows that count, with their number behind it, or None)."""
+    rows, dev = hidden.shape[0], hidden.device
+    L = K.lib()
+    index = torch.empty(rows + 1, dtype=torch.int32, device=dev) if want_grad or rows > HEAD_TILE else None
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+    parts = int(L.nx_head_parts(C.c_int32(vocab)))
+    part = torch.empty((2 * parts + 1) * rows, dtype=torch.float32, device=dev)
+    a = _head_args(hidden, weight, targets, index, stats, vocab, ignore_index, inv_temp)
+    moved = _gathered(hidden) if index is not None else None
+    a.gathered = None if moved is None else moved.data_ptr()
+    K._check(L.nx_head_logprobs(C.byref(a), K._p(logp), K._p(part), C.c_void_p(part.data_ptr() + 8 * parts * rows), K._stream()),
+             "nx_head_logprobs")
+    return logp, stats, index
+
+
+def head_slices(rows: int, width: int, vocab: int, clusters: int = 74) -> int:
+    """Pieces of the vocabulary whose shares of a hidden-state gradient are summed afterwards: rounds of tiles over the CTA pairs times
+    (64-deep blocks of a piece, and about six for handing a tile over), and the sums' own traffic in the same units (0.39 us)."""
+    tiles, blocks = -(-rows // HEAD_TILE) * -(-width // HEAD_TILE), -(-vocab // 64)
+    best, pick = None, 1
+    for s in range(1, 17):
+        per = -(-blocks // s)
+        cost = -(-tiles * s // clusters) * (per + 6) + (0 if s == 1 else 8 + s * rows * width * 8 / 2.0e6)
+        if best is None or cost < best:
+            best, pick = cost, s
+    return pick
+
+
+def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, stats, index, coef, want_hidden: bool,
+                       want_weight: bool):
+    """(d_hidden [rows, width], d_weight [all rows of weight, width]), either None where not wanted."""
+    rows, width = hidden.shape
+    dev, dtype = hidden.device, hidden.dtype
+    a = _head_args(hidden, weight, targets, index, stats, vocab, ignore_index, inv_temp)
+    moved = _gathered(hidden)
+    a.gathered = moved.data_ptr()
+    g = HeadGrad()
+    ld = (vocab + 63) // 64 * 64
+    chunk = min((rows + 255) // 256 * 256, max(256, HEAD_GRAD_ELEMENTS // ld // 256 * 256))
+    logit_grad = torch.empty((chunk, ld), dtype=dtype, device=dev)
+    scale = torch.empty(2, dtype=torch.float32, device=dev)
+    g.coef, g.logit_grad, g.chunk, g.ld_logit_grad, g.scale = coef.data_ptr(), logit_grad.data_ptr(), chunk, ld, scale.data_ptr()
+    dh = torch.empty((rows, width), dtype=dtype, device=dev) if want_hidden else None
+    dw = torch.empty((weight.shape[0], width), dtype=dtype, device=dev) if want_weight else None
+    if want_weight and weight.shape[0] > vocab:
+        dw[vocab:].zero_()
+    g.slices = head_slices(min(rows, chunk), width, vocab) if want_hidden else 1
+    slice_sums = torch.empty((g.slices, chunk, width), dtype=torch.float32, device=dev) if g.slices > 1 else None
+    weight_sums = torch.empty((vocab, width), dtype=torch.float32, device=dev) if want_weight and chunk < rows else None
+    for name, t in (("d_hidden", dh), ("d_weight", dw), ("slice_sums", slice_sums), ("weight_sums", weight_sums)):
+        setattr(g, name, None if t is None else t.data_ptr())
+    K._check(K.lib().nx_head_logprobs_grad(C.byref(a), C.byref(g), K._stream()), "nx_head_logprobs_grad")
+    return dh, dw
+
+
 # ---------------------------------------------------------------------------------------------------- gradients of many tensors
 class GradTable(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("count", C.c_void_p), ("type", C.c_void_p), ("tensors", C.c_int64)]

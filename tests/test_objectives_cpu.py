@@ -116,3 +116,25 @@ def test_clip_refusals():
                  lambda: F.clip_grad_norm_([a, a], 1.0, out=[torch.ones(6), torch.ones(6)]), lambda: F.clip_grad_norm_([a.to_sparse()], 1.0)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_linear_logprobs_on_the_host():
+    g = torch.Generator().manual_seed(1)
+    h = torch.randn(2, 3, 8, dtype=torch.float64, generator=g, requires_grad=True)
+    w = torch.randn(11, 8, dtype=torch.float64, generator=g, requires_grad=True)
+    t = torch.randint(0, 10, (2, 3), generator=g)
+    t[0, 0] = -100
+    assert torch.autograd.gradcheck(lambda h, w: F.linear_logprobs(h, w, t, temperature=0.9, vocab=10), (h, w))
+    for call in (lambda: F.linear_logprobs(h, w.float(), t), lambda: F.linear_logprobs(h, w[:, :4], t), lambda: F.linear_logprobs(h, w, t[0]),
+                 lambda: F.linear_logprobs(h, w, t.float()), lambda: F.linear_logprobs(h, w, t, vocab=12), lambda: F.linear_logprobs(h, w[0], t),
+                 lambda: F.linear_logprobs(h, w, t, temperature=0.0), lambda: F.linear_logprobs(h.long(), w.long(), t)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_slices_of_the_vocabulary_fill_the_machine():
+    from nexus_b200.ops._objectives import head_slices
+    assert head_slices(8192, 4096, 32000) == 1
+    for rows, width, vocab in ((609, 896, 151936), (1, 64, 1000), (256, 4096, 32000)):
+        s = head_slices(rows, width, vocab)
+        assert 1 <= s <= 16
