@@ -21,10 +21,12 @@ typedef struct NxTokenRows {
   int32_t pad_;
 } NxTokenRows;
 
-// logp [rows] = log-probability of the target (0 where ignored); stats [rows] pairs: the largest logit, and log2 of the sum of
-// exp((logit - largest) * inv_temp).
-int nx_token_logprobs(const NxTokenRows* rows, float* logp, float* stats, nx_stream_t stream);
-// grad = coef (delta_target - p) * inv_temp in the layout and type of the logits (zeros in ignored rows and behind the vocabulary);
+// logp [rows] = log-probability of the target (0 where ignored); stats [rows] pairs: a logit x, and log2 of the sum of
+// exp((logit - x) * inv_temp).
+// status: device int, receives a non-zero nx::StatusCode when a wait timed out.
+int nx_token_logprobs(const NxTokenRows* rows, float* logp, float* stats, int* status, nx_stream_t stream);
+// A gradient has the layout and type of the logits and starts at the same place of a 16-byte line.
+// grad = coef (delta_target - p) * inv_temp (zeros in ignored rows and behind the vocabulary);
 // coef of row r: coef[r / coef_per] * *factor (factor: device scalar, may be null)
 int nx_token_logprobs_grad(const NxTokenRows* rows, const float* stats, const float* coef, int64_t coef_per, const float* factor,
                            void* grad, nx_stream_t stream);
@@ -45,7 +47,7 @@ typedef struct NxPolicyArgs {
 // both scratch; loss: one float;
 // grad (write_grad): d loss / d logits in the layout and type of the logits.
 int nx_policy_loss(const NxTokenRows* rows, const NxPolicyArgs* args, double* totals, int32_t* counts, float* logp, float* kl, float* entropy,
-                   float* row_loss, float* loss, void* grad, nx_stream_t stream);
+                   float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream);
 // x *= *factor in place, n elements; nothing is read or written where the factor is 1
 int nx_scale_unless_one(void* x, const float* factor, int dtype, int64_t n, nx_stream_t stream);
 

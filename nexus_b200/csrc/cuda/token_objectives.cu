@@ -3,23 +3,28 @@
 //   x = logits * inv_temp,  m = max,  s = sum exp(x - m),  logp_j = x_j - m - ln s,  p_j = exp(logp_j),  H = ln s - sum p_j (x_j - m)
 //   d logp_t / d x_j = delta_jt - p_j          d H / d x_j = -p_j (logp_j + H)
 //
-// Statistics are kept as the largest logit and log2 of the sum: with the difference taken before any product, p and logp have no
+// Statistics are kept as one logit and log2 of the sum relative to it: with the difference taken before any product, p and logp have no
 // rounding that grows with the logits (a sum m + ln s rounded to FP32 would put 2^-24 |lse| into the exponent of every p).
 // Everything here is bound by the bytes of the logits.
 #include "common.cuh"
 #include "nx_api_objectives.h"
 #include "row_vec.cuh"
+#include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 namespace {
 using namespace nx;
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 512;
 
+// rows, and with them `per`, `adv_per` and `seq_len` that divide them, stay below 2^31
+__device__ __forceinline__ uint32_t row_over(int64_t r, int64_t by) { return static_cast<uint32_t>(r) / static_cast<uint32_t>(by); }
 __device__ __forceinline__ int64_t row_offset(const NxTokenRows& a, int64_t r) {
-  const int64_t o = r / a.per;
+  const int64_t o = row_over(r, a.per);
   return o * a.stride_outer + (r - o * a.per) * a.stride_inner;
 }
 __device__ __forceinline__ int64_t target_at(const void* targets, int wide, int64_t r) {
@@ -71,73 +76,7 @@ struct Online {
   }
 };
 
-template <typename T, bool kEntropy>
-__device__ __forceinline__ void absorb_row(const T* p, int count, float k, Online<kEntropy>& on) {
-  constexpr int VN = RowVec<T>::kN;
-  const RowSplit<T> sp(p, count);
-  const T* body = p + sp.head;
-  const int step = blockDim.x;
-  int i = threadIdx.x;
-  for (; i + 3 * step < sp.pieces; i += 4 * step) {
-    uint4 raw[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) raw[u] = *reinterpret_cast<const uint4*>(body + static_cast<int64_t>(i + u * step) * VN);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float v[VN];
-      RowVec<T>::unpack(raw[u], v);
-      on.absorb(v, k);
-    }
-  }
-  for (; i < sp.pieces; i += step) {
-    float v[VN];
-    RowVec<T>::load(body + static_cast<int64_t>(i) * VN, v);
-    on.absorb(v, k);
-  }
-  if (static_cast<int>(threadIdx.x) < sp.head) {
-    const float v[1] = {Num<T>::load(p + threadIdx.x)};
-    on.absorb(v, k);
-  } else if (static_cast<int>(threadIdx.x) >= 32 && static_cast<int>(threadIdx.x) - 32 < sp.tail) {
-    const float v[1] = {Num<T>::load(body + static_cast<int64_t>(sp.pieces) * VN + threadIdx.x - 32)};
-    on.absorb(v, k);
-  }
-}
-
-// Every thread gets the block's maximum and sums.
-template <bool kEntropy>
-__device__ __forceinline__ void join_block(Online<kEntropy>& on, float k, float* scratch) {
-  const float top = block_max(on.m, scratch);
-  if (on.m != top) on.raise(top, k);
-  on.s = block_sum<float>(on.s, scratch);
-  if (kEntropy) on.h = block_sum<float>(on.h, scratch);
-}
-
-// ------------------------------------------------------------------------------------------------ log-probabilities
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_stats_kernel(const NxTokenRows a, float* __restrict__ logp, float2* __restrict__ stats) {
-  __shared__ float scratch[32];
-  pdl_dependency();
-  pdl_trigger();
-  const int64_t row = blockIdx.x;
-  const int64_t tg = target_at(a.targets, a.targets_wide, row);
-  const bool inside = tg >= 0 && tg < a.vocab;
-  if (tg == a.ignore_index || !inside) {
-    if (threadIdx.x == 0) {
-      logp[row] = tg == a.ignore_index ? 0.0f : NAN;
-      stats[row] = make_float2(0.0f, 0.0f);
-    }
-    return;
-  }
-  const T* p = reinterpret_cast<const T*>(a.logits) + row_offset(a, row);
-  Online<false> on;
-  absorb_row(p, a.vocab, a.inv_temp * kLog2e, on);
-  join_block(on, a.inv_temp * kLog2e, scratch);
-  if (threadIdx.x == 0) {
-    logp[row] = (Num<T>::load(p + tg) - on.m) * a.inv_temp - logf(on.s);
-    stats[row] = make_float2(on.m, log2f(on.s));
-  }
-}
-
+// ------------------------------------------------------------------------------------------------ gradients of rows
 // Gradient of a row, four pieces of loads at a time: f(logit) for every element of the vocabulary, `extra` added at the target, zeros behind.
 template <typename T, typename F>
 __device__ __forceinline__ void write_row(const T* p, T* g, int vocab, int width, int tg, float extra, F f) {
@@ -193,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) token_grad_kernel(const NxTokenRows 
                                                               const float* __restrict__ factor, T* __restrict__ grad) {
   pdl_dependency();
   pdl_trigger();
-  const int64_t row = blockIdx.x;
+  const int64_t row = gridDim.x - 1 - blockIdx.x;  // the last rows first: the sums have left them in L2
   const int64_t tg = target_at(a.targets, a.targets_wide, row);
   const int64_t at = row_offset(a, row);
   T* g = grad + at;
@@ -201,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) token_grad_kernel(const NxTokenRows 
     clear_row(g, a.width);
     return;
   }
-  const float c = coef[row / coef_per] * (factor != nullptr ? *factor : 1.0f) * a.inv_temp;
+  const float c = coef[row_over(row, coef_per)] * (factor != nullptr ? *factor : 1.0f) * a.inv_temp;
   const float2 st = stats[row];
   const float k = a.inv_temp * kLog2e;
   write_row(reinterpret_cast<const T*>(a.logits) + at, g, a.vocab, a.width, static_cast<int>(tg), c,
@@ -212,11 +151,6 @@ __global__ void __launch_bounds__(kThreads) token_grad_kernel(const NxTokenRows 
 // Sums over a few thousand to a million values by one cluster of eight blocks: partial sums meet in the first block's shared memory.
 constexpr int kJoinBlocks = 8, kJoinThreads = 1024;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // slot[rank] of the cluster's first block = v; one thread of each block, once every block of the cluster is known to run
@@ -235,7 +169,7 @@ token_count_kernel(const void* __restrict__ targets, int wide, int64_t sequences
   cluster_arrive();
   pdl_dependency();
   pdl_trigger();
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = cluster_ctarank();
   double mine = 0.0, full = 0.0;
   if (len >= 256) {
     for (int64_t q = rank; q < sequences; q += kJoinBlocks) {
@@ -287,7 +221,7 @@ sum_kernel(const float* __restrict__ x, int64_t n, float* __restrict__ out) {
   cluster_arrive();
   pdl_dependency();
   pdl_trigger();
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = cluster_ctarank();
   double acc = 0.0;
   for (int64_t i = rank * kJoinThreads + threadIdx.x; i < n; i += kJoinBlocks * kJoinThreads) acc += x[i];
   acc = block_sum<double>(acc, scratch);
@@ -308,16 +242,29 @@ struct PolicyRow {
   float ent;     // entropy coefficient, weighted
   float loss, kl;
 };
-__device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, int64_t row, float logp, float entropy, float weight) {
+struct PolicyIn {
+  float adv, old, ref, weight;
+};
+// A row's constants and weight: the whole batch's mean over tokens, the mean over sequences of the means over their tokens, or one.
+__device__ __forceinline__ PolicyIn policy_in(const NxPolicyArgs& g, const double* totals, const int32_t* counts, int64_t row) {
+  PolicyIn i;
+  i.adv = g.advantages[row_over(row, g.adv_per)];
+  i.old = g.old_logp[row];
+  i.ref = g.ref_logp != nullptr ? g.ref_logp[row] : 0.0f;
+  i.weight = g.scale;
+  if (g.mean == NX_MEAN_TOKEN) i.weight = static_cast<float>(g.scale / totals[0]);
+  if (g.mean == NX_MEAN_SEQUENCE) i.weight = static_cast<float>(g.scale / (totals[1] * counts[row_over(row, g.seq_len)]));
+  return i;
+}
+__device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, const PolicyIn& in, float logp, float entropy) {
   PolicyRow o;
-  const float adv = g.advantages[row / g.adv_per];
-  const float ratio = expf(logp - g.old_logp[row]);
-  const float free = ratio * adv, bound = fminf(fmaxf(ratio, 1.0f - g.clip_low), 1.0f + g.clip_high) * adv;
+  const float ratio = expf(logp - in.old);
+  const float free = ratio * in.adv, bound = fminf(fmaxf(ratio, 1.0f - g.clip_low), 1.0f + g.clip_high) * in.adv;
   const bool follows = free <= bound;  // the unclipped term is the smaller one, or they are equal
   float loss = follows ? -free : -bound, c = follows ? -free : 0.0f;
   o.kl = 0.0f;
   if (g.ref_logp != nullptr) {
-    const float d = g.ref_logp[row] - logp;
+    const float d = in.ref - logp;
     float slope;
     if (g.kl == NX_KL_K3) {
       const float e = expm1f(d);
@@ -334,65 +281,652 @@ __device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, int64_t r
     c = fmaf(g.kl_coef, slope, c);
   }
   if (g.entropy_coef != 0.0f) loss -= g.entropy_coef * entropy;
-  o.loss = loss * weight;
-  o.c = c * weight;
-  o.ent = g.entropy_coef * weight;
+  o.loss = loss * in.weight;
+  o.c = c * in.weight;
+  o.ent = g.entropy_coef * in.weight;
   return o;
 }
 
-// Weight of a row: the whole batch's mean over tokens, the mean over sequences of the means over their tokens, or one.
-__device__ __forceinline__ float policy_weight(const NxPolicyArgs& g, const double* totals, const int32_t* counts, int64_t row) {
-  if (g.mean == NX_MEAN_NONE) return g.scale;
-  if (g.mean == NX_MEAN_TOKEN) return static_cast<float>(g.scale / totals[0]);
-  return static_cast<float>(g.scale / (totals[1] * counts[row / g.seq_len]));
+// ------------------------------------------------------------------------------------------------ rows through shared memory
+// A persistent block reads its rows through a ring of 16 KiB slots in shared memory, filled by one warp with bulk copies: what a row needs
+// arrives while the block still works on the row before it.  Sums come from the first pass over a row's slots; where a gradient is written, the
+// slots stay for a second pass, which frees them one by one for the next row: one read of the logits.  Of a row that is longer than the ring,
+// the last slots stay and the others are read again, from L2.  Few rows are cut over a cluster of blocks, whose sums meet in each other's shared
+// memory.
+//
+// Three shapes (BF16, B200; bytes read and written over the time):
+//   sums only                 three blocks of four warps per SM      8192 x 50304: 146 us, 5.6 TB/s; two of eight warps 156, one of sixteen 180
+//   gradient, rows to 112 KiB two blocks of eight warps              8192 x 50304: 283 us, 5.8 TB/s; one of sixteen 336, three of four 332
+//   gradient, longer rows     one block of sixteen warps, 208 KiB    2368 x 32000 FP32: 101 us, 6.0 TB/s; two of eight 114
+// With sums and maxima kept per thread instead of a common base, 64-bit divisions per row in every thread and each row's target and constants
+// loaded at its beginning, the same ring took 465 us for 8192 x 50304 (11 instructions per element and pass instead of 5).
+constexpr int kSlotBytes = 16384, kSlotPieces = kSlotBytes / 16;
+constexpr int kMaxCuts = 8;
+
+template <int WORKERS, int SLOTS, int RESIDENT>
+struct Shape {
+  static constexpr int kWorkers = WORKERS, kThreads = WORKERS + 32;  // and the warp that copies
+  static constexpr int kSlots = SLOTS, kResident = RESIDENT;         // blocks per SM
+};
+using SumsShape = Shape<128, 4, 3>;
+using ShortShape = Shape<256, 7, 2>;
+using LongShape = Shape<512, 13, 1>;
+
+// A row's sums relative to its target's logit:  s = sum 2^t,  h = sum t 2^t  with  t = v k - B,  B = x_t k rounded,  k = log2(e) inv_temp.  The
+// base is the same for every thread and block, so joining is adding and no maximum is kept; the product is inside the fused multiply-add, so t
+// is exact to its own last bit, and results are taken relative to B itself.  The target's own term makes s at least 1.  A row where a logit lies
+// so far above its target's that the sums overflow (t of 120 and more), or where B would be too coarse (|x_t| above kFastLimit, -inf, NaN), is
+// done again in the form with running maxima and the difference first.
+constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f;
+constexpr float kFloor = -1.0e30f;  // stands for -inf where t is multiplied: the weight is zero either way, and zero times it is zero
+
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void halves(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
 }
 
+// A 16-byte piece as pairs of FP32 values; kFloored: -inf (and anything below kFloor) becomes a finite value, NaN stays
 template <typename T>
-__global__ void __launch_bounds__(kThreads) policy_kernel(const NxTokenRows a, const NxPolicyArgs g, const double* __restrict__ totals,
-                                                          const int32_t* __restrict__ counts, float* __restrict__ logp, float* __restrict__ kl, float* __restrict__ entropy,
-                                                          float* __restrict__ row_loss, T* __restrict__ grad) {
-  __shared__ float scratch[32];
+struct PieceOf;
+template <>
+struct PieceOf<__nv_bfloat16> {
+  static constexpr int kPairs = 4;
+  template <bool kFloored>
+  static __device__ __forceinline__ void get(const uint4& q, Pair (&p)[4]) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kFloored) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xf149f149u));  // -1e30
+      p[i] = pair_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+  }
+};
+template <>
+struct PieceOf<__half> {
+  static constexpr int kPairs = 4;
+  template <bool kFloored>
+  static __device__ __forceinline__ void get(const uint4& q, Pair (&p)[4]) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kFloored) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xfbfffbffu));  // -65504
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      p[i] = pair_of(f.x, f.y);
+    }
+  }
+};
+template <>
+struct PieceOf<float> {
+  static constexpr int kPairs = 2;
+  template <bool kFloored>
+  static __device__ __forceinline__ void get(const uint4& q, Pair (&p)[2]) {
+    float v[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
+    if (kFloored) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(v[i]) : "f"(kFloor));
+    }
+    p[0] = pair_of(v[0], v[1]);
+    p[1] = pair_of(v[2], v[3]);
+  }
+};
+
+template <bool kEntropy>
+struct Fast {
+  Pair s{0}, h{0};
+  template <typename T>
+  __device__ __forceinline__ void absorb(const uint4& q, Pair kk, Pair minus_base) {
+    constexpr int N = PieceOf<T>::kPairs;
+    Pair p[N];
+    PieceOf<T>::template get<kEntropy>(q, p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const Pair t = fma2(p[i], kk, minus_base);
+      float a, b;
+      halves(t, a, b);
+      const Pair e = pair_of(ex2_approx(a), ex2_approx(b));
+      s = add2(s, e);
+      if (kEntropy) h = fma2(t, e, h);
+    }
+  }
+  __device__ __forceinline__ void absorb_one(float v, float k, float base) {
+    if (kEntropy) asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(kFloor));
+    const float t = fmaf(v, k, -base), e = ex2_approx(t);
+    s = add2(s, pair_of(e, 0.0f));
+    if (kEntropy) h = fma2(pair_of(t, 0.0f), pair_of(e, 0.0f), h);
+  }
+};
+
+// What the producer has gathered of a row by the time the workers come to it.
+struct RowInfo {
+  int64_t at;       // offset of the row in elements
+  int32_t target;   // -1: ignored, -2: outside the vocabulary
+  float x;          // the target's logit
+  PolicyIn in;
+};
+// What the row's end makes of its sums, for every worker's second pass.
+struct RowEnd {
+  float c, c1, es, eb;   // g = 2^t (es t + eb), without an entropy term 2^t c1; c more at the target
+  int32_t careful;
+  float m, log2_s, slope, off;  // careful: g = 2^((v - m) k - log2_s) (slope (v - m) + off)
+};
+constexpr int kAhead = 4;
+template <typename S>
+struct RingSpace {
+  RowInfo info[kAhead];
+  RowEnd end;
+  float4 warps[S::kWorkers / 32];    // (m, s, h) of each warp
+  float4 blocks[2][kMaxCuts];        // of each block of the cluster, in turns
+  uint64_t full[S::kSlots], empty[S::kSlots], told[kAhead], heard[kAhead];
+  uint64_t arrived;                  // counts the blocks that have put theirs in
+  int abort_word;
+};
+
+template <typename S>
+__device__ __forceinline__ void workers_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(S::kWorkers) : "memory");
+}
+
+// s and h are relative to a maximum m: brings them to `top`, differences in units of the logits
+__device__ __forceinline__ void weigh(float4& v, float top, float k) {
+  if (v.x == -INFINITY) return;  // nothing but -inf: zero (or NaN) as it is
+  const float d = fmaxf(v.x - top, kFloor), f = ex2_approx(d * k);
+  v.z = fmaf(d, v.y, v.z) * f;
+  v.y *= f;
+}
+// (m, s, h) of 2^n lanes together; kMaxima: s and h are relative to m, otherwise m is not used
+template <bool kMaxima, int kLanes>
+__device__ __forceinline__ void join_lanes(float4& v, float k) {
+  if (kMaxima) {
+    float top = v.x;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    weigh(v, top, k);
+    v.x = top;
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) {
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+  }
+}
+
+// Joins all threads' and blocks' sums of a row; the first warp gets them.
+template <bool kMaxima, typename S>
+__device__ __forceinline__ float4 join_all(float4 v, float k, RingSpace<S>* sp, int rank, int cuts, int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  join_lanes<kMaxima, 32>(v, k);
+  if (lane == 0) sp->warps[warp] = v;
+  workers_sync<S>();
+  const int side = turn & 1;
+  if (cuts > 1) ++turn;
+  if (warp != 0) return v;
+  v = sp->warps[lane & (S::kWorkers / 32 - 1)];
+  join_lanes<kMaxima, S::kWorkers / 32>(v, k);
+  if (cuts > 1) {
+    if (lane < cuts) {  // a lane per block of the cluster
+      const uint32_t to = mapa_shared(smem_u32(&sp->blocks[side][rank]), lane);
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+      mbar_arrive_cluster(mapa_shared(smem_u32(&sp->arrived), lane));
+    }
+    uint32_t done = 0, tries = 0;
+    uint64_t began = 0;
+    while (!done) {
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(smem_u32(&sp->arrived)), "r"(static_cast<uint32_t>(side))
+          : "memory");
+      if (!done && (++tries & 63u) == 0) {
+        const uint64_t now = globaltimer_ns();
+        if (began == 0) began = now;
+        if (*static_cast<volatile int*>(&sp->abort_word) != 0 || now - began > NX_WAIT_LIMIT_NS) {
+          *static_cast<volatile int*>(&sp->abort_word) = 1;
+          break;
+        }
+      }
+    }
+    __syncwarp();
+    v = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    if ((lane & (kMaxCuts - 1)) < cuts) v = sp->blocks[side][lane & (kMaxCuts - 1)];
+    join_lanes<kMaxima, kMaxCuts>(v, k);
+  }
+  return v;
+}
+
+struct RingOut {
+  float* logp;
+  float2* stats;     // token log-probabilities: a logit x, log2 of the sum of exp((logit - x) inv_temp)
+  float* kl;
+  float* entropy;
+  float* row_loss;
+  const double* totals;
+  const int32_t* counts;
+  int* status;
+  int cuts;
+};
+
+template <typename T, bool kPolicy, typename S>
+__global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const NxTokenRows a, const NxPolicyArgs g, const RingOut o, T* __restrict__ grad) {
+  constexpr int kWorkers = S::kWorkers, kSlots = S::kSlots;
+  constexpr int VN = RowVec<T>::kN, kPer = kSlotPieces / kWorkers;
+  extern __shared__ __align__(128) uint8_t ring_smem[];
+  __shared__ __align__(16) RingSpace<S> space;
+  RingSpace<S>* const sp = &space;
+  volatile int* const abort_flag = &space.abort_word;
+  const int cuts = o.cuts, rank = cuts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const uint32_t rows = static_cast<uint32_t>(a.rows), first = blockIdx.x / cuts, step = gridDim.x / cuts;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&sp->full[s], 1);
+      mbar_init(&sp->empty[s], kWorkers / 32);
+    }
+    for (int s = 0; s < kAhead; ++s) {
+      mbar_init(&sp->told[s], 1);
+      mbar_init(&sp->heard[s], kWorkers / 32);
+    }
+    mbar_init(&sp->arrived, static_cast<uint32_t>(cuts));
+    sp->abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (cuts > 1) cluster_sync_all();  // the others' barriers exist
   pdl_dependency();
   pdl_trigger();
-  const int64_t row = blockIdx.x;
-  const int64_t tg = target_at(a.targets, a.targets_wide, row);
-  const int64_t at = row_offset(a, row);
-  if (tg == a.ignore_index || tg < 0 || tg >= a.vocab) {
-    if (threadIdx.x == 0) {
-      const float v = tg == a.ignore_index ? 0.0f : NAN;
-      logp[row] = kl[row] = entropy[row] = row_loss[row] = v;
-    }
-    if (g.write_grad) clear_row(grad + at, a.width);
-    return;
-  }
-  const float weight = policy_weight(g, totals, counts, row);
-  const T* p = reinterpret_cast<const T*>(a.logits) + at;
+
+  const bool second = kPolicy && g.write_grad;
+  // slots of `n` pieces that are freed in the first pass: all without a second one; with one, those that the ring has no room for (and of a long
+  // row two more, so that copies go on while the sums are joined)
+  auto freed = [&](int n) {
+    const int all = (n + kSlotPieces - 1) / kSlotPieces;
+    return !second ? all : (all <= kSlots ? 0 : all - (kSlots - 2));
+  };
   const float k = a.inv_temp * kLog2e;
-  Online<true> on;
-  absorb_row(p, a.vocab, k, on);
-  join_block(on, k, scratch);
-  const float ln_s = logf(on.s), log2_s = log2f(on.s);
-  const float lp = (Num<T>::load(p + tg) - on.m) * a.inv_temp - ln_s;
-  const float ent = ln_s - on.h / on.s * a.inv_temp;
-  const PolicyRow r = policy_row(g, row, lp, ent, weight);
-  if (threadIdx.x == 0) {
-    logp[row] = lp;
-    kl[row] = r.kl;
-    entropy[row] = ent;
-    row_loss[row] = r.loss;
-  }
-  if (!g.write_grad) return;
-  const float c = r.c * a.inv_temp;
-  if (g.entropy_coef == 0.0f) {
-    write_row(p, grad + at, a.vocab, a.width, static_cast<int>(tg), c,
-              [&](float v) { return -c * ex2_approx(fmaf(v - on.m, k, -log2_s)); });
+  const int shift = 31 - __clz(cuts);  // cuts is a power of two
+  // this block's pieces of a row
+  auto share = [&](const RowSplit<T>& r, int& lo, int& n) {
+    lo = static_cast<int>(static_cast<uint64_t>(r.pieces) * rank >> shift);
+    n = static_cast<int>(static_cast<uint64_t>(r.pieces) * (rank + 1) >> shift) - lo;
+  };
+
+  if (threadIdx.x >= kWorkers) {
+    // The copying warp: 32 rows at a time, a lane gathers what is known of one; then the first lane tells the workers and fills slots, row by row.
+    const int lane = threadIdx.x & 31;
+    int slot = 0, seat = 0;
+    uint32_t phase = 0, seat_phase = 0;
+    bool ok = true;
+    for (uint64_t batch = first; batch < rows; batch += 32ull * step) {
+      const uint64_t row = batch + static_cast<uint64_t>(lane) * step;
+      RowInfo info{};
+      info.target = -1;
+      if (row < rows) {
+        const uint32_t r = static_cast<uint32_t>(row);
+        const int64_t tg = target_at(a.targets, a.targets_wide, r);
+        info.at = row_offset(a, r);
+        info.target = tg == a.ignore_index ? -1 : (tg < 0 || tg >= a.vocab ? -2 : static_cast<int32_t>(tg));
+        if (info.target >= 0) {
+          info.x = Num<T>::load(reinterpret_cast<const T*>(a.logits) + info.at + info.target);
+          if (kPolicy) info.in = policy_in(g, o.totals, o.counts, r);
+        }
+      }
+      const int here = static_cast<int>(min(static_cast<uint64_t>(32), (rows - batch + step - 1) / step));
+      for (int j = 0; j < here; ++j) {
+        const int32_t tg = __shfl_sync(0xffffffffu, info.target, j);
+        const int64_t at = __shfl_sync(0xffffffffu, info.at, j);
+        ok = ok && mbar_wait_bounded(&sp->heard[seat], seat_phase ^ 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          if (lane == j) sp->info[seat] = info;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sp->told[seat]);
+        }
+        if (++seat == kAhead) {
+          seat = 0;
+          seat_phase ^= 1u;
+        }
+        if (lane == 0 && ok && tg >= 0) {
+          const T* p = reinterpret_cast<const T*>(a.logits) + at;
+          const RowSplit<T> r(p, a.vocab);
+          int lo, n;
+          share(r, lo, n);
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(p + r.head) + static_cast<int64_t>(lo) * 16;
+          const int slots = (n + kSlotPieces - 1) / kSlotPieces, loads = slots + (second ? freed(n) : 0);
+          for (int d = 0; d < loads; ++d) {
+            const int c = (d < slots ? d : d - slots) * kSlotPieces;
+            if (!mbar_wait_bounded(&sp->empty[slot], phase ^ 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bytes = static_cast<uint32_t>(min(kSlotPieces, n - c)) * 16;
+            mbar_arrive_expect_tx(&sp->full[slot], bytes);
+            bulk_load(ring_smem + slot * kSlotBytes, src + static_cast<int64_t>(c) * 16, bytes, &sp->full[slot]);
+            if (++slot == kSlots) {
+              slot = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      if (!ok) break;
+    }
+    if (!ok && lane == 0) atomicCAS(o.status, 0, kStatusTimeoutProducer);
   } else {
-    const float e1 = r.ent * a.inv_temp, slope = e1 * a.inv_temp, base = e1 * (ent - ln_s) - c;
-    write_row(p, grad + at, a.vocab, a.width, static_cast<int>(tg), c, [&](float v) {
-      float d = v - on.m;
-      asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(-1e30f));
-      return ex2_approx(fmaf(d, k, -log2_s)) * fmaf(d, slope, base);
-    });
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int slot = 0, turn = 0, seat = 0;
+    uint32_t phase = 0, seat_phase = 0;
+    bool fine = true;
+    auto wait = [&](uint64_t* bar, uint32_t ph) { fine = mbar_wait_bounded(bar, ph, abort_flag) && fine; };
+    auto release = [&](int s) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sp->empty[s]);
+    };
+    const Pair kk = pair_of(k, k);
+    for (uint64_t row = first; row < rows; row += step) {
+      wait(&sp->told[seat], seat_phase);
+      const int32_t tg = sp->info[seat].target;
+      const int64_t at = sp->info[seat].at;
+      const float xt = sp->info[seat].x;
+      PolicyIn in{};
+      if (kPolicy && warp == 0) in = sp->info[seat].in;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sp->heard[seat]);
+      if (++seat == kAhead) {
+        seat = 0;
+        seat_phase ^= 1u;
+      }
+      if (tg < 0) {
+        if (rank == 0 && tid == 0) {
+          const float v = tg == -1 ? 0.0f : NAN;
+          o.logp[row] = v;
+          if (kPolicy) o.kl[row] = o.entropy[row] = o.row_loss[row] = v;
+          else o.stats[row] = make_float2(0.0f, 0.0f);
+        }
+        if (second) {
+          T* gr = grad + at;
+          const RowSplit<T> r(gr, a.width);
+          for (int i = rank * kWorkers + tid; i < r.pieces; i += cuts * kWorkers)
+            *reinterpret_cast<uint4*>(gr + r.head + static_cast<int64_t>(i) * VN) = make_uint4(0, 0, 0, 0);
+          if (rank == 0 && tid < r.head) Num<T>::store(gr + tid, 0.0f);
+          if (rank == 0 && tid >= 32 && tid - 32 < r.tail) Num<T>::store(gr + r.head + static_cast<int64_t>(r.pieces) * VN + tid - 32, 0.0f);
+        }
+        continue;
+      }
+      const T* p = reinterpret_cast<const T*>(a.logits) + at;
+      const RowSplit<T> r(p, a.vocab);
+      int lo, n;
+      share(r, lo, n);
+      // single elements before the first and behind the last piece: one per thread of the first block
+      int edge = -1;
+      if (rank == 0) {
+        if (tid < r.head) edge = tid;
+        else if (tid >= 32 && tid - 32 < r.tail) edge = r.head + r.pieces * VN + tid - 32;
+      }
+      const float ev = edge >= 0 ? Num<T>::load(p + edge) : 0.0f;
+      const float base = xt * k;
+      const Pair bb = pair_of(-base, -base);
+
+      Fast<kPolicy> on;
+      const int slots = (n + kSlotPieces - 1) / kSlotPieces, free_now = freed(n);
+      int s = slot, c = 0;
+      uint32_t ph = phase;
+      auto next = [&] {
+        if (++s == kSlots) {
+          s = 0;
+          ph ^= 1u;
+        }
+        if (c / kSlotPieces + 1 == free_now) {  // the first slot that stays is the next one
+          slot = s;
+          phase = ph;
+        }
+      };
+      for (; c + kSlotPieces <= n; c += kSlotPieces) {
+        wait(&sp->full[s], ph);
+        const uint4* data = reinterpret_cast<const uint4*>(ring_smem + s * kSlotBytes) + tid;
+        uint4 q[kPer];
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) q[u] = data[u * kWorkers];
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) on.template absorb<T>(q[u], kk, bb);
+        if (c < free_now * kSlotPieces) release(s);
+        next();
+      }
+      if (c < n) {
+        wait(&sp->full[s], ph);
+        const uint4* data = reinterpret_cast<const uint4*>(ring_smem + s * kSlotBytes);
+        for (int i = tid; i < n - c; i += kWorkers) on.template absorb<T>(data[i], kk, bb);
+        if (c < free_now * kSlotPieces) release(s);
+        next();
+      }
+      if (edge >= 0) on.absorb_one(ev, k, base);
+      float s0, s1, h0, h1;
+      halves(on.s, s0, s1);
+      halves(on.h, h0, h1);
+      float4 st = join_all<false, S>(make_float4(0.0f, s0 + s1, h0 + h1, 0.0f), k, sp, rank, cuts, turn);
+      // The first warp ends the row and tells the others how its gradient comes.  `m`, `sum` and `h` relative to it where done with maxima.
+      auto end_row = [&](const float4& v, bool careful) {
+        RowEnd e{};
+        e.careful = careful;
+        const float ln_s = logf(v.y), log2_s = log2f(v.y), coarse = fmaf(xt, k, -base);  // x_t k - B is the rounding of B
+        const float lp = careful ? (xt - v.x) * a.inv_temp - ln_s : coarse * kLn2 - ln_s;
+        if constexpr (!kPolicy) {
+          if (rank == 0 && lane == 0) {
+            o.logp[row] = lp;
+            o.stats[row] = make_float2(careful ? v.x : xt, log2_s - (careful ? 0.0f : coarse));
+          }
+        } else {
+          const float ent = careful ? ln_s - v.z / v.y * a.inv_temp : ln_s - v.z / v.y * kLn2;
+          const PolicyRow pr = policy_row(g, in, lp, ent);
+          if (rank == 0 && lane == 0) {
+            o.logp[row] = lp;
+            o.kl[row] = pr.kl;
+            o.entropy[row] = ent;
+            o.row_loss[row] = pr.loss;
+          }
+          const float inv_s = 1.0f / v.y, e1 = pr.ent * a.inv_temp;
+          e.c = pr.c * a.inv_temp;
+          e.c1 = -e.c * inv_s;
+          e.es = e1 * inv_s * kLn2;
+          e.eb = e1 * inv_s * (ent - ln_s) + e.c1;
+          e.m = v.x;
+          e.log2_s = log2_s;
+          e.slope = e1 * a.inv_temp;
+          e.off = g.entropy_coef != 0.0f ? e1 * (ent - ln_s) - e.c : -e.c;
+          if (lane == 0) sp->end = e;
+        }
+      };
+      if (warp == 0) {
+        const bool careful = !(fabsf(xt) <= kFastLimit && st.y <= kFastSum);
+        if (!careful) end_row(st, false);
+        else if (lane == 0) sp->end.careful = 1;
+        if (!kPolicy && !careful && lane == 0) sp->end.careful = 0;
+      }
+      workers_sync<S>();
+      if (sp->end.careful) {  // the same in every block of the cluster; from memory, with maxima and the difference first
+        Online<true> on2;
+        const T* body = p + r.head + static_cast<int64_t>(lo) * VN;
+        for (int i = tid; i < n; i += kWorkers) {
+          float v[VN];
+          RowVec<T>::load(body + static_cast<int64_t>(i) * VN, v);
+          on2.absorb(v, k);
+        }
+        if (edge >= 0) {
+          const float v[1] = {ev};
+          on2.absorb(v, k);
+        }
+        st = join_all<true, S>(make_float4(on2.m, on2.s, on2.h, 0.0f), k, sp, rank, cuts, turn);
+        if (warp == 0) end_row(st, true);
+        workers_sync<S>();
+      }
+      if (kPolicy && second) {
+        const RowEnd e = sp->end;
+        T* gr = grad + at;
+        const int col0 = r.head + lo * VN;
+        if (e.careful) {
+          auto one = [&](float v) {
+            float d = v - e.m;
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(kFloor));
+            return ex2_approx(fmaf(d, k, -e.log2_s)) * (g.entropy_coef != 0.0f ? fmaf(d, e.slope, e.off) : e.off);
+          };
+          for (int i = tid; i < n; i += kWorkers) {
+            float v[VN];
+            RowVec<T>::load(p + col0 + static_cast<int64_t>(i) * VN, v);
+#pragma unroll
+            for (int j = 0; j < VN; ++j) v[j] = one(v[j]) + (col0 + i * VN + j == tg ? e.c : 0.0f);
+            RowVec<T>::store(gr + col0 + static_cast<int64_t>(i) * VN, v);
+          }
+          if (edge >= 0) Num<T>::store(gr + edge, one(ev) + (edge == tg ? e.c : 0.0f));
+          for (int d = 0; d < slots; ++d) {  // the slots were not needed
+            wait(&sp->full[slot], phase);
+            release(slot);
+            if (++slot == kSlots) {
+              slot = 0;
+              phase ^= 1u;
+            }
+          }
+        } else {
+          const Pair cc = pair_of(e.c1, e.c1), ee = pair_of(e.es, e.es), eo = pair_of(e.eb, e.eb);
+          uint4* const out = reinterpret_cast<uint4*>(gr + col0);
+          auto second_pass = [&](auto entropy) {
+            constexpr bool kEnt = decltype(entropy)::value;
+            auto piece = [&](int i, const uint4& q) {
+              constexpr int N = PieceOf<T>::kPairs;
+              Pair v[N];
+              PieceOf<T>::template get<kEnt>(q, v);
+              float w[VN];
+#pragma unroll
+              for (int u = 0; u < N; ++u) {
+                const Pair t = fma2(v[u], kk, bb);
+                float x, y;
+                halves(t, x, y);
+                const Pair ex = pair_of(ex2_approx(x), ex2_approx(y));
+                halves(mul2(ex, kEnt ? fma2(t, ee, eo) : cc), w[2 * u], w[2 * u + 1]);
+              }
+              RowVec<T>::store(reinterpret_cast<T*>(out + i), w);
+            };
+            for (int d = free_now; d < slots + free_now; ++d) {  // those that stayed, then those that come again
+              c = (d < slots ? d : d - slots) * kSlotPieces;
+              const uint4* data = reinterpret_cast<const uint4*>(ring_smem + slot * kSlotBytes);
+              if (d >= slots) wait(&sp->full[slot], phase);
+              if (c + kSlotPieces <= n) {
+                uint4 q[kPer];
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) q[u] = data[tid + u * kWorkers];
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) piece(c + tid + u * kWorkers, q[u]);
+              } else {
+                for (int i = tid; i < n - c; i += kWorkers) piece(c + i, data[i]);
+              }
+              release(slot);
+              if (++slot == kSlots) {
+                slot = 0;
+                phase ^= 1u;
+              }
+            }
+          };
+          if (g.entropy_coef != 0.0f) second_pass(std::true_type{});
+          else second_pass(std::false_type{});
+          auto single = [&](float v) {
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(kFloor));
+            const float t = fmaf(v, k, -base);
+            return ex2_approx(t) * (g.entropy_coef != 0.0f ? fmaf(t, e.es, e.eb) : e.c1);
+          };
+          if (edge >= 0 && edge != tg) Num<T>::store(gr + edge, single(ev));
+          // The target's element, by the thread that wrote its piece (or has it at the edge): once more, with c added before it is rounded.
+          const int off = tg - col0;
+          const bool at_edge = edge == tg;
+          const bool in_piece = off >= 0 && off < n * VN && (off / VN) % kWorkers == tid;
+          if (at_edge || in_piece) Num<T>::store(gr + tg, single(xt) + e.c);
+        }
+        for (int w = a.vocab + rank * kWorkers + tid; w < a.width; w += cuts * kWorkers) Num<T>::store(gr + w, 0.0f);
+      }
+    }
+    if (!fine) atomicCAS(o.status, 0, kStatusTimeoutEpilogue);
+  }
+  __syncthreads();
+  if (*abort_flag != 0) {  // a wait ran out: copies still in flight land before the shared memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(2000);
+  }
+  if (cuts > 1) cluster_sync_all();  // no block leaves while another may still write to it
+}
+
+// Blocks that a row is cut over, while rows are too few for the SMs
+inline int cuts_for(int64_t rows, int64_t pieces) {
+  int cuts = 1;
+  while (cuts < kMaxCuts && rows * cuts < kNumSmsB200 && pieces / cuts >= 512) cuts *= 2;
+  return cuts;
+}
+
+template <typename T, bool kPolicy, typename S>
+int launch_shape(const NxTokenRows& a, const NxPolicyArgs& g, RingOut o, T* grad, cudaStream_t st) {
+  auto kern = ring_kernel<T, kPolicy, S>;
+  constexpr int kRingBytes = S::kSlots * kSlotBytes;
+  NX_ALLOW_SMEM(kern, kRingBytes);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(o.cuts);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = kRingBytes;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = o.cuts > 1 ? 2 : 1;
+  // All clusters at the same time: the GPCs' SMs do not divide by four and eight, and a cluster left over would double the time.
+  static std::atomic<int> resident[4];
+  int at = 0;
+  while ((1 << at) < o.cuts) ++at;
+  int most = o.cuts == 1 ? S::kResident * kNumSmsB200 : resident[at].load(std::memory_order_relaxed);
+  if (most == 0) {
+    cfg.gridDim = dim3(static_cast<unsigned>(S::kResident * kNumSmsB200 / o.cuts * o.cuts));
+    if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess || most < 1) {
+      (void)cudaGetLastError();
+      return -2;
+    }
+    resident[at].store(most, std::memory_order_relaxed);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, most) * o.cuts));
+  if (cudaLaunchKernelEx(&cfg, kern, a, g, o, grad) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return -2;
+  }
+  return 0;
+}
+
+template <typename T, bool kPolicy>
+int launch_ring(const NxTokenRows& a, const NxPolicyArgs& g, RingOut o, T* grad, cudaStream_t st) {
+  const int64_t pieces = static_cast<int64_t>(a.vocab) * sizeof(T) / 16;
+  o.cuts = cuts_for(a.rows, pieces);
+  if constexpr (!kPolicy) {
+    return launch_shape<T, false, SumsShape>(a, g, o, grad, st);
+  } else {
+    if (!g.write_grad) return launch_shape<T, true, SumsShape>(a, g, o, grad, st);
+    if ((pieces + o.cuts - 1) / o.cuts + 1 <= ShortShape::kSlots * kSlotPieces) return launch_shape<T, true, ShortShape>(a, g, o, grad, st);
+    return launch_shape<T, true, LongShape>(a, g, o, grad, st);
   }
 }
 
@@ -423,7 +957,7 @@ preference_kernel(const NxPreferenceArgs a, float* __restrict__ seq_logp, float*
   cluster_arrive();
   pdl_dependency();
   pdl_trigger();
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = cluster_ctarank();
   const bool by_block = a.seq_len >= 256;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t first = by_block ? rank : rank * 32 + warp, step = by_block ? kJoinBlocks : kJoinBlocks * 32;
@@ -486,9 +1020,11 @@ preference_kernel(const NxPreferenceArgs a, float* __restrict__ seq_logp, float*
 }
 
 bool rows_ok(const NxTokenRows* a) {
-  return a != nullptr && a->rows >= 0 && a->rows <= 0x7fffffff && a->per > 0 && a->vocab > 0 && a->vocab <= a->width &&
+  return a != nullptr && a->rows >= 0 && a->rows <= 0x7fffffff && a->per > 0 && a->per <= 0x7fffffff && a->vocab > 0 && a->vocab <= a->width &&
          (a->rows == 0 || (a->logits != nullptr && a->targets != nullptr));
 }
+// the kernels write a row's gradient in the pieces that they read it in
+bool same_lines(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
 }  // namespace
 
 #define NX_BY_TYPE(CODE_, ...)               \
@@ -512,17 +1048,19 @@ bool rows_ok(const NxTokenRows* a) {
       return -1;                             \
   }
 
-extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats, nx_stream_t stream) {
-  if (!rows_ok(a) || logp == nullptr || stats == nullptr) return -1;
+extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats, int* status, nx_stream_t stream) {
+  if (!rows_ok(a) || logp == nullptr || stats == nullptr || status == nullptr) return -1;
   if (a->rows == 0) return 0;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  NX_BY_TYPE(a->dtype, NX_PDL((token_stats_kernel<T>), a->rows, kThreads, 0, st, *a, logp, reinterpret_cast<float2*>(stats)))
-  return 0;
+  RingOut o{};
+  o.logp = logp;
+  o.stats = reinterpret_cast<float2*>(stats);
+  o.status = status;
+  NX_BY_TYPE(a->dtype, return launch_ring<T, false>(*a, NxPolicyArgs{}, o, nullptr, static_cast<cudaStream_t>(stream)))
 }
 
 extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, const float* coef, int64_t coef_per, const float* factor,
                                       void* grad, nx_stream_t stream) {
-  if (!rows_ok(a) || stats == nullptr || coef == nullptr || coef_per < 1 || grad == nullptr) return -1;
+  if (!rows_ok(a) || stats == nullptr || coef == nullptr || coef_per < 1 || coef_per > 0x7fffffff || grad == nullptr || !same_lines(a->logits, grad)) return -1;
   if (a->rows == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   NX_BY_TYPE(a->dtype, NX_PDL((token_grad_kernel<T>), a->rows, kThreads, 0, st, *a, reinterpret_cast<const float2*>(stats), coef, coef_per,
@@ -531,15 +1069,27 @@ extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, 
 }
 
 extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, double* totals, int32_t* counts, float* logp, float* kl,
-                              float* entropy, float* row_loss, float* loss, void* grad, nx_stream_t stream) {
-  if (!rows_ok(a) || g == nullptr || totals == nullptr || counts == nullptr || loss == nullptr || g->adv_per < 1 || g->seq_len < 1 ||
-      a->rows % g->seq_len != 0 || (g->write_grad && grad == nullptr))
+                              float* entropy, float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream) {
+  if (!rows_ok(a) || g == nullptr || totals == nullptr || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
+      g->seq_len < 1 || g->seq_len > 0x7fffffff ||
+      a->rows % g->seq_len != 0 || (g->write_grad && a->rows > 0 && (grad == nullptr || !same_lines(a->logits, grad))))
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (g->mean != NX_MEAN_NONE)
     NX_PDL(token_count_kernel, kJoinBlocks, kJoinThreads, 0, st, a->targets, a->targets_wide, a->rows / g->seq_len, g->seq_len, a->ignore_index, totals, counts);
-  if (a->rows > 0)
-    NX_BY_TYPE(a->dtype, NX_PDL((policy_kernel<T>), a->rows, kThreads, 0, st, *a, *g, totals, counts, logp, kl, entropy, row_loss, static_cast<T*>(grad)))
+  if (a->rows > 0) {
+    RingOut o{};
+    o.logp = logp;
+    o.kl = kl;
+    o.entropy = entropy;
+    o.row_loss = row_loss;
+    o.totals = totals;
+    o.counts = counts;
+    o.status = status;
+    int rc = 0;
+    NX_BY_TYPE(a->dtype, rc = (launch_ring<T, true>(*a, *g, o, static_cast<T*>(grad), st)))
+    if (rc != 0) return rc;
+  }
   NX_PDL(sum_kernel, kJoinBlocks, kJoinThreads, 0, st, row_loss, a->rows, loss);
   return 0;
 }

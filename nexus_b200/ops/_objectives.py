@@ -89,7 +89,8 @@ def token_logprobs(rows: TokenRows, device):
     """FP32 (logp [rows], stats [rows, 2])."""
     logp = torch.empty(rows.rows, dtype=torch.float32, device=device)
     stats = torch.empty((rows.rows, 2), dtype=torch.float32, device=device)
-    K._check(K.lib().nx_token_logprobs(C.byref(rows), K._p(logp), K._p(stats), K._stream()), "nx_token_logprobs")
+    K._check(K.lib().nx_token_logprobs(C.byref(rows), K._p(logp), K._p(stats), K._p(K.status_word(device)), K._stream()),
+             "nx_token_logprobs")
     return logp, stats
 
 
@@ -107,7 +108,8 @@ def policy_loss(rows: TokenRows, args: PolicyArgs, device, grad):
     totals = torch.empty(2 + (sequences + 1) // 2, dtype=torch.float64, device=device)
     args.write_grad = int(grad is not None)
     K._check(K.lib().nx_policy_loss(C.byref(rows), C.byref(args), K._p(totals), C.c_void_p(totals.data_ptr() + 16), K._p(per_row[0]),
-                                    K._p(per_row[1]), K._p(per_row[2]), K._p(per_row[3]), K._p(loss), K._p(grad), K._stream()),
+                                    K._p(per_row[1]), K._p(per_row[2]), K._p(per_row[3]), K._p(loss), K._p(grad),
+                                    K._p(K.status_word(device)), K._stream()),
              "nx_policy_loss")
     return loss, per_row[0], per_row[1], per_row[2]
 
