@@ -207,8 +207,6 @@ int run(const NxGradTable* g, double max_norm, int clip, double* partial, double
 }
 }  // namespace
 
-extern "C" int64_t nx_grad_clip_partials(int64_t tensors) { return (tensors + kTableMax - 1) / kTableMax * kClipBlocks; }
-
 extern "C" int nx_grad_clip(const NxGradTable* g, double max_norm, int clip, double* partial, double* out, nx_stream_t stream) {
   if (g == nullptr || g->tensors < 1 || g->src == nullptr || g->count == nullptr || g->type == nullptr || partial == nullptr || out == nullptr ||
       !(max_norm >= 0.0))

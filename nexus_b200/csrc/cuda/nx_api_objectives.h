@@ -106,7 +106,7 @@ typedef struct NxGradTable {
   const uint8_t* type;
   int64_t tensors;
 } NxGradTable;
-int64_t nx_grad_clip_partials(int64_t tensors);  // doubles of scratch
+// partial: 592 doubles per 256 tensors or part of them.
 // out[0] = sum of squares; (float*)(out + 1) = norm = sqrt of it.  clip: the gradients times min(1, max_norm / (norm + 1e-6)); where the norm
 // is not finite they stay (dst: are copied) as they are.  Sums in a fixed order.
 int nx_grad_clip(const NxGradTable* table, double max_norm, int clip, double* partial, double* out, nx_stream_t stream);

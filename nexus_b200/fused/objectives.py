@@ -10,6 +10,7 @@ takes its token out of everything (prompts, padding): its results and gradients 
 hold.  A target outside the vocabulary gives NaN and a gradient of zeros.  Statistics are FP32; sums over tokens FP64."""
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import List, NamedTuple, Optional, Sequence
 
@@ -17,6 +18,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 _KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_KERNEL_SET = set(_KERNEL_TYPES)
+_TARGET_TYPES = (torch.int32, torch.int64)
+O = None     # nexus_b200.ops._objectives, once a tensor on a GPU has been met
 
 
 class PolicyLoss(NamedTuple):
@@ -37,45 +41,63 @@ class PreferenceLoss(NamedTuple):
 
 
 def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature: float) -> int:
-    if not torch.is_floating_point(logits) or logits.dim() < 1:
+    if not logits.is_floating_point() or logits.dim() < 1:
         raise ValueError(f"{name}: logits must be a floating-point tensor [..., vocabulary]")
-    if targets.dtype not in (torch.int32, torch.int64):
+    shape = logits.shape
+    if targets.dtype not in _TARGET_TYPES:
         raise ValueError(f"{name}: targets must be int32 or int64, got {targets.dtype}")
-    if targets.shape != logits.shape[:-1]:
-        raise ValueError(f"{name}: targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
+    if targets.shape != shape[:-1]:
+        raise ValueError(f"{name}: targets {tuple(targets.shape)} do not match logits {tuple(shape)}")
     if targets.device != logits.device:
         raise ValueError(f"{name}: targets on {targets.device}, logits on {logits.device}")
     _check_temperature(name, temperature)
-    V = logits.shape[-1] if vocab is None else int(vocab)
-    if not 1 <= V <= logits.shape[-1]:
-        raise ValueError(f"{name}: vocab must be between 1 and {logits.shape[-1]}, got {V}")
-    if logits.shape[-1] >= 2 ** 31 or targets.numel() >= 2 ** 31:
+    V = shape[-1] if vocab is None else int(vocab)
+    if not 1 <= V <= shape[-1]:
+        raise ValueError(f"{name}: vocab must be between 1 and {shape[-1]}, got {V}")
+    if shape[-1] >= 2 ** 31 or targets.numel() >= 2 ** 31:
         raise ValueError(f"{name}: at most 2^31 - 1 rows and columns")
     return V
 
 
 def _check_temperature(name: str, temperature: float) -> None:
-    if not (math.isfinite(temperature) and temperature > 0.0):
+    if not 0.0 < temperature < math.inf:
         raise ValueError(f"{name}: temperature must be positive, got {temperature}")
 
 
 def _check_values(name: str, what: str, t, shapes, device) -> torch.Tensor:
     """A tensor of constants of the loss in FP32: log-probabilities, advantages."""
-    if not torch.is_tensor(t) or not torch.is_floating_point(t):
+    if not isinstance(t, torch.Tensor) or not t.is_floating_point():
         raise ValueError(f"{name}: {what} must be a floating-point tensor")
-    if tuple(t.shape) not in shapes:
+    if t.shape not in shapes:
         raise ValueError(f"{name}: {what} must have the shape {' or '.join(map(str, shapes))}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name}: {what} on {t.device}, logits on {device}")
-    return t.detach().float().contiguous()
+    if t.requires_grad:
+        t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """Makes a tensor's device the current one, where it is not: the launches go to the current device's stream."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _kernels(t: torch.Tensor) -> bool:
     if not t.is_cuda or t.dtype not in _KERNEL_TYPES:
         return False
-    from ..ops import _cuda as K
-    K.lib()  # raises loudly when the library is missing on a GPU machine
+    global O
+    if O is None:
+        from ..ops import _cuda, _objectives
+        _cuda.lib()  # raises loudly when the library is missing on a GPU machine
+        O = _objectives
     return True
+
+
+def _wants(*ts: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
 
 def _token_parts(logits, targets, ignore_index, temperature, V):
@@ -93,26 +115,28 @@ def _token_parts(logits, targets, ignore_index, temperature, V):
 
 
 # ------------------------------------------------------------------------------------- log-probabilities of given tokens
+def _token_forward(logits, targets, vocab, ignore_index, temperature):
+    with _on(logits):
+        logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+        return (logits, targets, *O.token_logprobs(rows, targets))
+
+
 class _TokenLogprobs(torch.autograd.Function):
-    """One read of the logits forward (largest logit and sum per row are kept), one read and one write backward."""
+    """One read of the logits forward (one logit and a sum per row are kept), one read and one write backward."""
 
     @staticmethod
     def forward(ctx, logits, targets, vocab, ignore_index, temperature):
-        from ..ops import _objectives as O
-        with torch.cuda.device(logits.device):
-            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
-            logp, stats = O.token_logprobs(rows, logits.device)
+        logits, targets, logp, stats = _token_forward(logits, targets, vocab, ignore_index, temperature)
         ctx.save_for_backward(logits, targets, stats)
         ctx.cfg = (vocab, ignore_index, temperature)
-        return logp.view(targets.shape)
+        return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
-        from ..ops import _objectives as O
         logits, targets, stats = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
-        with torch.cuda.device(logits.device):
+        with _on(logits):
             logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
             coef = dlogp.float().contiguous()
             grad = O.empty_grad(logits)
@@ -126,35 +150,39 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: in
     `ignore_index`.  Differentiable (once) with respect to the logits; any row strides, the innermost one 1 (others are copied)."""
     V = _check_logits("token_logprobs", logits, targets, vocab, temperature)
     if targets.numel() and _kernels(logits):
-        return _TokenLogprobs.apply(logits, targets, V, ignore_index, float(temperature))
+        if _wants(logits):
+            return _TokenLogprobs.apply(logits, targets, V, ignore_index, float(temperature))
+        return _token_forward(logits, targets, V, ignore_index, temperature)[2]
     return _token_parts(logits, targets, ignore_index, temperature, V)[2].view(targets.shape)
+
+
+def _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, want_grad):
+    with _on(hidden):
+        h, w, t = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight), targets.contiguous()
+        logp, stats, index = O.head_logprobs(h, w, t, vocab, ignore_index, 1.0 / temperature, want_grad)
+    return logp, t, stats, index
 
 
 class _LinearLogprobs(torch.autograd.Function):
     """The logits exist a tile at a time, in tensor memory; the backward pass makes them again."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, vocab, ignore_index, temperature, want_grad):
-        from ..ops import _objectives as O
-        with torch.cuda.device(hidden.device):
-            h, w, t = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight), targets.contiguous()
-            logp, stats, index = O.head_logprobs(h, w, t, vocab, ignore_index, 1.0 / temperature, want_grad)
-        if want_grad:
-            ctx.save_for_backward(hidden, weight, t, stats, index)
+    def forward(ctx, hidden, weight, targets, vocab, ignore_index, temperature):
+        logp, t, stats, index = _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, True)
+        ctx.save_for_backward(hidden, weight, t, stats, index)
         ctx.cfg = (vocab, ignore_index, temperature)
-        return logp.view(targets.shape)
+        return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
-        from ..ops import _objectives as O
         hidden, weight, t, stats, index = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
-        with torch.cuda.device(hidden.device):
+        with _on(hidden):
             h, w = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight)
             dh, dw = O.head_logprobs_grad(h, w, t, vocab, ignore_index, 1.0 / temperature, stats, index, dlogp.float().contiguous(),
                                           ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None, None
+        return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None
 
 
 def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
@@ -180,45 +208,43 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
         raise ValueError(f"{name}: vocab must be between 1 and {weight.shape[0]}, got {V}")
     d, n = hidden.shape[-1], targets.numel()
     if n and d and d % 8 == 0 and hidden.dtype != torch.float32 and max(n, V) <= 1 << 30 and _kernels(hidden):
-        want = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
-        return _LinearLogprobs.apply(hidden, weight, targets, V, ignore_index, float(temperature), want)
+        if _wants(hidden, weight):
+            return _LinearLogprobs.apply(hidden, weight, targets, V, ignore_index, float(temperature))
+        return _linear_forward(hidden, weight, targets, V, ignore_index, temperature, False)[0]
     return token_logprobs(torch.nn.functional.linear(hidden, weight), targets, ignore_index, temperature, V)
 
 
 # ---------------------------------------------------------------------------------------------------------- policy loss
+def _policy_forward(logits, targets, vocab, ignore_index, temperature, args, want_grad):
+    with _on(logits):
+        logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+        grad = O.empty_grad(logits) if want_grad else None
+        return O.policy_loss(rows, args, targets, grad), grad
+
+
 class _PolicyLoss(torch.autograd.Function):
     """Loss and gradient from one pass; the backward pass multiplies the gradient where the loss's own is not 1."""
 
     @staticmethod
-    def forward(ctx, logits, targets, vocab, ignore_index, temperature, args, constants, want_grad):
-        from ..ops import _objectives as O
-        with torch.cuda.device(logits.device):
-            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
-            grad = O.empty_grad(logits) if want_grad else None
-            out = O.policy_loss(rows, args, logits.device, grad)
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature, args):
+        (loss, logp, kl, entropy), grad = _policy_forward(logits, targets, vocab, ignore_index, temperature, args, True)
         ctx.save_for_backward(grad)
-        loss, logp, kl, entropy = (t.view(targets.shape) if i else t for i, t in enumerate(out))
         ctx.mark_non_differentiable(logp, kl, entropy)
+        ctx.set_materialize_grads(False)
         return loss, logp, kl, entropy
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, *_):
-        from ..ops import _objectives as O
+        if dloss is None:
+            return (None,) * 6
         (grad,) = ctx.saved_tensors
         # a graph that is kept may be walked again, and then needs the gradient as it was
         if torch._C._autograd._get_current_graph_task_keep_graph():
-            return ((grad.float() * dloss.float()).to(grad.dtype), *(None,) * 7)
-        with torch.cuda.device(grad.device):
-            O.scale_unless_one_(_memory_of(grad), dloss.float())
-        return (grad, *(None,) * 7)
-
-
-def _memory_of(t: torch.Tensor) -> torch.Tensor:
-    """The elements between the first and the last of a tensor as a vector."""
-    if t.is_contiguous():
-        return t.view(-1)
-    return t.as_strided((1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())),), (1,))
+            return ((grad.float() * dloss.float()).to(grad.dtype), *(None,) * 5)
+        with _on(grad):
+            O.scale_unless_one_(grad, dloss.float())
+        return (grad, *(None,) * 5)
 
 
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
@@ -255,14 +281,11 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     adv = _check_values(name, "advantages", advantages, [(B, T), (B,)], logits.device)
     ref = None if ref_logp is None else _check_values(name, "ref_logp", ref_logp, [(B, T)], logits.device)
     if targets.numel() and _kernels(logits):
-        from ..ops import _objectives as O
-        a = O.PolicyArgs()
-        a.old_logp, a.advantages, a.ref_logp = old.data_ptr(), adv.data_ptr(), None if ref is None else ref.data_ptr()
-        a.adv_per, a.seq_len = (T if adv.dim() == 1 else 1), T
-        a.clip_low, a.clip_high, a.kl_coef, a.entropy_coef, a.scale = clip_low, clip_high, kl_coef, entropy_coef, scale
-        a.kl, a.mean = O.KL[kl], O.MEAN[reduction]
-        want = torch.is_grad_enabled() and logits.requires_grad
-        return PolicyLoss(*_PolicyLoss.apply(logits, targets, V, ignore_index, float(temperature), a, (old, adv, ref), want))
+        a = O.PolicyArgs(old.data_ptr(), None if ref is None else ref.data_ptr(), adv.data_ptr(), T if adv.dim() == 1 else 1, T, clip_low, clip_high,
+                         kl_coef, entropy_coef, scale, O.KL[kl], O.MEAN[reduction], 0)
+        if _wants(logits):
+            return PolicyLoss(*_PolicyLoss.apply(logits, targets, V, ignore_index, float(temperature), a))
+        return PolicyLoss(*_policy_forward(logits, targets, V, ignore_index, temperature, a, False)[0])
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     zero = torch.zeros((), dtype=lp.dtype, device=lp.device)
     p = lp.exp()
@@ -285,34 +308,37 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
 
 
 # ------------------------------------------------------------------------------------------------------ preference loss
+def _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options):
+    with _on(logits):
+        logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+        logp, stats = O.token_logprobs(rows, targets)
+        return (logits, targets, stats, *O.preference_loss(logp, targets, ref, targets.shape[0] // 2, ignore_index, **options))
+
+
 class _PreferenceLoss(torch.autograd.Function):
     """Forward: one read of the logits, then the pairs' losses and slopes; backward: one read and one write."""
 
     @staticmethod
-    def forward(ctx, logits, targets, vocab, ignore_index, temperature, ref, kind, average, beta, smoothing, target_margin):
-        from ..ops import _objectives as O
-        pairs = targets.shape[0] // 2
-        with torch.cuda.device(logits.device):
-            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
-            logp, stats = O.token_logprobs(rows, logits.device)
-            loss, seq, margin, coef = O.preference_loss(logp, targets, ref, pairs, ignore_index, kind=kind, average=average, beta=beta,
-                                                        smoothing=smoothing, target_margin=target_margin)
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature, ref, options):
+        logits, targets, stats, loss, seq, margin, coef = _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options)
         ctx.save_for_backward(logits, targets, stats, coef)
         ctx.cfg = (vocab, ignore_index, temperature)
         ctx.mark_non_differentiable(seq, margin)
+        ctx.set_materialize_grads(False)
         return loss, seq, margin
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, *_):
-        from ..ops import _objectives as O
+        if dloss is None:
+            return (None,) * 7
         logits, targets, stats, coef = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
-        with torch.cuda.device(logits.device):
+        with _on(logits):
             logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
             grad = O.empty_grad(logits)
             O.token_logprobs_grad(rows, stats, coef, targets.shape[1], dloss.float(), grad)
-        return (grad, *(None,) * 10)
+        return (grad, *(None,) * 6)
 
 
 def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, beta: float = 0.1,
@@ -340,8 +366,10 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optio
     pairs = targets.shape[0] // 2
     ref = None if ref_logp is None else _check_values(name, "ref_logp", ref_logp, [(2 * pairs,)], logits.device)
     if targets.numel() and _kernels(logits):
-        return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, V, ignore_index, float(temperature), ref, kind, bool(average),
-                                                     float(beta), float(label_smoothing), float(target_margin)))
+        options = dict(kind=kind, average=bool(average), beta=beta, smoothing=label_smoothing, target_margin=target_margin)
+        if _wants(logits):
+            return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, V, ignore_index, float(temperature), ref, options))
+        return PreferenceLoss(*_preference_forward(logits, targets, V, ignore_index, temperature, ref, options)[3:6])
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     seq = logp.double().view(targets.shape).sum(-1)
     if average:
@@ -377,9 +405,7 @@ def _spans(ts) -> List[tuple]:
 
 def _grad_list(name: str, grads, out):
     """The tensors that count, without None, empty ones and repetitions; with `out`, the tensors their clipped values go to."""
-    grads = list(grads) if not torch.is_tensor(grads) else [grads]
     if out is not None:
-        out = list(out) if not torch.is_tensor(out) else [out]
         if len(out) != len(grads):
             raise ValueError(f"{name}: {len(grads)} gradients and {len(out)} outputs")
         pairs = [(g, o) for g, o in zip(grads, out) if g is not None]
@@ -425,6 +451,26 @@ def _separate(name: str, grads, out):
     return grads
 
 
+def _plain_list(grads, out) -> Optional[List[int]]:
+    """Numbers of elements of a list that needs no second look: contiguous, non-empty tensors of one GPU that the kernels take, each with memory of
+    its own.  None for every other list, wrong ones among them."""
+    every = grads if out is None else grads + out
+    if not every or not all([isinstance(t, torch.Tensor) for t in every]) or not every[0].is_cuda:
+        return None
+    if len({t.device for t in every}) != 1 or not {t.dtype for t in every} <= _KERNEL_SET or {t.layout for t in every} != {torch.strided}:
+        return None
+    if not all([t.is_contiguous() for t in every]) or (out is not None and [t.shape for t in grads] != [t.shape for t in out]):
+        return None
+    counts = [t.numel() for t in grads]
+    at = sorted([(t.data_ptr(), t.nbytes) for t in every])
+    end = 0
+    for start, size in at:
+        if start < end or size == 0:
+            return None
+        end = start + size
+    return counts if _kernels(grads[0]) else None
+
+
 def _square_sum_plain(grads) -> float:
     sq = 0.0
     for g in grads:
@@ -442,19 +488,26 @@ def _packed(t: torch.Tensor) -> torch.Tensor:
 
 def grad_square_sum(grads: Sequence[Optional[torch.Tensor]]) -> float:
     """Sum of squares of all elements in FP64, on the host (one synchronisation): the square of the global gradient norm."""
-    grads, _ = _grad_list("grad_square_sum", grads, None)
+    grads, _ = _grad_list("grad_square_sum", list(grads), None)
     if not _kernel_list(grads):
         return _square_sum_plain(grads)
-    from ..ops import _objectives as O
-    with torch.cuda.device(grads[0].device):
+    with _on(grads[0]):
         ts = [_packed(g) for g in grads if g.numel()]
-        return float(O.grad_clip(ts, None)[0]) if ts else 0.0
+        return float(O.grad_clip(ts, [t.numel() for t in ts], None)[0]) if ts else 0.0
 
 
 def clip_grads(name: str, grads, max_norm: float, out=None):
     """`clip_grad_norm_` with the FP64 sum of squares beside the FP32 norm."""
     if not max_norm >= 0.0:
         raise ValueError(f"{name}: max_norm must not be negative, got {max_norm}")
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    out = out if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    counts = _plain_list(grads, out)
+    if counts is not None:
+        with _on(grads[0]):
+            norms = O.grad_clip(grads, counts, max_norm, out)
+        torch.autograd.graph.increment_version(grads if out is None else out)
+        return norms
     grads, out = _grad_list(name, grads, out)
     if not grads:
         return torch.zeros((), dtype=torch.float64), torch.zeros((), dtype=torch.float32)
@@ -472,11 +525,10 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
             return tuple(torch.zeros((), dtype=dt, device=grads[0].device) for dt in (torch.float64, torch.float32))
         full = _separate(name, full, outs)
         if _kernel_list(full) and (outs is None or all(o.dtype in _KERNEL_TYPES for o in outs)):
-            from ..ops import _objectives as O
-            with torch.cuda.device(full[0].device):
+            with _on(full[0]):
                 src = [_packed(g) for g in full]
                 if outs is None:
-                    norms = O.grad_clip(src, max_norm)
+                    norms = O.grad_clip(src, [t.numel() for t in src], max_norm)
                     torch.autograd.graph.increment_version(src)
                     for g, s in zip(full, src):
                         if s is not g:
@@ -484,7 +536,7 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
                     return norms
                 # element order of the memory: an output of another order than its gradient is written through a copy of that order
                 dst = [o if o.stride() == s.stride() else torch.empty_like(s, dtype=o.dtype) for o, s in zip(outs, src)]
-                norms = O.grad_clip(src, max_norm, dst)
+                norms = O.grad_clip(src, [t.numel() for t in src], max_norm, dst)
                 torch.autograd.graph.increment_version(dst)
                 for o, d in zip(outs, dst):
                     if d is not o:

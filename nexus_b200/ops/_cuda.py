@@ -104,8 +104,6 @@ def lib():
         if hasattr(_lib, "nx_grad_norm_partials"):
             _lib.nx_grad_norm_partials.restype = C.c_int64
             _lib.nx_grad_norm_partials.argtypes = [C.c_int64]
-        if hasattr(_lib, "nx_grad_clip_partials"):
-            _lib.nx_grad_clip_partials.restype = C.c_int64
         if hasattr(_lib, "nx_head_parts"):
             _lib.nx_head_parts.restype = C.c_int64
     return _lib

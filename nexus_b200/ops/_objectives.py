@@ -11,6 +11,31 @@ import torch
 
 from . import _cuda as K
 
+_functions = {}
+_P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
+_SIGNATURES = {
+    "nx_token_logprobs": [_P, _P, _P, _P, _P],
+    "nx_token_logprobs_grad": [_P, _P, _P, _L, _P, _P, _P],
+    "nx_policy_loss": [_P] * 11 + [_P],
+    "nx_scale_unless_one": [_P, _P, _I, _L, _P],
+    "nx_preference_loss": [_P, _P, _P, _P, _P, _P],
+    "nx_head_logprobs": [_P, _P, _P, _P, _P],
+    "nx_head_logprobs_grad": [_P, _P, _P],
+    "nx_grad_clip": [_P, _D, _I, _P, _P, _P],
+}
+
+
+def _call(name: str, *args) -> None:
+    """Calls a C entry point on the current stream with plain integers, floats and structures (their types are declared once: a wrapper per
+    argument is a third of a microsecond, and these operators have small forms whose time is the host's)."""
+    f = _functions.get(name)
+    if f is None:
+        f = getattr(K.lib(), name)
+        f.argtypes, f.restype = _SIGNATURES[name], C.c_int
+        _functions[name] = f
+    K._check(f(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
 KL = {"k1": 0, "k2": 1, "k3": 2}
 MEAN = {"token": 0, "sequence": 1, "sum": 2}
 PREFERENCE = {"sigmoid": 0, "hinge": 1, "ipo": 2}
@@ -61,80 +86,76 @@ def row_layout(x: torch.Tensor) -> Optional[Tuple[int, int, int]]:
 
 
 def prepare_rows(logits: torch.Tensor, targets: torch.Tensor, vocab: int, ignore_index: int, inv_temp: float):
-    """(logits that the kernels read, their description).  The returned tensors must outlive the calls."""
-    lay = row_layout(logits)
-    if lay is None:
-        logits = logits.contiguous()
-        lay = (max(1, logits.numel() // max(1, logits.shape[-1])), 0, logits.shape[-1])
-    targets = targets.contiguous()
-    r = TokenRows()
-    r.logits, r.targets, r.rows = logits.data_ptr(), targets.data_ptr(), targets.numel()
-    r.per, r.stride_outer, r.stride_inner = lay
-    r.ignore_index, r.dtype, r.targets_wide = ignore_index, K._DT[logits.dtype], int(targets.dtype == torch.int64)
-    r.vocab, r.width, r.inv_temp = vocab, logits.shape[-1], inv_temp
-    return logits, targets, r
+    """(logits that the kernels read, targets, their description).  The returned tensors must outlive the calls."""
+    W, n = logits.shape[-1], targets.numel()
+    if logits.is_contiguous():
+        lay = n, 0, W
+    else:
+        lay = row_layout(logits)
+        if lay is None:
+            logits = logits.contiguous()
+            lay = n, 0, W
+    if not targets.is_contiguous():
+        targets = targets.contiguous()
+    return logits, targets, TokenRows(logits.data_ptr(), targets.data_ptr(), n, lay[0], lay[1], lay[2], ignore_index, K._DT[logits.dtype],
+                                      targets.dtype == torch.int64, vocab, W, inv_temp)
 
 
 def empty_grad(logits: torch.Tensor) -> torch.Tensor:
     """A tensor of the layout of `logits` (as `prepare_rows` returned it) that starts at the same place of a 16-byte line."""
     off = logits.data_ptr() % 16 // logits.element_size()
-    if logits.is_contiguous() and off == 0:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if off == 0 and logits.is_contiguous():
+        return torch.empty_like(logits, requires_grad=False)
     extent = 1 + sum((n - 1) * s for n, s in zip(logits.shape, logits.stride()))
     buf = torch.empty(extent + off, dtype=logits.dtype, device=logits.device)
     return buf.as_strided(logits.shape, logits.stride(), off)
 
 
-def token_logprobs(rows: TokenRows, device):
-    """FP32 (logp [rows], stats [rows, 2])."""
-    logp = torch.empty(rows.rows, dtype=torch.float32, device=device)
-    stats = torch.empty((rows.rows, 2), dtype=torch.float32, device=device)
-    K._check(K.lib().nx_token_logprobs(C.byref(rows), K._p(logp), K._p(stats), K._p(K.status_word(device)), K._stream()),
-             "nx_token_logprobs")
+def token_logprobs(rows: TokenRows, like: torch.Tensor):
+    """FP32 (logp of the shape of `like` (the targets), stats [rows, 2])."""
+    dev = like.device
+    logp = torch.empty(like.shape, dtype=torch.float32, device=dev)
+    stats = torch.empty((rows.rows, 2), dtype=torch.float32, device=dev)
+    _call("nx_token_logprobs", C.byref(rows), logp.data_ptr(), stats.data_ptr(), K.status_word(dev).data_ptr())
     return logp, stats
 
 
 def token_logprobs_grad(rows: TokenRows, stats, coef, coef_per: int, factor, grad) -> None:
-    K._check(K.lib().nx_token_logprobs_grad(C.byref(rows), K._p(stats), K._p(coef), C.c_int64(coef_per), K._p(factor), K._p(grad),
-                                            K._stream()), "nx_token_logprobs_grad")
+    _call("nx_token_logprobs_grad", C.byref(rows), stats.data_ptr(), coef.data_ptr(), coef_per, None if factor is None else factor.data_ptr(),
+          grad.data_ptr())
 
 
-def policy_loss(rows: TokenRows, args: PolicyArgs, device, grad):
-    """FP32 (loss, logp, kl, entropy); `grad` (or None) is written."""
-    n = rows.rows
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    per_row = torch.empty((4, n), dtype=torch.float32, device=device)
-    sequences = n // args.seq_len
-    totals = torch.empty(2 + (sequences + 1) // 2, dtype=torch.float64, device=device)
-    args.write_grad = int(grad is not None)
-    K._check(K.lib().nx_policy_loss(C.byref(rows), C.byref(args), K._p(totals), C.c_void_p(totals.data_ptr() + 16), K._p(per_row[0]),
-                                    K._p(per_row[1]), K._p(per_row[2]), K._p(per_row[3]), K._p(loss), K._p(grad),
-                                    K._p(K.status_word(device)), K._stream()),
-             "nx_policy_loss")
-    return loss, per_row[0], per_row[1], per_row[2]
+def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad):
+    """FP32 (loss, logp, kl, entropy) of the shape of `like` (the targets); `grad` (or None) is written."""
+    n, dev, shape = rows.rows, like.device, like.shape
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    logp, kl, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
+    scratch = torch.empty(16 + 4 * (n // args.seq_len) + 4 * n, dtype=torch.uint8, device=dev)   # totals, counts, the rows' losses
+    at = scratch.data_ptr()
+    args.write_grad = grad is not None
+    _call("nx_policy_loss", C.byref(rows), C.byref(args), at, at + 16, logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
+          at + 16 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(), K.status_word(dev).data_ptr())
+    return loss, logp, kl, entropy
 
 
-def scale_unless_one_(x: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
-    """x *= factor in place (x dense, factor one FP32 value on the device); where the factor is 1, nothing is read or written."""
-    K._check(K.lib().nx_scale_unless_one(K._p(x), K._p(factor), C.c_int(K._DT[x.dtype]), C.c_int64(x.numel()), K._stream()),
-             "nx_scale_unless_one")
-    return x
+def scale_unless_one_(x: torch.Tensor, factor: torch.Tensor) -> None:
+    """x *= factor in place, factor one FP32 value on the device; where it is 1, nothing is read or written.  x may have gaps, whose memory is its
+    own (`empty_grad`): they are multiplied too."""
+    n = x.numel() if x.is_contiguous() else 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    _call("nx_scale_unless_one", x.data_ptr(), factor.data_ptr(), K._DT[x.dtype], n)
 
 
 def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, kind: str, average: bool, beta: float, smoothing: float,
                     target_margin: float):
     """FP32 (loss, logp of the sequences [2 * pairs], margin [pairs], coef [2 * pairs])."""
     dev = logp.device
-    a = PreferenceArgs()
-    a.logp, a.targets, a.pairs, a.seq_len = logp.data_ptr(), targets.data_ptr(), pairs, targets.numel() // (2 * pairs)
-    a.ref_logp = None if ref_logp is None else ref_logp.data_ptr()
-    a.ignore_index, a.targets_wide, a.kind, a.average = ignore_index, int(targets.dtype == torch.int64), PREFERENCE[kind], int(average)
-    a.beta, a.smoothing, a.target_margin = beta, smoothing, target_margin
+    a = PreferenceArgs(logp.data_ptr(), targets.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(), pairs,
+                       targets.numel() // (2 * pairs), ignore_index, targets.dtype == torch.int64, PREFERENCE[kind], average, beta, smoothing,
+                       target_margin)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    out = torch.empty(5 * pairs, dtype=torch.float32, device=dev)
-    seq_logp, margin, coef = out[: 2 * pairs], out[2 * pairs: 3 * pairs], out[3 * pairs:]
-    K._check(K.lib().nx_preference_loss(C.byref(a), K._p(seq_logp), K._p(margin), K._p(coef), K._p(loss), K._stream()),
-             "nx_preference_loss")
+    seq_logp, coef = (torch.empty(2 * pairs, dtype=torch.float32, device=dev) for _ in range(2))
+    margin = torch.empty(pairs, dtype=torch.float32, device=dev)
+    _call("nx_preference_loss", C.byref(a), seq_logp.data_ptr(), margin.data_ptr(), coef.data_ptr(), loss.data_ptr())
     return loss, seq_logp, margin, coef
 
 
@@ -180,20 +201,19 @@ def _gathered(hidden) -> torch.Tensor:
 
 
 def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, want_grad: bool):
-    """FP32 logp [rows] for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient needs: (stats, index
+    """FP32 logp (of the shape of `targets`) for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient needs: (stats, index
     of the rows that count, with their number behind it, or None)."""
     rows, dev = hidden.shape[0], hidden.device
     L = K.lib()
     index = torch.empty(rows + 1, dtype=torch.int32, device=dev) if want_grad or rows > HEAD_TILE else None
-    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
     parts = int(L.nx_head_parts(C.c_int32(vocab)))
     part = torch.empty((2 * parts + 1) * rows, dtype=torch.float32, device=dev)
     a = _head_args(hidden, weight, targets, index, stats, vocab, ignore_index, inv_temp)
     moved = _gathered(hidden) if index is not None else None
     a.gathered = None if moved is None else moved.data_ptr()
-    K._check(L.nx_head_logprobs(C.byref(a), K._p(logp), K._p(part), C.c_void_p(part.data_ptr() + 8 * parts * rows), K._stream()),
-             "nx_head_logprobs")
+    _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), part.data_ptr(), part.data_ptr() + 8 * parts * rows)
     return logp, stats, index
 
 
@@ -233,7 +253,7 @@ def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, i
     weight_sums = torch.empty((vocab, width), dtype=torch.float32, device=dev) if want_weight and chunk < rows else None
     for name, t in (("d_hidden", dh), ("d_weight", dw), ("slice_sums", slice_sums), ("weight_sums", weight_sums)):
         setattr(g, name, None if t is None else t.data_ptr())
-    K._check(K.lib().nx_head_logprobs_grad(C.byref(a), C.byref(g), K._stream()), "nx_head_logprobs_grad")
+    _call("nx_head_logprobs_grad", C.byref(a), C.byref(g))
     return dh, dw
 
 
@@ -242,25 +262,23 @@ class GradTable(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("count", C.c_void_p), ("type", C.c_void_p), ("tensors", C.c_int64)]
 
 
-def grad_clip(grads, max_norm: Optional[float], out=None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(FP64 sum of squares, FP32 norm) of dense, non-empty tensors; with `max_norm` they are clipped, in place or into `out`."""
-    n = len(grads)
-    src = array("Q", map(torch.Tensor.data_ptr, grads))
-    count = array("q", map(torch.Tensor.numel, grads))
+GRAD_TABLE = 256                 # tensors of a launch, and
+GRAD_PARTS = 4 * 148             # partial sums that it leaves, at most
+
+
+def grad_clip(grads, counts, max_norm: Optional[float], out=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(FP64 sum of squares, FP32 norm) of dense, non-empty tensors of `counts` elements; with `max_norm` they are clipped, in place or into
+    `out`."""
+    n, dt = len(grads), K._DT
+    src, count = array("Q", [t.data_ptr() for t in grads]), array("q", counts)
     if out is None:
-        types = bytes([17 * K._DT[t.dtype] for t in grads])
-        dst = None
+        types, dst = bytes([17 * dt[t.dtype] for t in grads]), None
     else:
-        types = bytes([K._DT[t.dtype] | K._DT[o.dtype] << 4 for t, o in zip(grads, out)])
-        dst = array("Q", map(torch.Tensor.data_ptr, out))
-    L = K.lib()
-    parts = int(L.nx_grad_clip_partials(C.c_int64(n)))
-    buf = torch.empty(2 + parts, dtype=torch.float64, device=grads[0].device)
-    a = GradTable()
-    a.src, a.count, a.tensors = src.buffer_info()[0], count.buffer_info()[0], n
-    a.dst = None if dst is None else dst.buffer_info()[0]
-    a.type = C.cast(C.c_char_p(types), C.c_void_p).value
+        types = bytes([dt[t.dtype] | dt[o.dtype] << 4 for t, o in zip(grads, out)])
+        dst = array("Q", [t.data_ptr() for t in out])
+    buf = torch.empty(2 + -(-n // GRAD_TABLE) * GRAD_PARTS, dtype=torch.float64, device=grads[0].device)
+    a = GradTable(src.buffer_info()[0], None if dst is None else dst.buffer_info()[0], count.buffer_info()[0],
+                  C.cast(C.c_char_p(types), C.c_void_p), n)
     at = buf.data_ptr()
-    K._check(L.nx_grad_clip(C.byref(a), C.c_double(0.0 if max_norm is None else max_norm), C.c_int(int(max_norm is not None)),
-                            C.c_void_p(at + 16), C.c_void_p(at), K._stream()), "nx_grad_clip")
-    return buf[0], buf[1:2].view(torch.float32)[0]
+    _call("nx_grad_clip", C.byref(a), 0.0 if max_norm is None else max_norm, max_norm is not None, at + 16, at)
+    return buf[0], buf.view(torch.float32)[2]
