@@ -5,9 +5,10 @@
 //
 // Four products on one persistent CTA-pair kernel (tcgen05, 256 x 256 tiles over two SMs, operands by TMA, two accumulators in tensor memory):
 //   stats   h W^T, whose epilogue leaves the largest logit and the sum of exponentials of each row and 128 columns (8 bytes instead of 512)
-//           and the target's logit; a join over the vocabulary follows
-//   grad    h W^T again, whose epilogue turns the logits into G in 16 bits: the gradient costs one product more than with stored logits, and
-//           G of a bounded number of rows is all that is ever in memory
+//           and the target's logit; a join over the vocabulary follows.  Where the whole G is small enough to be held, the epilogue also
+//           writes the exponentials in 16 bits, relative to that largest logit, and the gradient is a pass over them;
+//   grad    otherwise h W^T again, whose epilogue turns the logits into G in 16 bits: one product more, and G of a bounded number of rows is
+//           all that is ever in memory
 //   dh, dW  G W and G^T h
 // Rows whose target does not count are left out before the first product: the others are brought together in order (their number stays on the
 // device and bounds every loop), so that prompts and padding cost no tensor-core time.  A tile is 256 rows: without a gradient, up to that
@@ -45,6 +46,8 @@ struct Params {
   int targets_wide;
   int vocab, width;         // columns of the logits; columns of h
   int group;                // stats, grad: row tiles that pass over the vocabulary together
+  int part_blocks;          // stats: 64-deep blocks that one accumulator sums
+  int keep;                 // stats: write the exponentials
   int slices, blocks_per_slice;  // input gradient: pieces of the vocabulary
   float inv_temp;
   float2* part;             // stats: [2 * column tiles][part_ld]
@@ -257,42 +260,47 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       bool ok = true;
       for (int u = unit_first; u < e.units && ok; u += unit_step) {
         const Unit w = unit_at<MODE>(p, e, u);
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u, abort_flag))) {
-          if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kTile);
-        for (int kb = w.kb_begin; kb < w.kb_end; ++kb) {
-          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[stage], phase, abort_flag))) {
-            ok = false;
+        int kb = w.kb_begin;
+        do {
+          const int kb_stop = MODE == kStats ? min(w.kb_end, kb + p.part_blocks) : w.kb_end;
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u, abort_flag))) {
             if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
+            ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t sa = smem_u32(smem + stage * kStageBytes), sb = sa + kOperandBytes;
-          const uint64_t da0 = make_smem_desc_sw128(sa, kAmn ? 64 * kBK * 2 : 16, 1024);
-          const uint64_t db0 = make_smem_desc_sw128(sb, kBmn ? 64 * kBK * 2 : 16, 1024);
-          if (leader) {
+          const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kTile);
+          for (const int kb_first = kb; kb < kb_stop; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[stage], phase, abort_flag))) {
+              ok = false;
+              if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t sa = smem_u32(smem + stage * kStageBytes), sb = sa + kOperandBytes;
+            const uint64_t da0 = make_smem_desc_sw128(sa, kAmn ? 64 * kBK * 2 : 16, 1024);
+            const uint64_t db0 = make_smem_desc_sw128(sb, kBmn ? 64 * kBK * 2 : 16, 1024);
+            if (leader) {
 #pragma unroll
-            for (int ks = 0; ks < kBK / 16; ++ks)
-              umma_f16_ss_pair(tmem_d, da0 + static_cast<uint64_t>(kAmn ? ks * 128 : ks * 2), db0 + static_cast<uint64_t>(kBmn ? ks * 128 : ks * 2),
-                               idesc, (kb > w.kb_begin || ks > 0) ? 1u : 0u);
-            umma_commit_pair(&empty_bar[stage], 3);
+              for (int ks = 0; ks < kBK / 16; ++ks)
+                umma_f16_ss_pair(tmem_d, da0 + static_cast<uint64_t>(kAmn ? ks * 128 : ks * 2),
+                                 db0 + static_cast<uint64_t>(kBmn ? ks * 128 : ks * 2), idesc, (kb > kb_first || ks > 0) ? 1u : 0u);
+              umma_commit_pair(&empty_bar[stage], 3);
+            }
+            __syncwarp();
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
+          if (!ok) break;
+          if (leader) umma_commit_pair(&tfull_bar[acc], 3);
           __syncwarp();
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1u;
           }
-        }
-        if (!ok) break;
-        if (leader) umma_commit_pair(&tfull_bar[acc], 3);
-        __syncwarp();
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1u;
-        }
+        } while (kb < w.kb_end);
       }
     }
   } else {
@@ -327,6 +335,100 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           }
         }
       }
+      if constexpr (MODE == kStats) {
+        // Accumulators of `part_blocks` blocks are added up here: the tensor cores' own sums truncate at every addition, which over 4096 columns
+        // put 1.5e-6 of itself into logp (2.0e-7 with four accumulators of 1024).
+        uint32_t x[4][32];
+        const int chunks = c0 >= n_end ? 0 : min(4, (n_end - c0 + 31) / 32);
+        bool ok = true;
+        for (int kb = 0; kb < e.kb; kb += p.part_blocks) {
+          const bool got = mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag);
+          if (!__all_sync(0xffffffffu, got)) {
+            if (lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kTile + half * 128);
+          if (kb == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(taddr + i * 32, x[i]);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(taddr + i * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[i][j] = __float_as_uint(__uint_as_float(x[i][j]) + __uint_as_float(r[j]));
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), 0));
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (chunks == 0) continue;
+        if (n_end - c0 < 128) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c0 + i * 32 + j >= n_end) x[i][j] = 0xff800000u;  // -inf
+        }
+        const int off = tcol - c0;
+        if (__any_sync(0xffffffffu, off >= 0 && off < 128)) {
+          float t = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (i * 32 + j == off) t = __uint_as_float(x[i][j]);
+          if (off >= 0 && off < 128) p.tlogit[row] = t;
+        }
+        float top4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top4[i] = __uint_as_float(x[i][0]);
+#pragma unroll
+        for (int j = 1; j < 32; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top4[i] = fmaxf(top4[i], __uint_as_float(x[i][j]));
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        const float base = top == -INFINITY ? 0.0f : top;
+        if (p.keep) {
+          if (lane == 0) tma_store_wait_read<0>();  // the staging tiles are free once the last group has been read
+          __syncwarp();
+        }
+        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr float kLift = BF ? 0.0f : 15.0f;  // FP16: exponentials times 2^15, so that small ones keep their digits
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float d = __uint_as_float(x[i][j]) - base;
+            v[j] = ex2(BF ? d * k2 : fmaf(d, k2, kLift));
+            s4[j & 3] += v[j];
+          }
+          if (p.keep) stage_row<BF>(st + i * 2048, lane, v);
+        }
+        const float sum = ((s4[0] + s4[1]) + (s4[2] + s4[3])) * (BF ? 1.0f : 1.0f / 32768.0f);
+        if (row < live) p.part[static_cast<int64_t>(w.n0 / 128 + half) * p.part_ld + row] = make_float2(top, sum);
+        if (p.keep) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < static_cast<int>(p.cap)) {
+            for (int i = 0; i < chunks; ++i) tma_store_3d(&map_out, st + i * 2048, c0 + 32 * i, row0, 0);
+            tma_store_commit();
+          }
+        }
+        continue;
+      }
       const bool got = mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag);
       if (!__all_sync(0xffffffffu, got)) {
         if (lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
@@ -334,7 +436,6 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kTile + half * 128);
-      float top = -INFINITY, sum = 0.0f;
       const int chunks = c0 >= n_end ? 0 : min(4, (n_end - c0 + 31) / 32);
       uint32_t r[32];
       if (chunks > 0) tmem_ld_32x32b_x32(taddr, r);
@@ -357,36 +458,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (i + 1 < chunks) tmem_ld_32x32b_x32(taddr + (i + 1) * 32, r);
         else release();
         const int valid = min(32, n_end - col0);
-        if constexpr (MODE == kStats) {
-          if (valid < 32) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j >= valid) v[j] = -INFINITY;
-          }
-          const int off = tcol - col0;
-          if (__any_sync(0xffffffffu, off >= 0 && off < 32)) {
-            if (off >= 0 && off < 32) {
-              float t = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j == off) t = v[j];
-              p.tlogit[row] = t;
-            }
-          }
-          float cm[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-          for (int j = 4; j < 32; ++j) cm[j & 3] = fmaxf(cm[j & 3], v[j]);
-          const float m = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3]));
-          if (m > top) {
-            if (top != -INFINITY) sum *= ex2((top - m) * k2);
-            top = m;
-          }
-          const float base = top == -INFINITY ? 0.0f : top;
-          float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int j = 0; j < 32; ++j) s4[j & 3] += ex2((v[j] - base) * k2);
-          sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-        } else if constexpr (MODE == kGrad) {
+        if constexpr (MODE == kGrad) {
           // rows that do not count, those behind the last one among them, are zeros whatever the product left there
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -441,9 +513,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
       }
       if (chunks == 0) release();
-      if constexpr (MODE == kStats) {
-        if (row < live && chunks > 0) p.part[static_cast<int64_t>(w.n0 / 128 + half) * p.part_ld + row] = make_float2(top, sum);
-      } else if constexpr (MODE == kGrad || MODE == kWeightGrad) {
+      if constexpr (MODE == kGrad || MODE == kWeightGrad) {
         if (chunks > 0 && (MODE == kGrad || p.partial == nullptr)) {
           fence_proxy_async_smem();
           __syncwarp();
@@ -459,7 +529,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         acc_phase ^= 1u;
       }
     }
-    if ((MODE == kGrad || MODE == kWeightGrad) && lane == 0) tma_store_wait_all();  // the staging tiles die with the CTA
+    if (MODE != kInputGrad && lane == 0) tma_store_wait_all();  // the staging tiles die with the CTA
   }
 
   tc_fence_before_sync();
@@ -590,8 +660,60 @@ __global__ void __launch_bounds__(1024) coef_scale_kernel(const float* __restric
 }
 
 template <bool BF>
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
+  if constexpr (BF) {
+    unpack_bf16x2(w, a, b);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x;
+    b = f.y;
+  }
+}
+template <bool BF>
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+}
+
+// Exponentials relative to the largest logit of their row and 128 columns -> gradient of the logits: each times the row's coefficient and the
+// 128 columns' share, the target's c more.  Rows up to the next multiple of 256 are cleared: the products read them.  from and to may be the same.
+template <bool BF>
+__global__ void __launch_bounds__(256) weigh_kernel(const Params p, const uint4* from, uint4* to, int64_t ld) {
+  pdl_dependency();
+  pdl_trigger();
+  const int64_t live = live_rows(p), end = min((live + kTile - 1) / kTile * kTile, p.cap);
+  const float k2 = p.inv_temp * kLog2e, up = p.scale != nullptr ? p.scale[0] : 1.0f;
+  const int pieces = (p.vocab + 7) / 8;
+  for (int64_t r = blockIdx.x; r < end; r += gridDim.x) {
+    uint4* const out = to + r * ld;
+    int64_t tg = -1;
+    float c = 0.0f;
+    float2 mine = make_float2(0.0f, 0.0f);
+    if (r < live) {
+      const int64_t at = place(p, r);
+      tg = target_of(p.targets, p.targets_wide, at);
+      if (tg == p.ignore || tg < 0 || tg >= p.vocab) tg = -1;
+      c = p.coef[at] * p.inv_temp * up;
+      mine = p.stats[r];
+    }
+    if (tg < 0) {
+      for (int i = threadIdx.x; i < pieces; i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const uint4* const in = from + r * ld;
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+      const uint4 q = in[i];
+      const float share = p.part[static_cast<int64_t>(i >> 4) * p.part_ld + r].x;
+      const float f = -c * ex2(fmaf(share - mine.x, k2, -mine.y)) * (BF ? 1.0f : 1.0f / 32768.0f);
+      float v[8];
+      unpack2<BF>(q.x, v[0], v[1]);
+      unpack2<BF>(q.y, v[2], v[3]);
+      unpack2<BF>(q.z, v[4], v[5]);
+      unpack2<BF>(q.w, v[6], v[7]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * f + (i * 8 + j == tg ? c : 0.0f);
+      out[i] = pack8<BF>(v);
+    }
+  }
 }
 
 // Rows of dh = sum of the slices in order, times the inverse scale
@@ -691,7 +813,8 @@ bool args_ok(const NxHeadArgs* a) {
          a->vocab > 0 && a->vocab <= (1 << 30) && a->hidden != nullptr && a->weight != nullptr && a->targets != nullptr && !off(a->hidden) &&
          !off(a->weight) && a->ld_hidden % 8 == 0 && a->ld_weight % 8 == 0 && a->ld_hidden >= a->width && a->ld_weight >= a->width &&
          a->stats != nullptr && a->status != nullptr && (a->index == nullptr) == (a->count == nullptr) &&
-         (a->index == nullptr) == (a->gathered == nullptr) && !off(a->gathered);
+         (a->index == nullptr) == (a->gathered == nullptr) && !off(a->gathered) &&
+         (a->weights == nullptr || (!off(a->weights) && a->ld_weights >= a->vocab && a->ld_weights % 64 == 0));
 }
 
 Params base_params(const NxHeadArgs* a) {
@@ -709,6 +832,9 @@ Params base_params(const NxHeadArgs* a) {
   p.stats = reinterpret_cast<const float2*>(a->stats);
   p.status = a->status;
   p.slices = 1;
+  p.part_blocks = 1024 / kBK;
+  p.part = reinterpret_cast<float2*>(a->part);
+  p.part_ld = a->rows;
   // row tiles whose part of h is about 40 MB pass over the vocabulary together
   p.group = static_cast<int>(std::max<int64_t>(1, (40ll << 20) / (static_cast<int64_t>(kTile) * a->width * 2)));
   return p;
@@ -725,10 +851,8 @@ int gather(const NxHeadArgs* a, cudaStream_t st) {
 
 #define NX_HEAD(MODE_, ...) (a->dtype == NX_BF16 ? launch<MODE_, true>(__VA_ARGS__) : launch<MODE_, false>(__VA_ARGS__))
 
-extern "C" int64_t nx_head_parts(int32_t vocab) { return 2 * tiles(vocab); }
-
-extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* part, float* tlogit, nx_stream_t stream) {
-  if (!args_ok(a) || logp == nullptr || part == nullptr || tlogit == nullptr) return -1;
+extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* tlogit, nx_stream_t stream) {
+  if (!args_ok(a) || logp == nullptr || a->part == nullptr || tlogit == nullptr) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (a->index != nullptr) {
@@ -740,10 +864,12 @@ extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* part, f
   CUtensorMap ma, mb;
   if ((rc = map_k(&ma, a, h, a->width, a->rows, ldh)) != 0 || (rc = map_k(&mb, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0) return rc;
   Params p = base_params(a);
-  p.part = reinterpret_cast<float2*>(part);
-  p.part_ld = a->rows;
   p.tlogit = tlogit;
-  if ((rc = NX_HEAD(kStats, ma, mb, ma, p, tiles(a->rows) * tiles(a->vocab), st)) != 0) return rc;
+  p.keep = a->weights != nullptr;
+  CUtensorMap mo = ma;
+  if (p.keep && (rc = map_store(&mo, a, a->weights, a->vocab, (a->rows + kTile - 1) / kTile * kTile, a->ld_weights)) != 0) return rc;
+  p.cap = (a->rows + kTile - 1) / kTile * kTile;
+  if ((rc = NX_HEAD(kStats, ma, mb, mo, p, tiles(a->rows) * tiles(a->vocab), st)) != 0) return rc;
   // the last column tile may have no second half
   const int parts = static_cast<int>((a->vocab + 127) / 128);
   NX_PDL(join_kernel, static_cast<unsigned>((a->rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
@@ -755,7 +881,8 @@ extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, n
       g->ld_logit_grad < a->vocab || g->ld_logit_grad % 64 != 0 || (reinterpret_cast<uintptr_t>(g->logit_grad) & 15) != 0 ||
       (a->dtype == NX_F16 && g->scale == nullptr) || g->slices < 1 || (g->slices > 1 && g->slice_sums == nullptr) ||
       (reinterpret_cast<uintptr_t>(g->d_hidden) & 15) != 0 || (reinterpret_cast<uintptr_t>(g->d_weight) & 15) != 0 ||
-      (g->d_weight != nullptr && g->chunk < a->rows && g->weight_sums == nullptr))
+      (g->d_weight != nullptr && g->chunk < a->rows && g->weight_sums == nullptr) ||
+      (a->weights != nullptr && (a->part == nullptr || g->chunk < a->rows || g->ld_logit_grad != a->ld_weights)))
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
@@ -786,7 +913,15 @@ extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, n
     CUtensorMap h_k, h_mn;
     const uint16_t* hp = static_cast<const uint16_t*>(h) + row0 * ldh;
     if ((rc = map_k(&h_k, a, hp, a->width, here, ldh)) != 0 || (rc = map_mn(&h_mn, a, hp, a->width, here, ldh)) != 0) return rc;
-    if ((rc = NX_HEAD(kGrad, h_k, w_k, g_out, p, tiles(here) * tiles(a->vocab), st)) != 0) return rc;
+    if (a->weights != nullptr) {
+      const unsigned blocks_in = static_cast<unsigned>(std::min<int64_t>(p.cap, kNumSmsB200 * 16));
+      const auto from = static_cast<const uint4*>(a->weights);
+      const auto to = static_cast<uint4*>(g->logit_grad);
+      if (half) NX_PDL((weigh_kernel<false>), blocks_in, 256, 0, st, p, from, to, ldg / 8);
+      else NX_PDL((weigh_kernel<true>), blocks_in, 256, 0, st, p, from, to, ldg / 8);
+    } else if ((rc = NX_HEAD(kGrad, h_k, w_k, g_out, p, tiles(here) * tiles(a->vocab), st)) != 0) {
+      return rc;
+    }
     if (g->d_hidden != nullptr) {
       p.out = g->d_hidden;
       p.out_ld = a->width;

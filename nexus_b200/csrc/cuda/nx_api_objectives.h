@@ -43,8 +43,8 @@ typedef struct NxPolicyArgs {
   int32_t kl, mean;
   int32_t write_grad;
 } NxPolicyArgs;
-// Clipped policy loss with KL and entropy terms.  logp, kl, entropy, row_loss: [rows]; totals: two doubles, counts: [rows / seq_len],
-// both scratch; loss: one float;
+// Clipped policy loss with KL and entropy terms.  logp, kl, entropy, row_loss: [rows]; totals: three doubles, counts: [rows / seq_len],
+// both scratch; loss: one float; at least one row;
 // grad (write_grad): d loss / d logits in the layout and type of the logits.
 int nx_policy_loss(const NxTokenRows* rows, const NxPolicyArgs* args, double* totals, int32_t* counts, float* logp, float* kl, float* entropy,
                    float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream);
@@ -75,18 +75,20 @@ typedef struct NxHeadArgs {
   int32_t* count;
   void* gathered;
   float* stats;
-  int* status;  // receives a non-zero nx::StatusCode when a wait timed out
-  int64_t rows, ld_hidden, ld_weight, ignore_index;
+  float* part;     // [2 * (vocab / 256 rounded up), rows] pairs: scratch of the forward call; with `weights` read by the gradient too
+  void* weights;   // may be null: [rows rounded up to 256, ld_weights] of the operands' type, the logits' exponentials for the gradient
+  int* status;     // receives a non-zero nx::StatusCode when a wait timed out
+  int64_t ld_weights, rows, ld_hidden, ld_weight, ignore_index;
   int32_t vocab, width, dtype, targets_wide;
   float inv_temp;
   int32_t pad_;
 } NxHeadArgs;
-int64_t nx_head_parts(int32_t vocab);  // `part` holds this many pairs of floats per row
-// logp [rows] (0 where ignored, NaN where the target lies outside the vocabulary); part, tlogit [rows]: scratch
-int nx_head_logprobs(const NxHeadArgs* args, float* logp, float* part, float* tlogit, nx_stream_t stream);
+// logp [rows] (0 where ignored, NaN where the target lies outside the vocabulary); tlogit [rows]: scratch
+int nx_head_logprobs(const NxHeadArgs* args, float* logp, float* tlogit, nx_stream_t stream);
 typedef struct NxHeadGrad {
   const float* coef;       // [rows] gradient of logp
-  void* logit_grad;        // scratch [chunk, ld_logit_grad] of the operands' type: rows are taken `chunk` (a multiple of 256) at a time
+  void* logit_grad;        // scratch [chunk, ld_logit_grad] of the operands' type: rows are taken `chunk` (a multiple of 256) at a time; with
+                           // `weights` all at once, ld_weights apart, and it may be the same memory
   int64_t chunk, ld_logit_grad;  // ld a multiple of 64
   float* scale;            // two floats of scratch (FP16)
   void* d_hidden;          // [rows, width], may be null

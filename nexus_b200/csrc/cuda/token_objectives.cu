@@ -160,7 +160,8 @@ __device__ __forceinline__ void put_in_first(double* slot, uint32_t rank, double
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(v) : "memory");
 }
 
-// totals[0] = rows that count, totals[1] = sequences with such rows; counts[q] = rows of sequence q that count
+// totals[0] = rows that count, totals[1] = sequences with such rows, totals[2] = no block has ended (the policy kernel counts them there);
+// counts[q] = rows of sequence q that count
 __global__ void __cluster_dims__(kJoinBlocks, 1, 1) __launch_bounds__(kJoinThreads)
 token_count_kernel(const void* __restrict__ targets, int wide, int64_t sequences, int64_t len, int64_t ignore, double* __restrict__ totals,
                    int32_t* __restrict__ counts) {
@@ -211,29 +212,7 @@ token_count_kernel(const void* __restrict__ targets, int wide, int64_t sequences
     }
     totals[0] = a;
     totals[1] = b;
-  }
-}
-
-// out = sum of x in a fixed order
-__global__ void __cluster_dims__(kJoinBlocks, 1, 1) __launch_bounds__(kJoinThreads)
-sum_kernel(const float* __restrict__ x, int64_t n, float* __restrict__ out) {
-  __shared__ double part[kJoinBlocks], scratch[32];
-  cluster_arrive();
-  pdl_dependency();
-  pdl_trigger();
-  const uint32_t rank = cluster_ctarank();
-  double acc = 0.0;
-  for (int64_t i = rank * kJoinThreads + threadIdx.x; i < n; i += kJoinBlocks * kJoinThreads) acc += x[i];
-  acc = block_sum<double>(acc, scratch);
-  cluster_wait();
-  if (threadIdx.x == 0) put_in_first(part, rank, acc);
-  __syncthreads();
-  cluster_arrive();
-  cluster_wait();
-  if (rank == 0 && threadIdx.x == 0) {
-    double a = 0.0;
-    for (int i = 0; i < kJoinBlocks; ++i) a += part[i];
-    *out = static_cast<float>(a);
+    totals[2] = 0.0;
   }
 }
 
@@ -521,6 +500,8 @@ struct RingOut {
   float* row_loss;
   const double* totals;
   const int32_t* counts;
+  int* ended;        // policy: blocks that have ended, zero before; the last one adds up the rows' losses
+  float* loss;
   int* status;
   int cuts;
 };
@@ -868,6 +849,22 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(2000);
   }
+  if constexpr (kPolicy) {
+    __shared__ int last;
+    __shared__ double scratch[32];
+    if (threadIdx.x == 0) {  // the thread that wrote this block's losses
+      __threadfence();
+      last = atomicAdd(o.ended, 1) == static_cast<int>(gridDim.x) - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (last) {
+      double acc = 0.0;
+      for (uint32_t i = threadIdx.x; i < rows; i += S::kThreads) acc += __ldcg(o.row_loss + i);
+      acc = block_sum<double>(acc, scratch);
+      if (threadIdx.x == 0) *o.loss = static_cast<float>(acc);
+    }
+  }
   if (cuts > 1) cluster_sync_all();  // no block leaves while another may still write to it
 }
 
@@ -1070,28 +1067,24 @@ extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, 
 
 extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, double* totals, int32_t* counts, float* logp, float* kl,
                               float* entropy, float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream) {
-  if (!rows_ok(a) || g == nullptr || totals == nullptr || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
+  if (!rows_ok(a) || a->rows == 0 || g == nullptr || totals == nullptr || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
       g->seq_len < 1 || g->seq_len > 0x7fffffff ||
-      a->rows % g->seq_len != 0 || (g->write_grad && a->rows > 0 && (grad == nullptr || !same_lines(a->logits, grad))))
+      a->rows % g->seq_len != 0 || (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (g->mean != NX_MEAN_NONE)
-    NX_PDL(token_count_kernel, kJoinBlocks, kJoinThreads, 0, st, a->targets, a->targets_wide, a->rows / g->seq_len, g->seq_len, a->ignore_index, totals, counts);
-  if (a->rows > 0) {
-    RingOut o{};
-    o.logp = logp;
-    o.kl = kl;
-    o.entropy = entropy;
-    o.row_loss = row_loss;
-    o.totals = totals;
-    o.counts = counts;
-    o.status = status;
-    int rc = 0;
-    NX_BY_TYPE(a->dtype, rc = (launch_ring<T, true>(*a, *g, o, static_cast<T*>(grad), st)))
-    if (rc != 0) return rc;
-  }
-  NX_PDL(sum_kernel, kJoinBlocks, kJoinThreads, 0, st, row_loss, a->rows, loss);
-  return 0;
+  NX_PDL(token_count_kernel, kJoinBlocks, kJoinThreads, 0, st, a->targets, a->targets_wide, g->mean != NX_MEAN_NONE ? a->rows / g->seq_len : 0,
+         g->seq_len, a->ignore_index, totals, counts);
+  RingOut o{};
+  o.logp = logp;
+  o.kl = kl;
+  o.entropy = entropy;
+  o.row_loss = row_loss;
+  o.totals = totals;
+  o.counts = counts;
+  o.ended = reinterpret_cast<int*>(totals + 2);
+  o.loss = loss;
+  o.status = status;
+  NX_BY_TYPE(a->dtype, return (launch_ring<T, true>(*a, *g, o, static_cast<T*>(grad), st)))
 }
 
 extern "C" int nx_scale_unless_one(void* x, const float* factor, int dtype, int64_t n, nx_stream_t stream) {

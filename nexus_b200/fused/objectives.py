@@ -156,40 +156,43 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: in
     return _token_parts(logits, targets, ignore_index, temperature, V)[2].view(targets.shape)
 
 
-def _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, want_grad):
+def _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, want_grad, recompute):
     with _on(hidden):
         h, w, t = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight), targets.contiguous()
-        logp, stats, index = O.head_logprobs(h, w, t, vocab, ignore_index, 1.0 / temperature, want_grad)
-    return logp, t, stats, index
+        return t, *O.head_logprobs(h, w, t, vocab, ignore_index, 1.0 / temperature, want_grad, recompute)
 
 
 class _LinearLogprobs(torch.autograd.Function):
-    """The logits exist a tile at a time, in tensor memory; the backward pass makes them again."""
+    """The logits exist a tile at a time, in tensor memory; what the backward pass needs of them are their exponentials in 16 bits, or it makes
+    them again."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, vocab, ignore_index, temperature):
-        logp, t, stats, index = _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, True)
-        ctx.save_for_backward(hidden, weight, t, stats, index)
+    def forward(ctx, hidden, weight, targets, vocab, ignore_index, temperature, recompute):
+        t, logp, stats, index, part, weights = _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, True, recompute)
+        ctx.save_for_backward(hidden, weight, t, stats, index, part, weights)
         ctx.cfg = (vocab, ignore_index, temperature)
         return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
-        hidden, weight, t, stats, index = ctx.saved_tensors
+        hidden, weight, t, stats, index, part, weights = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
+        again = torch._C._autograd._get_current_graph_task_keep_graph()
         with _on(hidden):
             h, w = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight)
-            dh, dw = O.head_logprobs_grad(h, w, t, vocab, ignore_index, 1.0 / temperature, stats, index, dlogp.float().contiguous(),
-                                          ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None
+            dh, dw = O.head_logprobs_grad(h, w, t, vocab, ignore_index, 1.0 / temperature, stats, index, part, weights,
+                                          dlogp.float().contiguous(), ctx.needs_input_grad[0], ctx.needs_input_grad[1], again)
+        return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None, None
 
 
 def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
-                    vocab: Optional[int] = None) -> torch.Tensor:
+                    vocab: Optional[int] = None, recompute: bool = False) -> torch.Tensor:
     """`token_logprobs` of the logits ``hidden @ weight.T`` without the logits in memory: hidden [..., d], weight [V(+pad), d] of one type,
-    targets [...].  Differentiable (once) with respect to both; the backward pass holds the gradient of at most 2^29 logits (or of 256 rows) at
-    a time.  The kernels take BF16 and FP16 with d a multiple of 8 (logits in FP32, rounded nowhere; their gradient rounded to the type for
+    targets [...].  Differentiable (once) with respect to both.  Where a gradient is wanted and there are at most 2^29 logits, their exponentials
+    are held in 16 bits (1 GiB at most) until the backward pass turns them into the logits' gradient in place; with more of them, or with
+    ``recompute``, nothing is held and the backward pass makes the logits again (a third more products), their gradient of at most 2^29 logits
+    (or of 256 rows) at a time.  The kernels take BF16 and FP16 with d a multiple of 8 (logits in FP32, rounded nowhere; their gradient rounded to the type for
     its products); other types and sizes go through the logits."""
     name = "linear_logprobs"
     if not torch.is_floating_point(hidden) or hidden.dim() < 1 or weight.dim() != 2 or weight.dtype != hidden.dtype:
@@ -209,8 +212,8 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
     d, n = hidden.shape[-1], targets.numel()
     if n and d and d % 8 == 0 and hidden.dtype != torch.float32 and max(n, V) <= 1 << 30 and _kernels(hidden):
         if _wants(hidden, weight):
-            return _LinearLogprobs.apply(hidden, weight, targets, V, ignore_index, float(temperature))
-        return _linear_forward(hidden, weight, targets, V, ignore_index, temperature, False)[0]
+            return _LinearLogprobs.apply(hidden, weight, targets, V, ignore_index, float(temperature), bool(recompute))
+        return _linear_forward(hidden, weight, targets, V, ignore_index, temperature, False, False)[1]
     return token_logprobs(torch.nn.functional.linear(hidden, weight), targets, ignore_index, temperature, V)
 
 

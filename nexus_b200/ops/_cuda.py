@@ -104,8 +104,6 @@ def lib():
         if hasattr(_lib, "nx_grad_norm_partials"):
             _lib.nx_grad_norm_partials.restype = C.c_int64
             _lib.nx_grad_norm_partials.argtypes = [C.c_int64]
-        if hasattr(_lib, "nx_head_parts"):
-            _lib.nx_head_parts.restype = C.c_int64
     return _lib
 
 
@@ -118,7 +116,7 @@ def _p(t: Optional[torch.Tensor]) -> C.c_void_p:
 
 
 _KERNELS_PER_CALL = {"nx_norm_bwd": 2, "nx_embedding_bwd": 2, "nx_cross_entropy_shifted": 3, "nx_grad_norm": 2,
-                     "nx_colsum": 2, "nx_attention_bwd": 2, "nx_talk_paged": 3, "nx_policy_loss": 3,
+                     "nx_colsum": 2, "nx_attention_bwd": 2, "nx_talk_paged": 3, "nx_policy_loss": 2,
                      "nx_grad_clip": 2, "nx_head_logprobs": 4, "nx_head_logprobs_grad": 5}
 
 

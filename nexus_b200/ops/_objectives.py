@@ -12,6 +12,7 @@ import torch
 from . import _cuda as K
 
 _functions = {}
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the current stream's handle, without an object around it
 _P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 _SIGNATURES = {
     "nx_token_logprobs": [_P, _P, _P, _P, _P],
@@ -19,7 +20,7 @@ _SIGNATURES = {
     "nx_policy_loss": [_P] * 11 + [_P],
     "nx_scale_unless_one": [_P, _P, _I, _L, _P],
     "nx_preference_loss": [_P, _P, _P, _P, _P, _P],
-    "nx_head_logprobs": [_P, _P, _P, _P, _P],
+    "nx_head_logprobs": [_P, _P, _P, _P],
     "nx_head_logprobs_grad": [_P, _P, _P],
     "nx_grad_clip": [_P, _D, _I, _P, _P, _P],
 }
@@ -33,7 +34,7 @@ def _call(name: str, *args) -> None:
         f = getattr(K.lib(), name)
         f.argtypes, f.restype = _SIGNATURES[name], C.c_int
         _functions[name] = f
-    K._check(f(*args, torch.cuda.current_stream().cuda_stream), name)
+    K._check(f(*args, _stream(torch.cuda.current_device())), name)
 
 
 KL = {"k1": 0, "k2": 1, "k3": 2}
@@ -130,11 +131,11 @@ def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad):
     n, dev, shape = rows.rows, like.device, like.shape
     loss = torch.empty((), dtype=torch.float32, device=dev)
     logp, kl, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
-    scratch = torch.empty(16 + 4 * (n // args.seq_len) + 4 * n, dtype=torch.uint8, device=dev)   # totals, counts, the rows' losses
+    scratch = torch.empty(24 + 4 * (n // args.seq_len) + 4 * n, dtype=torch.uint8, device=dev)   # totals, counts, the rows' losses
     at = scratch.data_ptr()
     args.write_grad = grad is not None
-    _call("nx_policy_loss", C.byref(rows), C.byref(args), at, at + 16, logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
-          at + 16 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(), K.status_word(dev).data_ptr())
+    _call("nx_policy_loss", C.byref(rows), C.byref(args), at, at + 24, logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
+          at + 24 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(), K.status_word(dev).data_ptr())
     return loss, logp, kl, entropy
 
 
@@ -162,7 +163,8 @@ def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, k
 # ------------------------------------------------------------------------------------------- log-probabilities from hidden states
 class HeadArgs(C.Structure):
     _fields_ = [("hidden", C.c_void_p), ("weight", C.c_void_p), ("targets", C.c_void_p), ("index", C.c_void_p), ("count", C.c_void_p),
-                ("gathered", C.c_void_p), ("stats", C.c_void_p), ("status", C.c_void_p), ("rows", C.c_int64), ("ld_hidden", C.c_int64),
+                ("gathered", C.c_void_p), ("stats", C.c_void_p), ("part", C.c_void_p), ("weights", C.c_void_p), ("status", C.c_void_p),
+                ("ld_weights", C.c_int64), ("rows", C.c_int64), ("ld_hidden", C.c_int64),
                 ("ld_weight", C.c_int64), ("ignore_index", C.c_int64), ("vocab", C.c_int32), ("width", C.c_int32), ("dtype", C.c_int32),
                 ("targets_wide", C.c_int32), ("inv_temp", C.c_float), ("pad_", C.c_int32)]
 
@@ -174,6 +176,7 @@ class HeadGrad(C.Structure):
 
 
 HEAD_TILE = 256
+HEAD_PARTS = 2                   # maxima and sums of a row that a column tile leaves
 HEAD_GRAD_ELEMENTS = 1 << 29     # of the logits' gradient at a time: 1 GiB
 
 
@@ -184,15 +187,19 @@ def head_rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _head_args(hidden, weight, targets, index, stats, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
+def _head_args(hidden, weight, targets, index, stats, part, weights, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
     a = HeadArgs()
     a.hidden, a.weight, a.targets, a.stats = hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr()
     a.status = K.status_word(hidden.device).data_ptr()
     a.rows, a.width = hidden.shape
     a.ld_hidden, a.ld_weight, a.ignore_index, a.vocab = hidden.stride(0), weight.stride(0), ignore_index, vocab
-    a.dtype, a.targets_wide, a.inv_temp = K._DT[hidden.dtype], int(targets.dtype == torch.int64), inv_temp
+    a.dtype, a.targets_wide, a.inv_temp = K._DT[hidden.dtype], targets.dtype == torch.int64, inv_temp
     if index is not None:
         a.index, a.count = index.data_ptr(), index.data_ptr() + 4 * a.rows
+    if part is not None:
+        a.part = part.data_ptr()
+    if weights is not None:
+        a.weights, a.ld_weights = weights.data_ptr(), weights.stride(0)
     return a
 
 
@@ -200,21 +207,28 @@ def _gathered(hidden) -> torch.Tensor:
     return torch.empty(((hidden.shape[0] + 63) // 64 * 64, hidden.shape[1]), dtype=hidden.dtype, device=hidden.device)
 
 
-def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, want_grad: bool):
-    """FP32 logp (of the shape of `targets`) for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient needs: (stats, index
-    of the rows that count, with their number behind it, or None)."""
+def _head_pitch(vocab: int) -> int:
+    return (vocab + 63) // 64 * 64
+
+
+def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, want_grad: bool, recompute: bool = False):
+    """FP32 logp (of the shape of `targets`) for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient
+    needs: (stats, index of the rows that count, with their number behind it, or None, the column tiles' maxima and the logits' exponentials, or
+    None twice)."""
     rows, dev = hidden.shape[0], hidden.device
-    L = K.lib()
     index = torch.empty(rows + 1, dtype=torch.int32, device=dev) if want_grad or rows > HEAD_TILE else None
     logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    parts = int(L.nx_head_parts(C.c_int32(vocab)))
-    part = torch.empty((2 * parts + 1) * rows, dtype=torch.float32, device=dev)
-    a = _head_args(hidden, weight, targets, index, stats, vocab, ignore_index, inv_temp)
+    part = torch.empty(2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * rows, dtype=torch.float32, device=dev)
+    tlogit = torch.empty(rows, dtype=torch.float32, device=dev)
+    full, ld = -(-rows // HEAD_TILE) * HEAD_TILE, _head_pitch(vocab)
+    keep = want_grad and not recompute and full * ld <= HEAD_GRAD_ELEMENTS
+    weights = torch.empty((full, ld), dtype=hidden.dtype, device=dev) if keep else None
+    a = _head_args(hidden, weight, targets, index, stats, part, weights, vocab, ignore_index, inv_temp)
     moved = _gathered(hidden) if index is not None else None
     a.gathered = None if moved is None else moved.data_ptr()
-    _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), part.data_ptr(), part.data_ptr() + 8 * parts * rows)
-    return logp, stats, index
+    _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), tlogit.data_ptr())
+    return logp, stats, index, (part if keep else None), weights
 
 
 def head_slices(rows: int, width: int, vocab: int, clusters: int = 74) -> int:
@@ -230,18 +244,23 @@ def head_slices(rows: int, width: int, vocab: int, clusters: int = 74) -> int:
     return pick
 
 
-def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, stats, index, coef, want_hidden: bool,
-                       want_weight: bool):
-    """(d_hidden [rows, width], d_weight [all rows of weight, width]), either None where not wanted."""
+def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, stats, index, part, weights, coef,
+                       want_hidden: bool, want_weight: bool, again: bool = False):
+    """(d_hidden [rows, width], d_weight [all rows of weight, width]), either None where not wanted.  The exponentials become the gradient of the
+    logits in place, unless they are needed `again`."""
     rows, width = hidden.shape
     dev, dtype = hidden.device, hidden.dtype
-    a = _head_args(hidden, weight, targets, index, stats, vocab, ignore_index, inv_temp)
+    a = _head_args(hidden, weight, targets, index, stats, part, weights, vocab, ignore_index, inv_temp)
     moved = _gathered(hidden)
     a.gathered = moved.data_ptr()
     g = HeadGrad()
-    ld = (vocab + 63) // 64 * 64
-    chunk = min((rows + 255) // 256 * 256, max(256, HEAD_GRAD_ELEMENTS // ld // 256 * 256))
-    logit_grad = torch.empty((chunk, ld), dtype=dtype, device=dev)
+    ld = _head_pitch(vocab)
+    chunk = -(-rows // HEAD_TILE) * HEAD_TILE
+    if weights is not None:
+        logit_grad = torch.empty_like(weights) if again else weights
+    else:
+        chunk = min(chunk, max(HEAD_TILE, HEAD_GRAD_ELEMENTS // ld // HEAD_TILE * HEAD_TILE))
+        logit_grad = torch.empty((chunk, ld), dtype=dtype, device=dev)
     scale = torch.empty(2, dtype=torch.float32, device=dev)
     g.coef, g.logit_grad, g.chunk, g.ld_logit_grad, g.scale = coef.data_ptr(), logit_grad.data_ptr(), chunk, ld, scale.data_ptr()
     dh = torch.empty((rows, width), dtype=dtype, device=dev) if want_hidden else None

@@ -45,7 +45,8 @@ def expect(h, w, t, vocab, dlogp, temperature=1.0, ignore=-100):
     G = c * -p
     G.scatter_add_(1, at, c)
     z = -lp.clamp(min=-110.0)
-    eg = c.abs() * p * (ex + mean_ex[:, None] + U * (4 * z + 60 + vocab / 4096)) + STEP[dtype] * G.abs() + 4 * U * c.abs() * (G.abs() > 0) * torch.minimum(G.abs() / c.abs().clamp(min=1e-300), torch.ones_like(G))
+    # the exponentials and their product with the row's share are both rounded to the type (once, where the logits are made again)
+    eg = c.abs() * p * (ex + mean_ex[:, None] + U * (4 * z + 60 + vocab / 4096) + STEP[dtype]) + STEP[dtype] * G.abs() + 4 * U * c.abs() * (G.abs() > 0) * torch.minimum(G.abs() / c.abs().clamp(min=1e-300), torch.ones_like(G))
     if dtype == F16:
         eg = eg + float(c.abs().max()) * 2.0 ** -39
     dh, dw = G @ W, G.t() @ H
@@ -95,6 +96,12 @@ def test_forward_and_gradients(dtype, shape, d, vocab):
     close(w.grad[:vocab], want[4], want[5])
     assert bool((w.grad[vocab:] == 0).all())
     assert bool((h.grad.view(-1, d)[t.view(-1) == -100] == 0).all())
+    h2, w2 = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    again = F.linear_logprobs(h2, w2, t, temperature=0.7, vocab=vocab, recompute=True)
+    assert torch.equal(again.detach(), logp.detach())
+    again.backward(dl)
+    close(h2.grad, want[2], want[3])
+    close(w2.grad[:vocab], want[4], want[5])
     # as a whole: two roundings to the type, each at most half a step of every element
     assert relative(h.grad, want[2]) <= 2 * STEP[dtype] and relative(w.grad[:vocab], want[4]) <= 2 * STEP[dtype]
 
@@ -131,6 +138,21 @@ def test_slices_of_the_vocabulary():
         w.requires_grad_(True)
         F.linear_logprobs(h2, w, t).backward(dl)       # only the weight's
         close(w.grad, want[4], want[5])
+
+
+def test_backward_twice():
+    for dtype in (BF16, F16):
+        h, w, t, g = make((290,), 64, 800, dtype, seed=6)
+        h.requires_grad_(True)
+        w.requires_grad_(True)
+        logp = F.linear_logprobs(h, w, t)
+        d1, d2 = (torch.randn(290, generator=g).cuda() for _ in range(2))
+        a = torch.autograd.grad(logp, (h, w), d1, retain_graph=True)
+        b = torch.autograd.grad(logp, (h, w), d2, retain_graph=True)
+        c = torch.autograd.grad(logp, (h, w), d1)
+        assert all(torch.equal(x, y) for x, y in zip(a, c)) and not torch.equal(a[0], b[0])
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(logp, h, d1)
 
 
 def test_small_coefficients_in_fp16():
