@@ -48,7 +48,7 @@ struct Params {
   int group;                // stats, grad: row tiles that pass over the vocabulary together
   int part_blocks;          // stats: 64-deep blocks that one accumulator sums
   int keep;                 // stats: write the exponentials
-  int slices, blocks_per_slice;  // input gradient: pieces of the vocabulary
+  int slices;               // input gradient: pieces of the vocabulary at most, whose sums have room
   float inv_temp;
   float2* part;             // stats: [2 * column tiles][part_ld]
   int64_t part_ld;
@@ -77,7 +77,24 @@ struct Unit {
 };
 struct Extent {
   int tiles_m, tiles_n, kb, units;
+  int slices, per;          // input gradient: pieces of the vocabulary, and blocks of a piece
 };
+// Pieces of `blocks` 64-deep blocks for each of `tiles` tiles, so that the CTA pairs finish together: rounds times (blocks of a piece and six for
+// handing a tile over).  Chosen here, from the number of rows that count: by all rows, 380 of 609 kept 48 of the 74 pairs busy (154 us, not 105).
+__device__ __forceinline__ void cut(Extent& e, int tiles, int blocks, int most) {
+  int best = 0x7fffffff;
+  e.slices = 1;
+  e.per = blocks;
+  for (int s = 1; s <= most; ++s) {
+    const int per = (blocks + s - 1) / s;
+    const int cost = (tiles * s + kNumSmsB200 / 2 - 1) / (kNumSmsB200 / 2) * (per + 6);
+    if (cost < best) {
+      best = cost;
+      e.per = per;
+      e.slices = (blocks + per - 1) / per;
+    }
+  }
+}
 template <int MODE>
 __device__ __forceinline__ Extent extent(const Params& p, int live) {
   Extent e;
@@ -94,7 +111,10 @@ __device__ __forceinline__ Extent extent(const Params& p, int live) {
     e.tiles_n = (p.width + kTile - 1) / kTile;
     e.kb = (live + kBK - 1) / kBK;
   }
-  e.units = e.tiles_m * e.tiles_n * (MODE == kInputGrad ? p.slices : 1);
+  e.slices = 1;
+  e.per = e.kb;
+  if (MODE == kInputGrad) cut(e, e.tiles_m * e.tiles_n, e.kb, p.slices);
+  e.units = e.tiles_m * e.tiles_n * e.slices;
   return e;
 }
 template <int MODE>
@@ -116,8 +136,8 @@ __device__ __forceinline__ Unit unit_at(const Params& p, const Extent& e, int u)
     tm = u % e.tiles_m;
     if (MODE == kInputGrad) {
       w.slice = u / e.tiles_m;
-      w.kb_begin = w.slice * p.blocks_per_slice;
-      w.kb_end = min(e.kb, w.kb_begin + p.blocks_per_slice);
+      w.kb_begin = w.slice * e.per;
+      w.kb_end = min(e.kb, w.kb_begin + e.per);
     }
   }
   w.m0 = tm * kTile;
@@ -337,7 +357,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       }
       if constexpr (MODE == kStats) {
         // Accumulators of `part_blocks` blocks are added up here: the tensor cores' own sums truncate at every addition, which over 4096 columns
-        // put 1.5e-6 of itself into logp (2.0e-7 with four accumulators of 1024).
+        // put an error of 1.45e-6 of itself into logp; with accumulators of 1024 columns 3.3e-7, at the same time.
         uint32_t x[4][32];
         const int chunks = c0 >= n_end ? 0 : min(4, (n_end - c0 + 31) / 32);
         bool ok = true;
@@ -422,7 +442,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (p.keep) {
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && row0 < static_cast<int>(p.cap)) {
+          if (lane == 0 && row0 < live) {
             for (int i = 0; i < chunks; ++i) tma_store_3d(&map_out, st + i * 2048, c0 + 32 * i, row0, 0);
             tma_store_commit();
           }
@@ -469,7 +489,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           stage_row<BF>(st + i * 2048, lane, v);
         } else if constexpr (MODE == kInputGrad) {
           if (row < live) {
-            if (p.slices > 1) {
+            if (e.slices > 1) {
               float* o = p.partial + (static_cast<int64_t>(w.slice) * p.cap + row) * p.width + col0;
 #pragma unroll
               for (int j = 0; j < 8; ++j)
@@ -700,9 +720,8 @@ __global__ void __launch_bounds__(256) weigh_kernel(const Params p, const uint4*
       continue;
     }
     const uint4* const in = from + r * ld;
-    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
-      const uint4 q = in[i];
-      const float share = p.part[static_cast<int64_t>(i >> 4) * p.part_ld + r].x;
+    const int tpiece = static_cast<int>(tg >> 3);
+    auto piece = [&](int i, const uint4& q, float share) {
       const float f = -c * ex2(fmaf(share - mine.x, k2, -mine.y)) * (BF ? 1.0f : 1.0f / 32768.0f);
       float v[8];
       unpack2<BF>(q.x, v[0], v[1]);
@@ -710,9 +729,28 @@ __global__ void __launch_bounds__(256) weigh_kernel(const Params p, const uint4*
       unpack2<BF>(q.z, v[4], v[5]);
       unpack2<BF>(q.w, v[6], v[7]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = v[j] * f + (i * 8 + j == tg ? c : 0.0f);
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * f;
+      if (i == tpiece) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i * 8 + j == tg) v[j] += c;
+      }
       out[i] = pack8<BF>(v);
+    };
+    const float2* const shares = p.part + r;
+    int i = threadIdx.x;
+    for (; i + 3 * 256 < pieces; i += 4 * 256) {
+      uint4 q[4];
+      float share[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        q[u] = in[i + u * 256];
+        share[u] = shares[static_cast<int64_t>((i + u * 256) >> 4) * p.part_ld].x;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) piece(i + u * 256, q[u], share[u]);
     }
+    for (; i < pieces; i += 256) piece(i, in[i], shares[static_cast<int64_t>(i >> 4) * p.part_ld].x);
   }
 }
 
@@ -722,12 +760,14 @@ __global__ void __launch_bounds__(128) slices_kernel(const Params p) {
   pdl_dependency();
   pdl_trigger();
   const int64_t live = live_rows(p);
+  const Extent e = extent<kInputGrad>(p, static_cast<int>(live));
+  if (e.slices == 1) return;  // the product has written the rows itself
   const float down = p.scale != nullptr ? p.scale[1] : 1.0f;
   for (int64_t r = blockIdx.x; r < live; r += gridDim.x) {
     uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + place(p, r) * p.out_ld;
     for (int i = threadIdx.x * 8; i < p.width; i += blockDim.x * 8) {
       float v[8] = {};
-      for (int s = 0; s < p.slices; ++s) {
+      for (int s = 0; s < e.slices; ++s) {
         const float4* q = reinterpret_cast<const float4*>(p.partial + (static_cast<int64_t>(s) * p.cap + r) * p.width + i);
         const float4 a = q[0], b = q[1];
         v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
@@ -925,10 +965,8 @@ extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, n
     if (g->d_hidden != nullptr) {
       p.out = g->d_hidden;
       p.out_ld = a->width;
-      const int64_t blocks = (a->vocab + kBK - 1) / kBK;
-      p.blocks_per_slice = static_cast<int>((blocks + g->slices - 1) / g->slices);
-      p.slices = static_cast<int>((blocks + p.blocks_per_slice - 1) / p.blocks_per_slice);
-      p.partial = p.slices > 1 ? g->slice_sums : nullptr;
+      p.slices = g->slices;
+      p.partial = g->slice_sums;
       if ((rc = NX_HEAD(kInputGrad, g_k, w_mn, g_out, p, tiles(here) * tiles(a->width) * p.slices, st)) != 0) return rc;
       if (p.slices > 1) {
         const unsigned blocks_out = static_cast<unsigned>(std::min<int64_t>(here, kNumSmsB200 * 16));

@@ -93,7 +93,7 @@ typedef struct NxHeadGrad {
   float* scale;            // two floats of scratch (FP16)
   void* d_hidden;          // [rows, width], may be null
   void* d_weight;          // [vocab, width], may be null
-  float* slice_sums;       // slices > 1: scratch [slices, chunk, width]: the vocabulary is cut to fill the machine
+  float* slice_sums;       // slices > 1: scratch [slices, chunk, width]: the vocabulary may be cut into so many to fill the machine
   float* weight_sums;      // chunk < rows: scratch [vocab, width]
   int32_t slices, pad_;
 } NxHeadGrad;

@@ -189,12 +189,15 @@ class _LinearLogprobs(torch.autograd.Function):
 def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
                     vocab: Optional[int] = None, recompute: bool = False) -> torch.Tensor:
     """`token_logprobs` of the logits ``hidden @ weight.T`` without the logits in memory: hidden [..., d], weight [V(+pad), d] of one type,
-    targets [...].  Differentiable (once) with respect to both.  Where a gradient is wanted and there are at most 2^29 logits, their exponentials
-    are held in 16 bits (1 GiB at most) until the backward pass turns them into the logits' gradient in place; with more of them, or with
+    targets [...].  Differentiable (once) with respect to both.  Where a gradient is wanted, d is 1024 or more and there are at most 2^29 logits, their exponentials
+    are held in 16 bits (1 GiB at most) until the backward pass turns them into the logits' gradient in place; else, or with
     ``recompute``, nothing is held and the backward pass makes the logits again (a third more products), their gradient of at most 2^29 logits
     (or of 256 rows) at a time.  The kernels take BF16 and FP16 with d a multiple of 8 (logits in FP32, rounded nowhere; their gradient rounded to the type for
-    its products); other types and sizes go through the logits."""
+    its products); other types and sizes go through the logits.  Under autocast the operands are cast as a linear layer's are."""
     name = "linear_logprobs"
+    if hidden.is_cuda and torch.is_autocast_enabled("cuda") and hidden.is_floating_point() and weight.is_floating_point():
+        dtype = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dtype), weight.to(dtype)
     if not torch.is_floating_point(hidden) or hidden.dim() < 1 or weight.dim() != 2 or weight.dtype != hidden.dtype:
         raise ValueError(f"{name}: hidden [..., d] and weight [V, d] must be floating-point tensors of one type")
     if weight.shape[1] != hidden.shape[-1]:

@@ -353,6 +353,43 @@ class LanguageModel(nn.Module):
 
     forward = loss
 
+    # ------------------------------------------------------- fine-tuning on rewards and preferences
+    def _next_targets(self, tokens: torch.Tensor, mask: Optional[torch.Tensor]) -> torch.Tensor:
+        """target[b, t] = tokens[b, t + 1]; ignored at the end of every row and, with ``mask`` [B, T], for tokens whose mask is false."""
+        tg = F_.shifted_targets(tokens)
+        if mask is not None:
+            if mask.shape != tokens.shape or mask.dtype != torch.bool:
+                raise ValueError(f"mask must be a bool tensor {tuple(tokens.shape)}")
+            tg[:, :-1].masked_fill_(~mask[:, 1:], -100)
+        return tg
+
+    def _logit_scale(self) -> float:
+        return self.config.mup_base_width / self.config.d_model if self.config.init == "mup" else 1.0
+
+    def token_logprobs(self, tokens: torch.Tensor, mask: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+        """FP32 log-probabilities [B, T] of the next tokens: entry t is that of ``tokens[:, t + 1]`` (zero at the last position and for
+        tokens whose ``mask`` is false: prompts, padding).  The logits are never in memory (`fused.ops.linear_logprobs`): what scores the
+        samples of an older policy or of a reference model, under ``torch.no_grad``, and what other objectives differentiate."""
+        h = self.hidden(tokens)
+        w = self.wte if self.lm_head is None else self.lm_head
+        return F_.linear_logprobs(h, w.to(h.dtype) if w.dtype != h.dtype else w, self._next_targets(tokens, mask),
+                                  temperature=temperature / self._logit_scale(), vocab=self.config.vocab_size)
+
+    def policy_loss(self, tokens: torch.Tensor, mask: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
+                    ref_logp: Optional[torch.Tensor] = None, **options) -> "F_.PolicyLoss":
+        """`fused.ops.policy_loss` of sampled sequences [B, T]; ``mask`` is true on the tokens that were sampled, ``old_logp`` and ``ref_logp``
+        are as `token_logprobs` returns them, advantages [B] or [B, T] (of the token that an entry predicts).  The router losses of MoE layers
+        are added to the loss."""
+        r = F_.policy_loss(self.logits(tokens), self._next_targets(tokens, mask), old_logp, advantages, ref_logp, vocab=self.config.vocab_size,
+                           **options)
+        return r._replace(loss=r.loss + self.aux_loss()) if self.config.moe_experts > 0 else r
+
+    def preference_loss(self, tokens: torch.Tensor, mask: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, **options) -> "F_.PreferenceLoss":
+        """`fused.ops.preference_loss` of pairs of sequences [2 P, T], the chosen ones first; ``mask`` is true on the answers' tokens, ``ref_logp``
+        [2 P] the sums (with ``average`` the means) of the reference model's `token_logprobs`."""
+        r = F_.preference_loss(self.logits(tokens), self._next_targets(tokens, mask), ref_logp, vocab=self.config.vocab_size, **options)
+        return r._replace(loss=r.loss + self.aux_loss()) if self.config.moe_experts > 0 else r
+
     # ------------------------------------------------------------------------------- generation
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, max_new: int, greedy: bool = True, temperature: float = 1.0,

@@ -178,6 +178,10 @@ class HeadGrad(C.Structure):
 HEAD_TILE = 256
 HEAD_PARTS = 2                   # maxima and sums of a row that a column tile leaves
 HEAD_GRAD_ELEMENTS = 1 << 29     # of the logits' gradient at a time: 1 GiB
+# From this width on the exponentials are held: writing them and turning them into the gradient is traffic per logit, making the logits again
+# work per logit and column.  Both, forward and backward together without the products with the gradient, at 896 columns (380 x 151936, FP16):
+# 228 held, 209 us again; at 4096 (5376 x 32000, BF16) 1150 and 2050 us.
+HEAD_KEEP_WIDTH = 1024
 
 
 def head_rows(t: torch.Tensor) -> torch.Tensor:
@@ -222,7 +226,7 @@ def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_te
     part = torch.empty(2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * rows, dtype=torch.float32, device=dev)
     tlogit = torch.empty(rows, dtype=torch.float32, device=dev)
     full, ld = -(-rows // HEAD_TILE) * HEAD_TILE, _head_pitch(vocab)
-    keep = want_grad and not recompute and full * ld <= HEAD_GRAD_ELEMENTS
+    keep = want_grad and not recompute and hidden.shape[1] >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
     weights = torch.empty((full, ld), dtype=hidden.dtype, device=dev) if keep else None
     a = _head_args(hidden, weight, targets, index, stats, part, weights, vocab, ignore_index, inv_temp)
     moved = _gathered(hidden) if index is not None else None
@@ -231,17 +235,13 @@ def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_te
     return logp, stats, index, (part if keep else None), weights
 
 
-def head_slices(rows: int, width: int, vocab: int, clusters: int = 74) -> int:
-    """Pieces of the vocabulary whose shares of a hidden-state gradient are summed afterwards: rounds of tiles over the CTA pairs times
-    (64-deep blocks of a piece, and about six for handing a tile over), and the sums' own traffic in the same units (0.39 us)."""
-    tiles, blocks = -(-rows // HEAD_TILE) * -(-width // HEAD_TILE), -(-vocab // 64)
-    best, pick = None, 1
-    for s in range(1, 17):
-        per = -(-blocks // s)
-        cost = -(-tiles * s // clusters) * (per + 6) + (0 if s == 1 else 8 + s * rows * width * 8 / 2.0e6)
-        if best is None or cost < best:
-            best, pick = cost, s
-    return pick
+def head_slices(rows: int, width: int) -> int:
+    """Pieces that the vocabulary may be cut into for a hidden-state gradient [rows, width] (how many it is, the kernels decide by the rows that
+    count): none where its tiles alone give every pair of SMs two, else up to 16 whose FP32 sums stay below 128 MiB."""
+    tiles = -(-rows // HEAD_TILE) * -(-width // HEAD_TILE)
+    if tiles >= 2 * 74:
+        return 1
+    return max(1, min(16, (1 << 25) // (-(-rows // HEAD_TILE) * HEAD_TILE * width)))
 
 
 def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, stats, index, part, weights, coef,
@@ -267,7 +267,7 @@ def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, i
     dw = torch.empty((weight.shape[0], width), dtype=dtype, device=dev) if want_weight else None
     if want_weight and weight.shape[0] > vocab:
         dw[vocab:].zero_()
-    g.slices = head_slices(min(rows, chunk), width, vocab) if want_hidden else 1
+    g.slices = head_slices(min(rows, chunk), width) if want_hidden else 1
     slice_sums = torch.empty((g.slices, chunk, width), dtype=torch.float32, device=dev) if g.slices > 1 else None
     weight_sums = torch.empty((vocab, width), dtype=torch.float32, device=dev) if want_weight and chunk < rows else None
     for name, t in (("d_hidden", dh), ("d_weight", dw), ("slice_sums", slice_sums), ("weight_sums", weight_sums)):

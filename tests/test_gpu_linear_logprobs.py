@@ -70,12 +70,12 @@ def relative(got, want):
 
 
 SIZES = [((1,), 8, 5), ((8,), 64, 300), ((3, 5), 72, 257), ((2, 64), 128, 1000), ((129,), 256, 513), ((2, 128), 96, 4097), ((257,), 64, 128),
-         ((3, 203), 160, 1031), ((1300,), 520, 777), ((700,), 264, 5003)]
+         ((3, 203), 160, 1031), ((1300,), 520, 777), ((700,), 264, 5003), ((300,), 2120, 1500)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("shape,d,vocab", SIZES)
-def test_forward_and_gradients(dtype, shape, d, vocab):
+def test_forward_and_gradients(dtype, shape, d, vocab, monkeypatch):
     h, w, t, g = make(shape, d, vocab, dtype, seed=d + vocab, pad=3)
     if t.numel() > 4:
         t.view(-1)[::3] = -100
@@ -96,10 +96,13 @@ def test_forward_and_gradients(dtype, shape, d, vocab):
     close(w.grad[:vocab], want[4], want[5])
     assert bool((w.grad[vocab:] == 0).all())
     assert bool((h.grad.view(-1, d)[t.view(-1) == -100] == 0).all())
+    # the other way of the backward pass, which the width alone would not take
+    from nexus_b200.ops import _objectives as O
+    monkeypatch.setattr(O, "HEAD_KEEP_WIDTH", 0 if d < O.HEAD_KEEP_WIDTH else 1 << 30)
     h2, w2 = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
-    again = F.linear_logprobs(h2, w2, t, temperature=0.7, vocab=vocab, recompute=True)
-    assert torch.equal(again.detach(), logp.detach())
-    again.backward(dl)
+    other = F.linear_logprobs(h2, w2, t, temperature=0.7, vocab=vocab)
+    assert torch.equal(other.detach(), logp.detach())
+    other.backward(dl)
     close(h2.grad, want[2], want[3])
     close(w2.grad[:vocab], want[4], want[5])
     # as a whole: two roundings to the type, each at most half a step of every element
@@ -126,7 +129,7 @@ def test_chunks_of_rows(rows, monkeypatch):
 
 def test_slices_of_the_vocabulary():
     from nexus_b200.ops import _objectives as O
-    assert O.head_slices(300, 64, 20000) > 1 and O.head_slices(8192, 4096, 32000) == 1
+    assert O.head_slices(300, 64) > 1 and O.head_slices(8192, 4096) == 1
     for dtype in (BF16, F16):
         h, w, t, g = make((300,), 64, 20000, dtype, seed=1)
         dl = torch.randn(300, generator=g).cuda()
@@ -140,7 +143,10 @@ def test_slices_of_the_vocabulary():
         close(w.grad, want[4], want[5])
 
 
-def test_backward_twice():
+@pytest.mark.parametrize("keep_width", [0, 1024])
+def test_backward_twice(keep_width, monkeypatch):
+    from nexus_b200.ops import _objectives as O
+    monkeypatch.setattr(O, "HEAD_KEEP_WIDTH", keep_width)
     for dtype in (BF16, F16):
         h, w, t, g = make((290,), 64, 800, dtype, seed=6)
         h.requires_grad_(True)
@@ -249,8 +255,9 @@ def test_agrees_with_logits_in_memory():
     assert float((a - b).abs().max()) < 260 * 4 * U * 256
 
 
-def test_streams_graphs_and_repeated_backward():
-    made = [make((3, 150), 128, 900, BF16, seed=s) for s in (1, 2)]
+@pytest.mark.parametrize("recompute", [False, True])
+def test_streams_graphs_and_repeated_backward(recompute):
+    made = [make((3, 150), 1024, 900, BF16, seed=s) for s in (1, 2)]
     for h, w, t, _ in made:
         t[:, :40] = -100
     dl = torch.randn(3, 150, device="cuda")
@@ -258,7 +265,7 @@ def test_streams_graphs_and_repeated_backward():
     def step(i):
         h, w, t, _ = made[i]
         h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
-        logp = F.linear_logprobs(h, w, t)
+        logp = F.linear_logprobs(h, w, t, recompute=recompute)
         return (logp.detach(), *torch.autograd.grad(logp, (h, w), dl))
 
     plain = [step(i) for i in (0, 1)]

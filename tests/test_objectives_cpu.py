@@ -132,9 +132,8 @@ def test_linear_logprobs_on_the_host():
             call()
 
 
-def test_slices_of_the_vocabulary_fill_the_machine():
+def test_slices_of_the_vocabulary():
     from nexus_b200.ops._objectives import head_slices
-    assert head_slices(8192, 4096, 32000) == 1
-    for rows, width, vocab in ((609, 896, 151936), (1, 64, 1000), (256, 4096, 32000)):
-        s = head_slices(rows, width, vocab)
-        assert 1 <= s <= 16
+    assert head_slices(8192, 4096) == 1 and head_slices(609, 896) == 16
+    for rows, width in ((1, 64), (256, 4096), (2048, 1024), (4096, 512), (100000, 8)):
+        assert 1 <= head_slices(rows, width) <= 16 and (head_slices(rows, width) - 1) * rows * width <= 1 << 25
