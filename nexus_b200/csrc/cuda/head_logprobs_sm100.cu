@@ -566,6 +566,227 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   }
 }
 
+// ------------------------------------------------------------------------------------------------ up to 64 rows
+// Scoring beside decoding: the time is that of reading the weight once.  The weight's rows are the tall operand here: every SM takes one run of
+// the vocabulary, in groups of 32 rows so that the runs differ by at most one group (with 256 x 256 tiles 50257 rows were 197 tiles for 74 pairs,
+// three rounds for 2.7), and a lane of the epilogue keeps maximum and sum of one row of a tile for every token, over all tiles of the run; lanes
+// meet once, at its end.  8 x 50257 x 1600 BF16: 30 us (5.3 TB/s of weights), 256 x 256 tiles 44.
+constexpr int kFewRows = 64, kFewThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2..5: a quarter of the 128 lanes each
+constexpr int kGroupBytes = 32 * kBK * 2, kFewAccumulators = 4;
+template <int NT>
+struct Few {
+  static constexpr int kStageBytes = 4 * kGroupBytes + NT * kBK * 2;
+  static constexpr int kStages = 200 * 1024 / kStageBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes;
+  static constexpr int kTmemCols = kFewAccumulators * NT;
+};
+
+template <int NT, bool BF>
+__global__ void __launch_bounds__(kFewThreads, 1)
+few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h, const Params p, const uint32_t idesc) {
+  using F = Few<NT>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t full_bar[F::kStages], empty_bar[F::kStages], tfull_bar[kFewAccumulators], tempty_bar[kFewAccumulators];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ int32_t target[NT];
+  __shared__ float2 met[4][NT];
+  volatile int* const abort_flag = &abort_word;
+  if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzle needs it
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, kStatusBadArgument);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < F::kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < kFewAccumulators; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 4);
+    }
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, F::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_h);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int rows = static_cast<int>(p.rows), kb_all = (p.width + kBK - 1) / kBK;
+  const int64_t groups = (p.vocab + 31) / 32;
+  const int g0 = static_cast<int>(groups * blockIdx.x / gridDim.x), g1 = static_cast<int>(groups * (blockIdx.x + 1) / gridDim.x);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int g = g0; g < g1 && ok; g += 4) {
+        const int here = min(4, g1 - g);
+        for (int kb = 0; kb < kb_all; ++kb) {
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            atomicCAS(p.status, 0, kStatusTimeoutProducer);
+            break;
+          }
+          uint8_t* const sa = smem + stage * F::kStageBytes;
+          mbar_arrive_expect_tx(&full_bar[stage], static_cast<uint32_t>(here * kGroupBytes + NT * kBK * 2));
+          for (int i = 0; i < here; ++i) tma_load_3d(sa + i * kGroupBytes, &map_w, &full_bar[stage], kb * kBK, (g + i) * 32, 0);
+          tma_load_3d(sa + 4 * kGroupBytes, &map_h, &full_bar[stage], kb * kBK, 0, 0);
+          if (++stage == F::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int g = g0; g < g1 && ok; g += 4) {
+      for (int kb = 0; kb < kb_all && ok;) {
+        const int stop = min(kb_all, kb + p.part_blocks);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u, abort_flag))) {
+          if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        for (const int first = kb; kb < stop; ++kb) {
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[stage], phase, abort_flag))) {
+            if (leader) atomicCAS(p.status, 0, kStatusTimeoutMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t sa = smem_u32(smem + stage * F::kStageBytes);
+          const uint64_t da = make_smem_desc_sw128(sa, 16, 1024), db = make_smem_desc_sw128(sa + 4 * kGroupBytes, 16, 1024);
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < kBK / 16; ++ks)
+              umma_f16_ss(tmem_base + static_cast<uint32_t>(acc * NT), da + static_cast<uint64_t>(ks * 2), db + static_cast<uint64_t>(ks * 2), idesc,
+                          (kb > first || ks > 0) ? 1u : 0u);
+            umma_commit(&empty_bar[stage]);
+          }
+          __syncwarp();
+          if (++stage == F::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (leader) umma_commit(&tfull_bar[acc]);
+        __syncwarp();
+        if (++acc == kFewAccumulators) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    for (int j = threadIdx.x - 64; j < NT; j += 128) {
+      int32_t t = -1;
+      if (j < rows) {
+        const int64_t tg = target_of(p.targets, p.targets_wide, j);
+        if (tg != p.ignore && tg >= 0 && tg < p.vocab) t = static_cast<int32_t>(tg);
+      }
+      target[j] = t;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const float k2 = p.inv_temp * kLog2e;
+    float top[NT], sum[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) top[j] = -INFINITY, sum[j] = 0.0f;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int g = g0; g < g1 && ok; g += 4) {
+      uint32_t x[NT];
+      for (int kb = 0; kb < kb_all; kb += p.part_blocks) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag))) {
+          if (lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t at = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * NT);
+#pragma unroll
+        for (int i = 0; i < NT / 16; ++i) {
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(at + i * 16, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            x[i * 16 + j] = kb == 0 ? r[j] : __float_as_uint(__uint_as_float(x[i * 16 + j]) + __uint_as_float(r[j]));
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty_bar[acc]);
+        if (++acc == kFewAccumulators) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      // this lane's row of the vocabulary; groups that the last tile does not have hold what an earlier one left
+      const int v = (g + quarter) * 32 + lane;
+      if (g + quarter < g1 && v < p.vocab) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float l = __uint_as_float(x[j]);
+          if (target[j] == v) p.tlogit[j] = l;
+          const float m = fmaxf(top[j], l), base = m == -INFINITY ? 0.0f : m;
+          sum[j] = sum[j] * ex2((top[j] - base) * k2) + ex2((l - base) * k2);
+          top[j] = m;
+        }
+      }
+    }
+    // the lanes of a warp, then the warps
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const float m = warp_max(top[j]);
+      const float s = warp_sum(top[j] == -INFINITY ? sum[j] : sum[j] * ex2((top[j] - m) * k2));
+      if (lane == 0) met[quarter][j] = make_float2(m, s);
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int j = threadIdx.x - 64; j < rows; j += 128) {
+      float m = met[0][j].x, s = 0.0f;
+      for (int w = 1; w < 4; ++w) m = fmaxf(m, met[w][j].x);
+      for (int w = 0; w < 4; ++w) {
+        const float2 v = met[w][j];
+        s += v.x == -INFINITY ? v.y : v.y * ex2((v.x - m) * k2);
+      }
+      p.part[static_cast<int64_t>(blockIdx.x) * p.part_ld + j] = make_float2(m, s);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0) {  // a wait ran out: copies still in flight land before the shared memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(2000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, F::kTmemCols);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ around the products
 // index[0 .. count) = the rows whose target counts, in order; the others' logp is written.  One block: a thread takes a run of rows.
 constexpr int kPickThreads = 1024;
@@ -833,6 +1054,24 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, c
 
 int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
 
+template <int NT, bool BF>
+int launch_few(const NxHeadArgs* a, const Params& p, int blocks, cudaStream_t st) {
+  const CUtensorMapDataType dt = BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap w, h;
+  int rc;
+  if ((rc = make_tensor_map_3d(&w, dt, 2, a->weight, a->width, a->vocab, 1, a->ld_weight, 0, kBK, 32)) != 0 ||
+      (rc = make_tensor_map_3d(&h, dt, 2, a->hidden, a->width, a->rows, 1, a->ld_hidden, 0, kBK, NT)) != 0)
+    return rc;
+  auto kern = few_rows_kernel<NT, BF>;
+  NX_ALLOW_SMEM(kern, Few<NT>::kSmemBytes);
+  const uint32_t fmt = BF ? kFmtBF16 : kFmtF16;
+  return launch_pdl(kern, dim3(blocks), dim3(kFewThreads), Few<NT>::kSmemBytes, st, w, h, p, make_idesc(fmt, fmt, false, false, 128, NT));
+}
+template <bool BF>
+int launch_few(const NxHeadArgs* a, const Params& p, int blocks, cudaStream_t st) {
+  return a->rows <= 16 ? launch_few<16, BF>(a, p, blocks, st) : a->rows <= 32 ? launch_few<32, BF>(a, p, blocks, st) : launch_few<64, BF>(a, p, blocks, st);
+}
+
 // K-major operand of [rows][k], or MN-major of [k][mn]; 128-byte swizzle
 int map_k(CUtensorMap* m, const NxHeadArgs* a, const void* base, int64_t k, int64_t rows, int64_t ld) {
   const CUtensorMapDataType dt = a->dtype == NX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -849,7 +1088,8 @@ int map_store(CUtensorMap* m, const NxHeadArgs* a, const void* base, int64_t col
 
 bool args_ok(const NxHeadArgs* a) {
   auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
-  return a != nullptr && (a->dtype == NX_BF16 || a->dtype == NX_F16) && a->rows > 0 && a->rows <= (1 << 30) && a->width > 0 && a->width % 8 == 0 &&
+  auto split = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) != 0; };  // pairs of floats
+  return a != nullptr && !split(a->stats) && !split(a->part) && (a->dtype == NX_BF16 || a->dtype == NX_F16) && a->rows > 0 && a->rows <= (1 << 30) && a->width > 0 && a->width % 8 == 0 &&
          a->vocab > 0 && a->vocab <= (1 << 30) && a->hidden != nullptr && a->weight != nullptr && a->targets != nullptr && !off(a->hidden) &&
          !off(a->weight) && a->ld_hidden % 8 == 0 && a->ld_weight % 8 == 0 && a->ld_hidden >= a->width && a->ld_weight >= a->width &&
          a->stats != nullptr && a->status != nullptr && (a->index == nullptr) == (a->count == nullptr) &&
@@ -899,21 +1139,28 @@ extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* tlogit,
     NX_PDL(pick_rows_kernel, 1, kPickThreads, 0, st, a->targets, a->targets_wide, a->rows, a->ignore_index, a->vocab, a->index, a->count, logp);
     if ((rc = gather(a, st)) != 0) return rc;
   }
+  Params p = base_params(a);
+  p.tlogit = tlogit;
+  auto join = [&](int parts) {
+    NX_PDL(join_kernel, static_cast<unsigned>((a->rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
+    return 0;
+  };
+  if (a->index == nullptr && a->rows <= kFewRows) {
+    // a part for every SM; `part` has room for one per 128 columns
+    const int blocks = static_cast<int>(std::min<int64_t>(kNumSmsB200, 2 * tiles(a->vocab)));
+    rc = a->dtype == NX_BF16 ? launch_few<true>(a, p, blocks, st) : launch_few<false>(a, p, blocks, st);
+    return rc != 0 ? rc : join(blocks);
+  }
   const void* h = a->index != nullptr ? a->gathered : a->hidden;
   const int64_t ldh = a->index != nullptr ? a->width : a->ld_hidden;
   CUtensorMap ma, mb;
   if ((rc = map_k(&ma, a, h, a->width, a->rows, ldh)) != 0 || (rc = map_k(&mb, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0) return rc;
-  Params p = base_params(a);
-  p.tlogit = tlogit;
   p.keep = a->weights != nullptr;
   CUtensorMap mo = ma;
   if (p.keep && (rc = map_store(&mo, a, a->weights, a->vocab, (a->rows + kTile - 1) / kTile * kTile, a->ld_weights)) != 0) return rc;
   p.cap = (a->rows + kTile - 1) / kTile * kTile;
   if ((rc = NX_HEAD(kStats, ma, mb, mo, p, tiles(a->rows) * tiles(a->vocab), st)) != 0) return rc;
-  // the last column tile may have no second half
-  const int parts = static_cast<int>((a->vocab + 127) / 128);
-  NX_PDL(join_kernel, static_cast<unsigned>((a->rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
-  return 0;
+  return join(static_cast<int>((a->vocab + 127) / 128));  // the last column tile may have no second half
 }
 
 extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, nx_stream_t stream) {

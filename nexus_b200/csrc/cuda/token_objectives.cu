@@ -1046,7 +1046,7 @@ bool same_lines(const void* a, const void* b) { return ((reinterpret_cast<uintpt
   }
 
 extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats, int* status, nx_stream_t stream) {
-  if (!rows_ok(a) || logp == nullptr || stats == nullptr || status == nullptr) return -1;
+  if (!rows_ok(a) || logp == nullptr || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 7) != 0 || status == nullptr) return -1;
   if (a->rows == 0) return 0;
   RingOut o{};
   o.logp = logp;
@@ -1057,7 +1057,7 @@ extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats
 
 extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, const float* coef, int64_t coef_per, const float* factor,
                                       void* grad, nx_stream_t stream) {
-  if (!rows_ok(a) || stats == nullptr || coef == nullptr || coef_per < 1 || coef_per > 0x7fffffff || grad == nullptr || !same_lines(a->logits, grad)) return -1;
+  if (!rows_ok(a) || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 7) != 0 || coef == nullptr || coef_per < 1 || coef_per > 0x7fffffff || grad == nullptr || !same_lines(a->logits, grad)) return -1;
   if (a->rows == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   NX_BY_TYPE(a->dtype, NX_PDL((token_grad_kernel<T>), a->rows, kThreads, 0, st, *a, reinterpret_cast<const float2*>(stats), coef, coef_per,
@@ -1067,7 +1067,7 @@ extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, 
 
 extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, double* totals, int32_t* counts, float* logp, float* kl,
                               float* entropy, float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream) {
-  if (!rows_ok(a) || a->rows == 0 || g == nullptr || totals == nullptr || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
+  if (!rows_ok(a) || a->rows == 0 || g == nullptr || totals == nullptr || (reinterpret_cast<uintptr_t>(totals) & 7) != 0 || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
       g->seq_len < 1 || g->seq_len > 0x7fffffff ||
       a->rows % g->seq_len != 0 || (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
     return -1;

@@ -158,7 +158,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: in
 
 def _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, want_grad, recompute):
     with _on(hidden):
-        h, w, t = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight), targets.contiguous()
+        h = O.head_rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1]))
+        w, t = O.head_rows(weight), targets if targets.is_contiguous() else targets.contiguous()
         return t, *O.head_logprobs(h, w, t, vocab, ignore_index, 1.0 / temperature, want_grad, recompute)
 
 

@@ -191,20 +191,13 @@ def head_rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _head_args(hidden, weight, targets, index, stats, part, weights, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
-    a = HeadArgs()
-    a.hidden, a.weight, a.targets, a.stats = hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), stats.data_ptr()
-    a.status = K.status_word(hidden.device).data_ptr()
-    a.rows, a.width = hidden.shape
-    a.ld_hidden, a.ld_weight, a.ignore_index, a.vocab = hidden.stride(0), weight.stride(0), ignore_index, vocab
-    a.dtype, a.targets_wide, a.inv_temp = K._DT[hidden.dtype], targets.dtype == torch.int64, inv_temp
-    if index is not None:
-        a.index, a.count = index.data_ptr(), index.data_ptr() + 4 * a.rows
-    if part is not None:
-        a.part = part.data_ptr()
-    if weights is not None:
-        a.weights, a.ld_weights = weights.data_ptr(), weights.stride(0)
-    return a
+def _head_args(hidden, weight, targets, index, moved, stats: int, part: int, weights, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
+    rows, width = hidden.shape
+    at = (None, None, None) if index is None else (index.data_ptr(), index.data_ptr() + 4 * rows, moved.data_ptr())
+    held, ld = (None, 0) if weights is None else (weights.data_ptr(), weights.stride(0))
+    return HeadArgs(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), *at, stats, part, held, K.status_word(hidden.device).data_ptr(),
+                    ld, rows, hidden.stride(0), weight.stride(0), ignore_index, vocab, width, K._DT[hidden.dtype], targets.dtype == torch.int64,
+                    inv_temp, 0)
 
 
 def _gathered(hidden) -> torch.Tensor:
@@ -217,20 +210,28 @@ def _head_pitch(vocab: int) -> int:
 
 def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, want_grad: bool, recompute: bool = False):
     """FP32 logp (of the shape of `targets`) for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient
-    needs: (stats, index of the rows that count, with their number behind it, or None, the column tiles' maxima and the logits' exponentials, or
-    None twice)."""
+    needs (all None where it is not wanted): stats, index of the rows that count, with their number behind it, and the column tiles' maxima and
+    the logits' exponentials where these are held."""
     rows, dev = hidden.shape[0], hidden.device
-    index = torch.empty(rows + 1, dtype=torch.int32, device=dev) if want_grad or rows > HEAD_TILE else None
     logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    parts = 2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * rows
+    if not want_grad:    # one block of scratch: column tiles and statistics (pairs), targets' logits
+        scratch = torch.empty(parts + 3 * rows, dtype=torch.float32, device=dev)
+        at = scratch.data_ptr()
+        index = torch.empty(rows + 1, dtype=torch.int32, device=dev) if rows > HEAD_TILE else None
+        moved = None if index is None else _gathered(hidden)
+        a = _head_args(hidden, weight, targets, index, moved, at + 4 * parts, at, None, vocab, ignore_index, inv_temp)
+        _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), at + 4 * (parts + 2 * rows))
+        return logp, None, None, None, None
+    index = torch.empty(rows + 1, dtype=torch.int32, device=dev)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    part = torch.empty(2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * rows, dtype=torch.float32, device=dev)
+    part = torch.empty(parts, dtype=torch.float32, device=dev)
     tlogit = torch.empty(rows, dtype=torch.float32, device=dev)
     full, ld = -(-rows // HEAD_TILE) * HEAD_TILE, _head_pitch(vocab)
-    keep = want_grad and not recompute and hidden.shape[1] >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
+    keep = not recompute and hidden.shape[1] >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
     weights = torch.empty((full, ld), dtype=hidden.dtype, device=dev) if keep else None
-    a = _head_args(hidden, weight, targets, index, stats, part, weights, vocab, ignore_index, inv_temp)
-    moved = _gathered(hidden) if index is not None else None
-    a.gathered = None if moved is None else moved.data_ptr()
+    moved = _gathered(hidden)
+    a = _head_args(hidden, weight, targets, index, moved, stats.data_ptr(), part.data_ptr(), weights, vocab, ignore_index, inv_temp)
     _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), tlogit.data_ptr())
     return logp, stats, index, (part if keep else None), weights
 
@@ -250,9 +251,9 @@ def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, i
     logits in place, unless they are needed `again`."""
     rows, width = hidden.shape
     dev, dtype = hidden.device, hidden.dtype
-    a = _head_args(hidden, weight, targets, index, stats, part, weights, vocab, ignore_index, inv_temp)
     moved = _gathered(hidden)
-    a.gathered = moved.data_ptr()
+    a = _head_args(hidden, weight, targets, index, moved, stats.data_ptr(), None if part is None else part.data_ptr(), weights, vocab, ignore_index,
+                   inv_temp)
     g = HeadGrad()
     ld = _head_pitch(vocab)
     chunk = -(-rows // HEAD_TILE) * HEAD_TILE

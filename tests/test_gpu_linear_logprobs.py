@@ -248,6 +248,23 @@ def test_other_types_and_sizes_go_through_the_logits():
     assert F.linear_logprobs(torch.zeros(0, 64, device="cuda", dtype=BF16), w.new_zeros(5, 64), torch.zeros(0, dtype=torch.long, device="cuda")).shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows", [1, 3, 16, 17, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("d,vocab", [(8, 1), (72, 31), (1088, 33), (64, 5000), (1600, 20011), (2056, 4737)])
+def test_few_rows(dtype, rows, d, vocab):
+    """The form for single tokens: runs of the vocabulary per SM, fewer groups than SMs, runs that end inside a tile."""
+    h, w, t, _ = make((rows,), d, vocab, dtype, seed=rows + d)
+    if rows > 2:
+        t[1] = -100
+        t[2] = vocab
+    logp = F.linear_logprobs(h, w, t, temperature=0.9)
+    tk = torch.where(t >= vocab, -100, t)
+    want = expect(h, w, tk, vocab, torch.ones(rows, device="cuda"), 0.9)
+    bad = t >= vocab
+    assert torch.equal(torch.isnan(logp), bad)
+    close(logp[~bad], want[0][~bad], want[1][~bad])
+
+
 def test_agrees_with_logits_in_memory():
     h, w, t, _ = make((4, 100), 256, 2000, BF16, seed=3)
     x = h.float().reshape(-1, 256) @ w.float().t()
