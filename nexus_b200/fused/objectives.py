@@ -12,13 +12,15 @@ from __future__ import annotations
 
 import contextlib
 import math
+from operator import attrgetter
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 from torch.autograd.function import once_differentiable
 
 _KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
-_KERNEL_SET = set(_KERNEL_TYPES)
+_BYTES = (2, 4, 2)     # of the kernels' type codes
+_shape = attrgetter("shape")
 _TARGET_TYPES = (torch.int32, torch.int64)
 O = None     # nexus_b200.ops._objectives, once a tensor on a GPU has been met
 
@@ -458,24 +460,28 @@ def _separate(name: str, grads, out):
     return grads
 
 
-def _plain_list(grads, out) -> Optional[List[int]]:
-    """Numbers of elements of a list that needs no second look: contiguous, non-empty tensors of one GPU that the kernels take, each with memory of
-    its own.  None for every other list, wrong ones among them."""
+def _plain_table(grads, out):
+    """The `grad_table` of a list that needs no second look: contiguous, non-empty tensors of one GPU that the kernels take, each with memory of its
+    own.  None for every other list, wrong ones among them."""
     every = grads if out is None else grads + out
-    if not every or not all([isinstance(t, torch.Tensor) for t in every]) or not every[0].is_cuda:
-        return None
-    if len({t.device for t in every}) != 1 or not {t.dtype for t in every} <= _KERNEL_SET or {t.layout for t in every} != {torch.strided}:
-        return None
-    if not all([t.is_contiguous() for t in every]) or (out is not None and [t.shape for t in grads] != [t.shape for t in out]):
-        return None
-    counts = [t.numel() for t in grads]
-    at = sorted([(t.data_ptr(), t.nbytes) for t in every])
-    end = 0
-    for start, size in at:
-        if start < end or size == 0:
+    try:
+        if not every or not _kernels(every[0]) or len(set(map(torch.Tensor.get_device, every))) != 1 or not all(map(torch.Tensor.is_contiguous, every)):
             return None
-        end = start + size
-    return counts if _kernels(grads[0]) else None
+        if out is not None and list(map(_shape, grads)) != list(map(_shape, out)):
+            return None
+        src, dst, counts, types = table = O.grad_table(grads, out)
+    except (AttributeError, KeyError, NotImplementedError, RuntimeError, TypeError):   # no tensors, or ones of other types, or without plain memory
+        return None
+    spans = [(at, n * _BYTES[t & 15]) for at, n, t in zip(src, counts, types)]
+    if dst is not None:
+        spans += [(at, n * _BYTES[t >> 4]) for at, n, t in zip(dst, counts, types)]
+    spans.sort()
+    end = 0
+    for at, size in spans:
+        if at < end or size == 0:
+            return None
+        end = at + size
+    return table
 
 
 def _square_sum_plain(grads) -> float:
@@ -500,7 +506,7 @@ def grad_square_sum(grads: Sequence[Optional[torch.Tensor]]) -> float:
         return _square_sum_plain(grads)
     with _on(grads[0]):
         ts = [_packed(g) for g in grads if g.numel()]
-        return float(O.grad_clip(ts, [t.numel() for t in ts], None)[0]) if ts else 0.0
+        return float(O.grad_clip(O.grad_table(ts), ts[0].device, None)[0]) if ts else 0.0
 
 
 def clip_grads(name: str, grads, max_norm: float, out=None):
@@ -509,10 +515,10 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
         raise ValueError(f"{name}: max_norm must not be negative, got {max_norm}")
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     out = out if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
-    counts = _plain_list(grads, out)
-    if counts is not None:
+    table = _plain_table(grads, out)
+    if table is not None:
         with _on(grads[0]):
-            norms = O.grad_clip(grads, counts, max_norm, out)
+            norms = O.grad_clip(table, grads[0].device, max_norm)
         torch.autograd.graph.increment_version(grads if out is None else out)
         return norms
     grads, out = _grad_list(name, grads, out)
@@ -535,7 +541,7 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
             with _on(full[0]):
                 src = [_packed(g) for g in full]
                 if outs is None:
-                    norms = O.grad_clip(src, [t.numel() for t in src], max_norm)
+                    norms = O.grad_clip(O.grad_table(src), src[0].device, max_norm)
                     torch.autograd.graph.increment_version(src)
                     for g, s in zip(full, src):
                         if s is not g:
@@ -543,7 +549,7 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
                     return norms
                 # element order of the memory: an output of another order than its gradient is written through a copy of that order
                 dst = [o if o.stride() == s.stride() else torch.empty_like(s, dtype=o.dtype) for o, s in zip(outs, src)]
-                norms = O.grad_clip(src, [t.numel() for t in src], max_norm, dst)
+                norms = O.grad_clip(O.grad_table(src, dst), src[0].device, max_norm)
                 torch.autograd.graph.increment_version(dst)
                 for o, d in zip(outs, dst):
                     if d is not o:

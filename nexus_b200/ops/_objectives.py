@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes as C
 from array import array
+from operator import attrgetter
 from typing import Optional, Tuple
 
 import torch
@@ -286,18 +287,26 @@ GRAD_TABLE = 256                 # tensors of a launch, and
 GRAD_PARTS = 4 * 148             # partial sums that it leaves, at most
 
 
-def grad_clip(grads, counts, max_norm: Optional[float], out=None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(FP64 sum of squares, FP32 norm) of dense, non-empty tensors of `counts` elements; with `max_norm` they are clipped, in place or into
-    `out`."""
-    n, dt = len(grads), K._DT
-    src, count = array("Q", [t.data_ptr() for t in grads]), array("q", counts)
+_ptr, _numel, _dtype = torch.Tensor.data_ptr, torch.Tensor.numel, attrgetter("dtype")
+
+
+def grad_table(grads, out=None):
+    """Pointers, numbers of elements and types of dense tensors, as `grad_clip` takes them: (sources, destinations or None, counts, types)."""
+    code = K._DT.__getitem__
+    src, counts, kinds = list(map(_ptr, grads)), list(map(_numel, grads)), list(map(code, map(_dtype, grads)))
     if out is None:
-        types, dst = bytes([17 * dt[t.dtype] for t in grads]), None
-    else:
-        types = bytes([dt[t.dtype] | dt[o.dtype] << 4 for t, o in zip(grads, out)])
-        dst = array("Q", [t.data_ptr() for t in out])
-    buf = torch.empty(2 + -(-n // GRAD_TABLE) * GRAD_PARTS, dtype=torch.float64, device=grads[0].device)
-    a = GradTable(src.buffer_info()[0], None if dst is None else dst.buffer_info()[0], count.buffer_info()[0],
+        return src, None, counts, bytes([17 * c for c in kinds])
+    return src, list(map(_ptr, out)), counts, bytes([c | o << 4 for c, o in zip(kinds, map(code, map(_dtype, out)))])
+
+
+def grad_clip(table, device, max_norm: Optional[float]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(FP64 sum of squares, FP32 norm) of the dense, non-empty tensors of a `grad_table`; with `max_norm` they are clipped, in place or into their
+    destinations."""
+    src, dst, counts, types = table
+    n = len(src)
+    src, counts, dst = array("Q", src), array("q", counts), None if dst is None else array("Q", dst)
+    buf = torch.empty(2 + -(-n // GRAD_TABLE) * GRAD_PARTS, dtype=torch.float64, device=device)
+    a = GradTable(src.buffer_info()[0], None if dst is None else dst.buffer_info()[0], counts.buffer_info()[0],
                   C.cast(C.c_char_p(types), C.c_void_p), n)
     at = buf.data_ptr()
     _call("nx_grad_clip", C.byref(a), 0.0 if max_norm is None else max_norm, max_norm is not None, at + 16, at)

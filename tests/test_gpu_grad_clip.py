@@ -161,3 +161,18 @@ def test_trainer_and_adamw_take_the_kernels_norm():
     before = K.launch_count
     norm = F.adamw_multi_tensor(ps, gs, m, v, 1, 1e-2, max_grad_norm=1.0)
     assert K.launch_count > before and norm == pytest.approx(true_norm(gs), rel=1e-13)
+
+
+def test_lists_that_are_no_plain_ones():
+    """What the quick look over a list leaves to the second one."""
+    a = torch.ones(8, device="cuda")
+    for call in (lambda: F.clip_grad_norm_([a, 3.0], 1.0), lambda: F.clip_grad_norm_([a, a.to_sparse()], 1.0),
+                 lambda: F.clip_grad_norm_([a, a.int()], 1.0), lambda: F.clip_grad_norm_([a.view(2, 4)], 1.0, out=[torch.ones(4, 2, device="cuda")]),
+                 lambda: F.clip_grad_norm_([a.view(BF16)[:8], a.view(F16)[:8]], 1.0), lambda: F.clip_grad_norm_([a], 1.0, out=[a.view(BF16)[:8]])):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.equal(a, torch.ones(8, device="cuda"))
+    out = [torch.empty(8, device="cuda", dtype=torch.float64)]
+    assert float(F.clip_grad_norm_([a], 1.0, out=out)) == pytest.approx(math.sqrt(8.0), rel=1e-6)
+    assert float(out[0][0]) == pytest.approx(1 / math.sqrt(8.0), rel=1e-5)
+    assert torch.equal(F.clip_grad_norm_(a, 100.0), F.clip_grad_norm_([a], 100.0, out=[a]))
