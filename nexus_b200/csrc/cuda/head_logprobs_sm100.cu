@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const Params p, int parts, f
       return;
     }
     logp[at] = (p.tlogit[mine] - m) * p.inv_temp - logf(s);
-    stats[mine] = make_float2(m, log2f(s));
+    stats[p.row0 + mine] = make_float2(m, log2f(s));
   }
 }
 
@@ -1094,7 +1094,7 @@ bool args_ok(const NxHeadArgs* a) {
          !off(a->weight) && a->ld_hidden % 8 == 0 && a->ld_weight % 8 == 0 && a->ld_hidden >= a->width && a->ld_weight >= a->width &&
          a->stats != nullptr && a->status != nullptr && (a->index == nullptr) == (a->count == nullptr) &&
          (a->index == nullptr) == (a->gathered == nullptr) && !off(a->gathered) &&
-         (a->weights == nullptr || (!off(a->weights) && a->ld_weights >= a->vocab && a->ld_weights % 64 == 0));
+         a->part_rows > 0 && a->part_rows % kTile == 0 && (a->weights == nullptr || (!off(a->weights) && a->part_rows >= a->rows && a->ld_weights >= a->vocab && a->ld_weights % 64 == 0));
 }
 
 Params base_params(const NxHeadArgs* a) {
@@ -1114,7 +1114,7 @@ Params base_params(const NxHeadArgs* a) {
   p.slices = 1;
   p.part_blocks = 1024 / kBK;
   p.part = reinterpret_cast<float2*>(a->part);
-  p.part_ld = a->rows;
+  p.part_ld = a->part_rows;
   // row tiles whose part of h is about 40 MB pass over the vocabulary together
   p.group = static_cast<int>(std::max<int64_t>(1, (40ll << 20) / (static_cast<int64_t>(kTile) * a->width * 2)));
   return p;
@@ -1141,26 +1141,32 @@ extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* tlogit,
   }
   Params p = base_params(a);
   p.tlogit = tlogit;
-  auto join = [&](int parts) {
-    NX_PDL(join_kernel, static_cast<unsigned>((a->rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
+  auto join = [&](int64_t rows, int parts) {
+    NX_PDL(join_kernel, static_cast<unsigned>((rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
     return 0;
   };
   if (a->index == nullptr && a->rows <= kFewRows) {
     // a part for every SM; `part` has room for one per 128 columns
     const int blocks = static_cast<int>(std::min<int64_t>(kNumSmsB200, 2 * tiles(a->vocab)));
     rc = a->dtype == NX_BF16 ? launch_few<true>(a, p, blocks, st) : launch_few<false>(a, p, blocks, st);
-    return rc != 0 ? rc : join(blocks);
+    return rc != 0 ? rc : join(a->rows, blocks);
   }
   const void* h = a->index != nullptr ? a->gathered : a->hidden;
   const int64_t ldh = a->index != nullptr ? a->width : a->ld_hidden;
   CUtensorMap ma, mb;
-  if ((rc = map_k(&ma, a, h, a->width, a->rows, ldh)) != 0 || (rc = map_k(&mb, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0) return rc;
+  if ((rc = map_k(&mb, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0) return rc;
   p.keep = a->weights != nullptr;
-  CUtensorMap mo = ma;
-  if (p.keep && (rc = map_store(&mo, a, a->weights, a->vocab, (a->rows + kTile - 1) / kTile * kTile, a->ld_weights)) != 0) return rc;
-  p.cap = (a->rows + kTile - 1) / kTile * kTile;
-  if ((rc = NX_HEAD(kStats, ma, mb, mo, p, tiles(a->rows) * tiles(a->vocab), st)) != 0) return rc;
-  return join(static_cast<int>((a->vocab + 127) / 128));  // the last column tile may have no second half
+  for (; p.row0 < a->rows; p.row0 += a->part_rows) {  // as many rows at a time as `part` has room for
+    const int64_t here = std::min(a->part_rows, a->rows - p.row0);
+    if ((rc = map_k(&ma, a, static_cast<const uint16_t*>(h) + p.row0 * ldh, a->width, here, ldh)) != 0) return rc;
+    CUtensorMap mo = ma;
+    p.cap = tiles(here) * kTile;
+    if (p.keep && (rc = map_store(&mo, a, a->weights, a->vocab, p.cap, a->ld_weights)) != 0) return rc;
+    if ((rc = NX_HEAD(kStats, ma, mb, mo, p, tiles(here) * tiles(a->vocab), st)) != 0) return rc;
+    // the last column tile may have no second half
+    if ((rc = join(here, static_cast<int>((a->vocab + 127) / 128))) != 0) return rc;
+  }
+  return 0;
 }
 
 extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, nx_stream_t stream) {

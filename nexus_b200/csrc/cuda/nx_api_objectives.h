@@ -75,10 +75,11 @@ typedef struct NxHeadArgs {
   int32_t* count;
   void* gathered;
   float* stats;
-  float* part;     // [2 * (vocab / 256 rounded up), rows] pairs: scratch of the forward call; with `weights` read by the gradient too
+  float* part;     // [2 * (vocab / 256 rounded up), part_rows] pairs: scratch of the forward call, which takes part_rows (a multiple of 256) rows
+                   // at a time; with `weights` all at once, and read by the gradient too
   void* weights;   // may be null: [rows rounded up to 256, ld_weights] of the operands' type, the logits' exponentials for the gradient
   int* status;     // receives a non-zero nx::StatusCode when a wait timed out
-  int64_t ld_weights, rows, ld_hidden, ld_weight, ignore_index;
+  int64_t part_rows, ld_weights, rows, ld_hidden, ld_weight, ignore_index;
   int32_t vocab, width, dtype, targets_wide;
   float inv_temp;
   int32_t pad_;

@@ -165,7 +165,7 @@ def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, k
 class HeadArgs(C.Structure):
     _fields_ = [("hidden", C.c_void_p), ("weight", C.c_void_p), ("targets", C.c_void_p), ("index", C.c_void_p), ("count", C.c_void_p),
                 ("gathered", C.c_void_p), ("stats", C.c_void_p), ("part", C.c_void_p), ("weights", C.c_void_p), ("status", C.c_void_p),
-                ("ld_weights", C.c_int64), ("rows", C.c_int64), ("ld_hidden", C.c_int64),
+                ("part_rows", C.c_int64), ("ld_weights", C.c_int64), ("rows", C.c_int64), ("ld_hidden", C.c_int64),
                 ("ld_weight", C.c_int64), ("ignore_index", C.c_int64), ("vocab", C.c_int32), ("width", C.c_int32), ("dtype", C.c_int32),
                 ("targets_wide", C.c_int32), ("inv_temp", C.c_float), ("pad_", C.c_int32)]
 
@@ -178,6 +178,7 @@ class HeadGrad(C.Structure):
 
 HEAD_TILE = 256
 HEAD_PARTS = 2                   # maxima and sums of a row that a column tile leaves
+HEAD_ROWS = 1 << 16              # rows whose column tiles' maxima and sums are in memory at a time
 HEAD_GRAD_ELEMENTS = 1 << 29     # of the logits' gradient at a time: 1 GiB
 # From this width on the exponentials are held: writing them and turning them into the gradient is traffic per logit, making the logits again
 # work per logit and column.  Both, forward and backward together without the products with the gradient, at 896 columns (380 x 151936, FP16):
@@ -197,8 +198,12 @@ def _head_args(hidden, weight, targets, index, moved, stats: int, part: int, wei
     at = (None, None, None) if index is None else (index.data_ptr(), index.data_ptr() + 4 * rows, moved.data_ptr())
     held, ld = (None, 0) if weights is None else (weights.data_ptr(), weights.stride(0))
     return HeadArgs(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), *at, stats, part, held, K.status_word(hidden.device).data_ptr(),
-                    ld, rows, hidden.stride(0), weight.stride(0), ignore_index, vocab, width, K._DT[hidden.dtype], targets.dtype == torch.int64,
+                    _part_rows(rows), ld, rows, hidden.stride(0), weight.stride(0), ignore_index, vocab, width, K._DT[hidden.dtype], targets.dtype == torch.int64,
                     inv_temp, 0)
+
+
+def _part_rows(rows: int) -> int:
+    return min(HEAD_ROWS, -(-rows // HEAD_TILE) * HEAD_TILE)
 
 
 def _gathered(hidden) -> torch.Tensor:
@@ -215,7 +220,7 @@ def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_te
     the logits' exponentials where these are held."""
     rows, dev = hidden.shape[0], hidden.device
     logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-    parts = 2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * rows
+    parts = 2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * _part_rows(rows)
     if not want_grad:    # one block of scratch: column tiles and statistics (pairs), targets' logits
         scratch = torch.empty(parts + 3 * rows, dtype=torch.float32, device=dev)
         at = scratch.data_ptr()
@@ -229,7 +234,7 @@ def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_te
     part = torch.empty(parts, dtype=torch.float32, device=dev)
     tlogit = torch.empty(rows, dtype=torch.float32, device=dev)
     full, ld = -(-rows // HEAD_TILE) * HEAD_TILE, _head_pitch(vocab)
-    keep = not recompute and hidden.shape[1] >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
+    keep = not recompute and rows <= HEAD_ROWS and hidden.shape[1] >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
     weights = torch.empty((full, ld), dtype=hidden.dtype, device=dev) if keep else None
     moved = _gathered(hidden)
     a = _head_args(hidden, weight, targets, index, moved, stats.data_ptr(), part.data_ptr(), weights, vocab, ignore_index, inv_temp)

@@ -85,7 +85,7 @@ def test_bf16_training_loop_runs():
     ps = list(m.parameters())
     with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
         old, refl = m.token_logprobs(tokens, mask), ref.token_logprobs(tokens, mask)
-        h, w = m.hidden(tokens), m.wte
+        h, w = m.hidden(tokens), m.lm_head          # not tied by default
         assert torch.equal(old, F.linear_logprobs(h.bfloat16(), w.bfloat16(), m._next_targets(tokens, mask), vocab=500))
     assert torch.equal(old, refl) and old.dtype == torch.float32
     for step in (1, 2, 3):

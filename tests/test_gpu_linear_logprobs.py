@@ -127,6 +127,31 @@ def test_chunks_of_rows(rows, monkeypatch):
             close(w2.grad, want[4], want[5])
 
 
+def test_forward_in_pieces_of_rows(monkeypatch):
+    from nexus_b200.ops import _objectives as O
+    h, w, t, g = make((900,), 72, 700, BF16, seed=12)
+    t[::5] = -100
+    t[7] = -3
+    dl = torch.randn(900, generator=g).cuda()
+    results = []
+    for rows in (1 << 16, 256, 512):
+        monkeypatch.setattr(O, "HEAD_ROWS", rows)
+        h2, w2 = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        with torch.no_grad():
+            plain = F.linear_logprobs(h2, w2, t)
+        logp = F.linear_logprobs(h2, w2, t)
+        assert torch.equal(plain.nan_to_num(9.0), logp.detach().nan_to_num(9.0)) and int(torch.isnan(plain).sum()) == 1
+        results.append((plain.nan_to_num(9.0), *torch.autograd.grad(logp, (h2, w2), dl)))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def test_one_token_without_a_batch():
+    h, w, t, _ = make((1,), 64, 50, BF16)
+    a = F.linear_logprobs(h[0], w, t[0])
+    assert a.shape == () and torch.equal(a, F.linear_logprobs(h, w, t)[0])
+
+
 def test_slices_of_the_vocabulary():
     from nexus_b200.ops import _objectives as O
     assert O.head_slices(300, 64) > 1 and O.head_slices(8192, 4096) == 1

@@ -276,6 +276,84 @@ def test_policy_loss(dtype, vocab, pitch, kl, reduction, ent, wide):
         assert bool((x.grad[..., vocab:] == 0).all())
 
 
+@pytest.mark.parametrize("vocab", [20011, 57327, 57344, 57353, 120000, 230001])
+@pytest.mark.parametrize("ent", [0.0, 0.02])
+def test_policy_many_rows(vocab, ent):
+    """Rows for every SM, at both sides of what the shorter ring holds, longer than the longer one, at odd addresses."""
+    B, T = 2, 90
+    x, t, old, ref, g = policy_inputs(B, T, vocab, BF16, seed=vocab)
+    t[0, 5:30] = -100
+    adv = torch.randn(B, generator=g).cuda()
+    want = policy64(x, t, old, adv, ref, vocab, "k3", "token", 0.1, ent, 0.2, 0.28)
+    x.requires_grad_(True)
+    r = F.policy_loss(x, t, old, adv, ref, clip_low=0.2, clip_high=0.28, kl_coef=0.1, entropy_coef=ent)
+    r.loss.backward()
+    err = logp_error(want[1], vocab)
+    close(r.logp, want[1], err)
+    close(r.entropy, want[3], U * (8 * want[3] + 40 + 2 * chain(vocab)) * (want[3] != 0))
+    p = softmax64(x, vocab, 1.0).exp()
+    keep = (t != -100)[..., None]
+    n = float(keep.sum())
+    size = torch.full_like(p[..., :1], (float(adv.abs().max()) * 2 + 0.1 * float(want[2].abs().max() + 1) + ent * 40) / n) * keep
+    close(x.grad, want[4], grad_error(want[4], p, size, BF16, vocab, coef_rel=float(4 * err.max() + 32 * U)) * keep)
+    a = F.token_logprobs(x.detach(), t)
+    close(a, want[1], err)
+
+
+def test_offsets_beyond_32_bits():
+    """Logits of more than 2^31 elements: the last rows and their gradients."""
+    vocab, rows = 50257, 43000
+    x = torch.empty(1, rows, vocab, dtype=BF16, device="cuda")
+    x.view(-1)[: vocab * 1000].normal_()
+    x.view(-1)[-vocab * 1000:].normal_()
+    t = torch.full((1, rows), -100, device="cuda")
+    t[0, :3] = t[0, -3:] = torch.tensor([0, 777, vocab - 1], device="cuda")
+    assert x.numel() > 2 ** 31
+    x.requires_grad_(True)
+    zero = torch.full((1, rows), -11.0, device="cuda")
+    logp = F.token_logprobs(x, t)
+    logp.backward(torch.ones_like(logp))
+    token_grad, x.grad = x.grad, None
+    r = F.policy_loss(x, t, zero, torch.ones(1, device="cuda"), reduction="sum")
+    r.loss.backward()  # its sums run over other threads than those of `token_logprobs`: each is held against the 64-bit values by itself
+    for part in (slice(0, 3), slice(rows - 3, rows)):
+        lp = torch.log_softmax(x.detach()[0, part].double(), -1)
+        want = lp.gather(1, t[0, part][:, None])[:, 0]
+        close(logp.detach()[0, part], want, logp_error(want, vocab))
+        close(r.logp[0, part], want, logp_error(want, vocab))
+        gw = -lp.exp()
+        gw.scatter_add_(1, t[0, part][:, None], torch.ones(3, 1, dtype=torch.float64, device="cuda"))
+        one = torch.ones(3, 1, dtype=torch.float64, device="cuda")
+        close(token_grad[0, part], gw, grad_error(gw, lp.exp(), one, BF16, vocab))
+        ratio = torch.exp(want + 11.0)[:, None]
+        c = torch.where(ratio <= 1.2, -ratio, 0.0)
+        close(x.grad[0, part], c * gw, grad_error(c * gw, lp.exp(), c.abs(), BF16, vocab, coef_rel=64 * U))
+    assert bool((token_grad[0, 3: 1000] == 0).all()) and bool((x.grad[0, rows - 1000: rows - 3] == 0).all())
+
+
+def test_one_token_without_a_batch():
+    x, t, _ = make((1,), 50, F32)
+    a = F.token_logprobs(x[0], t[0])
+    assert a.shape == () and torch.equal(a, F.token_logprobs(x, t)[0])
+
+
+def test_saved_tensors_on_the_host():
+    """Saved tensors that hooks move away and bring back at other addresses."""
+    x, t, old, ref, g = policy_inputs(2, 6, 333, BF16, 336)
+    adv = torch.randn(2, generator=g).cuda()
+    x.requires_grad_(True)
+
+    def grads():
+        a = torch.autograd.grad(F.policy_loss(x, t, old, adv, ref, kl_coef=0.1, vocab=333).loss * 0.5, x)[0]
+        b = torch.autograd.grad(F.token_logprobs(x[:, 1:, :333], t[:, 1:]).sum(), x)[0]
+        return a, b, torch.autograd.grad(F.preference_loss(x, t, vocab=333).loss, x)[0]
+
+    plain = grads()
+    with torch.autograd.graph.save_on_cpu():
+        moved = grads()
+    assert all(torch.equal(a, b) for a, b in zip(plain, moved))
+
+
 def test_policy_gradient_against_differences():
     """The gradient in FP32 against central differences of the loss in 64 bits along random directions."""
     B, T, vocab = 2, 6, 257
