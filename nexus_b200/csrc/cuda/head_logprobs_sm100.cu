@@ -837,14 +837,16 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* __restric
   }
 }
 
-// Joins the column tiles' maxima and sums of a row: 32 rows per block, a warp per share of the tiles.
+// Joins the column tiles' maxima and sums of a row.  Eight rows per block (64 contiguous bytes of every tile), a quarter of a warp's lanes per row
+// and four loads of each in flight: 1188 tiles of 380 rows took 24 us with 32 rows per block and a load at a time.
+constexpr int kJoinRows = 8;
 __global__ void __launch_bounds__(1024) join_kernel(const Params p, int parts, float* __restrict__ logp, float2* __restrict__ stats) {
-  __shared__ float2 share[32][33];
+  __shared__ float2 share[32][kJoinRows + 1];
   pdl_dependency();
   pdl_trigger();
-  const int64_t live = live_rows(p), row = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (static_cast<int64_t>(blockIdx.x) * 32 >= live) return;
+  const int64_t live = live_rows(p), row0 = static_cast<int64_t>(blockIdx.x) * kJoinRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in = lane & (kJoinRows - 1);
+  if (row0 >= live) return;
   const float k2 = p.inv_temp * kLog2e;
   float top = -INFINITY, sum = 0.0f;
   auto take = [&](const float2 v) {
@@ -855,15 +857,33 @@ __global__ void __launch_bounds__(1024) join_kernel(const Params p, int parts, f
     // a part of nothing but -inf has the sum 0 (or NaN)
     sum += v.x == -INFINITY ? v.y : v.y * ex2((v.x - top) * k2);
   };
-  if (row < live)
-    for (int i = warp; i < parts; i += 32) take(p.part[i * p.part_ld + row]);
-  share[warp][lane] = make_float2(top, sum);
+  if (row0 + in < live) {
+    const float2* const from = p.part + row0 + in;
+    int i = threadIdx.x / kJoinRows;
+    for (; i + 3 * 128 < parts; i += 4 * 128) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = from[(i + u * 128) * p.part_ld];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) take(v[u]);
+    }
+    for (; i < parts; i += 128) take(from[i * p.part_ld]);
+  }
+  auto meet = [&](int o) {  // with the lane that is `o` away and has the same row
+    const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
+    const float m = fmaxf(top, v.x);
+    sum = (top == -INFINITY ? sum : sum * ex2((top - m) * k2)) + (v.x == -INFINITY ? v.y : v.y * ex2((v.x - m) * k2));
+    top = m;
+  };
+  meet(8);
+  meet(16);
+  if (lane < kJoinRows) share[warp][lane] = make_float2(top, sum);
   __syncthreads();
-  const int r = warp;  // now a warp takes a row, a lane a share
-  const float2 v = share[lane][r];
+  if (warp >= kJoinRows) return;
+  const float2 v = share[lane][warp];  // a warp takes a row, a lane a warp's share
   const float m = warp_max(v.x);
   const float s = warp_sum(v.x == -INFINITY ? v.y : v.y * ex2((v.x - m) * k2));
-  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + r;
+  const int64_t mine = row0 + warp;
   if (lane == 0 && mine < live) {
     const int64_t at = place(p, mine);
     const int64_t tg = target_of(p.targets, p.targets_wide, at);
@@ -1142,7 +1162,7 @@ extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* tlogit,
   Params p = base_params(a);
   p.tlogit = tlogit;
   auto join = [&](int64_t rows, int parts) {
-    NX_PDL(join_kernel, static_cast<unsigned>((rows + 31) / 32), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
+    NX_PDL(join_kernel, static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows), 1024, 0, st, p, parts, logp, reinterpret_cast<float2*>(a->stats));
     return 0;
   };
   if (a->index == nullptr && a->rows <= kFewRows) {
