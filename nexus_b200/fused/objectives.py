@@ -192,7 +192,7 @@ class _LinearLogprobs(torch.autograd.Function):
 def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
                     vocab: Optional[int] = None, recompute: bool = False) -> torch.Tensor:
     """`token_logprobs` of the logits ``hidden @ weight.T`` without the logits in memory: hidden [..., d], weight [V(+pad), d] of one type,
-    targets [...].  Differentiable (once) with respect to both.  Where a gradient is wanted, d is 1024 or more and there are at most 2^29 logits, their exponentials
+    targets [...].  Differentiable (once) with respect to both.  Where a gradient is wanted, d is 512 or more and there are at most 2^29 logits, their exponentials
     are held in 16 bits (1 GiB at most) until the backward pass turns them into the logits' gradient in place; else, or with
     ``recompute``, nothing is held and the backward pass makes the logits again (a third more products), their gradient of at most 2^29 logits
     (or of 256 rows) at a time.  The kernels take BF16 and FP16 with d a multiple of 8 (logits in FP32, rounded nowhere; their gradient rounded to the type for

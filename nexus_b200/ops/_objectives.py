@@ -181,9 +181,9 @@ HEAD_PARTS = 2                   # maxima and sums of a row that a column tile l
 HEAD_ROWS = 1 << 16              # rows whose column tiles' maxima and sums are in memory at a time
 HEAD_GRAD_ELEMENTS = 1 << 29     # of the logits' gradient at a time: 1 GiB
 # From this width on the exponentials are held: writing them and turning them into the gradient is traffic per logit, making the logits again
-# work per logit and column.  Both, forward and backward together without the products with the gradient, at 896 columns (380 x 151936, FP16):
-# 228 held, 209 us again; at 4096 (5376 x 32000, BF16) 1150 and 2050 us.
-HEAD_KEEP_WIDTH = 1024
+# work per logit and column.  Forward and backward pass, held and again, us: 4096 x 50257 BF16 at 256 columns 549 and 540, 384 682 and 679, 512 711
+# and 741, 1024 1084 and 1207, 2048 2010 and 2327; 380 x 151936 FP16 at 896 columns 435 and 487.
+HEAD_KEEP_WIDTH = 512
 
 
 def head_rows(t: torch.Tensor) -> torch.Tensor:

@@ -168,7 +168,7 @@ def test_slices_of_the_vocabulary():
         close(w.grad, want[4], want[5])
 
 
-@pytest.mark.parametrize("keep_width", [0, 1024])
+@pytest.mark.parametrize("keep_width", [0, 1 << 30])
 def test_backward_twice(keep_width, monkeypatch):
     from nexus_b200.ops import _objectives as O
     monkeypatch.setattr(O, "HEAD_KEEP_WIDTH", keep_width)
