@@ -142,7 +142,7 @@ class _TokenLogprobs(torch.autograd.Function):
             logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
             coef = dlogp.float().contiguous()
             grad = O.empty_grad(logits)
-            O.token_logprobs_grad(rows, stats, coef, 1, None, grad)
+            O.token_logprobs_grad(rows, stats, coef.data_ptr(), 1, None, grad)
         return grad, None, None, None, None
 
 
@@ -224,19 +224,19 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
 
 # ---------------------------------------------------------------------------------------------------------- policy loss
-def _policy_forward(logits, targets, vocab, ignore_index, temperature, args, want_grad):
+def _policy_forward(logits, targets, vocab, ignore_index, temperature, old, args, want_grad):
     with _on(logits):
         logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
         grad = O.empty_grad(logits) if want_grad else None
-        return O.policy_loss(rows, args, targets, grad), grad
+        return O.policy_loss(rows, args, old, grad), grad
 
 
 class _PolicyLoss(torch.autograd.Function):
     """Loss and gradient from one pass; the backward pass multiplies the gradient where the loss's own is not 1."""
 
     @staticmethod
-    def forward(ctx, logits, targets, vocab, ignore_index, temperature, args):
-        (loss, logp, kl, entropy), grad = _policy_forward(logits, targets, vocab, ignore_index, temperature, args, True)
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature, old, args):
+        (loss, logp, kl, entropy), grad = _policy_forward(logits, targets, vocab, ignore_index, temperature, old, args, True)
         ctx.save_for_backward(grad)
         ctx.mark_non_differentiable(logp, kl, entropy)
         ctx.set_materialize_grads(False)
@@ -246,14 +246,14 @@ class _PolicyLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss, *_):
         if dloss is None:
-            return (None,) * 6
+            return (None,) * 7
         (grad,) = ctx.saved_tensors
         # a graph that is kept may be walked again, and then needs the gradient as it was
         if torch._C._autograd._get_current_graph_task_keep_graph():
-            return ((grad.float() * dloss.float()).to(grad.dtype), *(None,) * 5)
+            return ((grad.float() * dloss.float()).to(grad.dtype), *(None,) * 6)
         with _on(grad):
             O.scale_unless_one_(grad, dloss.float())
-        return (grad, *(None,) * 5)
+        return (grad, *(None,) * 6)
 
 
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
@@ -293,8 +293,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
         a = O.PolicyArgs(old.data_ptr(), None if ref is None else ref.data_ptr(), adv.data_ptr(), T if adv.dim() == 1 else 1, T, clip_low, clip_high,
                          kl_coef, entropy_coef, scale, O.KL[kl], O.MEAN[reduction], 0)
         if _wants(logits):
-            return PolicyLoss(*_PolicyLoss.apply(logits, targets, V, ignore_index, float(temperature), a))
-        return PolicyLoss(*_policy_forward(logits, targets, V, ignore_index, temperature, a, False)[0])
+            return PolicyLoss(*_PolicyLoss.apply(logits, targets, V, ignore_index, float(temperature), old, a))
+        return PolicyLoss(*_policy_forward(logits, targets, V, ignore_index, temperature, old, a, False)[0])
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     zero = torch.zeros((), dtype=lp.dtype, device=lp.device)
     p = lp.exp()
@@ -320,8 +320,9 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
 def _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options):
     with _on(logits):
         logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
-        logp, stats = O.token_logprobs(rows, targets)
-        return (logits, targets, stats, *O.preference_loss(logp, targets, ref, targets.shape[0] // 2, ignore_index, **options))
+        pairs, n = targets.shape[0] // 2, rows.rows
+        logp, stats = O.token_logprobs(rows, targets, 2 * pairs)      # the slopes lie behind the statistics
+        return (logits, targets, stats, *O.preference_loss(logp, targets, ref, pairs, ignore_index, stats.data_ptr() + 8 * n, **options))
 
 
 class _PreferenceLoss(torch.autograd.Function):
@@ -329,8 +330,8 @@ class _PreferenceLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, vocab, ignore_index, temperature, ref, options):
-        logits, targets, stats, loss, seq, margin, coef = _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options)
-        ctx.save_for_backward(logits, targets, stats, coef)
+        logits, targets, stats, loss, seq, margin = _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options)
+        ctx.save_for_backward(logits, targets, stats)
         ctx.cfg = (vocab, ignore_index, temperature)
         ctx.mark_non_differentiable(seq, margin)
         ctx.set_materialize_grads(False)
@@ -341,12 +342,12 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 7
-        logits, targets, stats, coef = ctx.saved_tensors
+        logits, targets, stats = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         with _on(logits):
             logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
             grad = O.empty_grad(logits)
-            O.token_logprobs_grad(rows, stats, coef, targets.shape[1], dloss.float(), grad)
+            O.token_logprobs_grad(rows, stats, stats.data_ptr() + 8 * rows.rows, targets.shape[1], dloss.float(), grad)
         return (grad, *(None,) * 6)
 
 

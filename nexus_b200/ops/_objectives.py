@@ -113,25 +113,25 @@ def empty_grad(logits: torch.Tensor) -> torch.Tensor:
     return buf.as_strided(logits.shape, logits.stride(), off)
 
 
-def token_logprobs(rows: TokenRows, like: torch.Tensor):
-    """FP32 (logp of the shape of `like` (the targets), stats [rows, 2])."""
-    dev = like.device
-    logp = torch.empty(like.shape, dtype=torch.float32, device=dev)
-    stats = torch.empty((rows.rows, 2), dtype=torch.float32, device=dev)
-    _call("nx_token_logprobs", C.byref(rows), logp.data_ptr(), stats.data_ptr(), K.status_word(dev).data_ptr())
+def token_logprobs(rows: TokenRows, like: torch.Tensor, more: int = 0):
+    """FP32 (logp of the shape of `like` (the contiguous targets), stats: two values per row, and `more` values behind them for the caller)."""
+    logp = torch.empty_like(like, dtype=torch.float32)
+    stats = torch.empty(2 * rows.rows + more, dtype=torch.float32, device=like.device)
+    _call("nx_token_logprobs", C.byref(rows), logp.data_ptr(), stats.data_ptr(), K.status_word(like.device).data_ptr())
     return logp, stats
 
 
-def token_logprobs_grad(rows: TokenRows, stats, coef, coef_per: int, factor, grad) -> None:
-    _call("nx_token_logprobs_grad", C.byref(rows), stats.data_ptr(), coef.data_ptr(), coef_per, None if factor is None else factor.data_ptr(),
+def token_logprobs_grad(rows: TokenRows, stats, coef: int, coef_per: int, factor, grad) -> None:
+    """`coef`: an address."""
+    _call("nx_token_logprobs_grad", C.byref(rows), stats.data_ptr(), coef, coef_per, None if factor is None else factor.data_ptr(),
           grad.data_ptr())
 
 
 def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad):
-    """FP32 (loss, logp, kl, entropy) of the shape of `like` (the targets); `grad` (or None) is written."""
-    n, dev, shape = rows.rows, like.device, like.shape
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    logp, kl, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
+    """FP32 (loss, logp, kl, entropy) of the shape of `like` (contiguous FP32, a value per token); `grad` (or None) is written."""
+    n, dev = rows.rows, like.device
+    loss = like.new_empty(())
+    logp, kl, entropy = torch.empty_like(like), torch.empty_like(like), torch.empty_like(like)
     scratch = torch.empty(24 + 4 * (n // args.seq_len) + 4 * n, dtype=torch.uint8, device=dev)   # totals, counts, the rows' losses
     at = scratch.data_ptr()
     args.write_grad = grad is not None
@@ -147,18 +147,15 @@ def scale_unless_one_(x: torch.Tensor, factor: torch.Tensor) -> None:
     _call("nx_scale_unless_one", x.data_ptr(), factor.data_ptr(), K._DT[x.dtype], n)
 
 
-def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, *, kind: str, average: bool, beta: float, smoothing: float,
-                    target_margin: float):
-    """FP32 (loss, logp of the sequences [2 * pairs], margin [pairs], coef [2 * pairs])."""
-    dev = logp.device
+def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, coef: int, *, kind: str, average: bool, beta: float,
+                    smoothing: float, target_margin: float):
+    """FP32 (loss, logp of the sequences [2 * pairs], margin [pairs]); the 2 * pairs slopes go to the address `coef`."""
     a = PreferenceArgs(logp.data_ptr(), targets.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(), pairs,
                        targets.numel() // (2 * pairs), ignore_index, targets.dtype == torch.int64, PREFERENCE[kind], average, beta, smoothing,
                        target_margin)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    seq_logp, coef = (torch.empty(2 * pairs, dtype=torch.float32, device=dev) for _ in range(2))
-    margin = torch.empty(pairs, dtype=torch.float32, device=dev)
-    _call("nx_preference_loss", C.byref(a), seq_logp.data_ptr(), margin.data_ptr(), coef.data_ptr(), loss.data_ptr())
-    return loss, seq_logp, margin, coef
+    loss, seq_logp, margin = logp.new_empty(()), logp.new_empty(2 * pairs), logp.new_empty(pairs)
+    _call("nx_preference_loss", C.byref(a), seq_logp.data_ptr(), margin.data_ptr(), coef, loss.data_ptr())
+    return loss, seq_logp, margin
 
 
 # ------------------------------------------------------------------------------------------- log-probabilities from hidden states
