@@ -239,7 +239,8 @@ __device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, const Pol
   PolicyRow o;
   const float ratio = expf(logp - in.old);
   const float free = ratio * in.adv, bound = fminf(fmaxf(ratio, 1.0f - g.clip_low), 1.0f + g.clip_high) * in.adv;
-  const bool follows = free <= bound;  // the unclipped term is the smaller one, or they are equal
+  // the unclipped term where it is the smaller one, or they are equal, or it is no number
+  const bool follows = !(free > bound);
   float loss = follows ? -free : -bound, c = follows ? -free : 0.0f;
   o.kl = 0.0f;
   if (g.ref_logp != nullptr) {

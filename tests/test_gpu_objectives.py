@@ -208,6 +208,14 @@ def test_nan_logits_show():
     r = F.policy_loss(x, t, torch.zeros(1, 3, device="cuda"), torch.ones(1, device="cuda"))
     assert torch.isnan(r.logp).tolist() == [[False, True, False]] and torch.isnan(r.entropy).tolist() == [[False, True, False]]
     assert torch.isnan(F.token_logprobs(x, t)).tolist() == [[False, True, False]]
+    assert math.isnan(float(r.loss)) and math.isnan(float(F.preference_loss(x.expand(2, 3, 700), t.expand(2, 3)).loss))
+    x.requires_grad_(True)
+    F.policy_loss(x, t, torch.zeros(1, 3, device="cuda"), torch.ones(1, device="cuda")).loss.backward()
+    assert bool(torch.isnan(x.grad[0, 1]).all()) and bool(torch.isfinite(x.grad[0, [0, 2]]).all())
+    y = torch.zeros(1, 3, 700, device="cuda", requires_grad=True)
+    for adv in (math.nan, math.inf):
+        loss = F.policy_loss(y, t, torch.zeros(1, 3, device="cuda"), torch.tensor([adv], device="cuda")).loss
+        assert not math.isfinite(float(loss.detach()))
 
 
 def policy_inputs(B, T, vocab, dtype, pitch=None, seed=1):
@@ -510,6 +518,40 @@ def test_other_stream_and_two_graphs():
     for out, want in zip(outs, plain):
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+def test_host_threads_on_streams_of_their_own():
+    from concurrent.futures import ThreadPoolExecutor
+    made = [policy_inputs(2, 30 + i, 3001, BF16, 3008, seed=i) for i in range(4)]
+    adv = [torch.randn(2, 30 + i, device="cuda") for i in range(4)]
+    h, w = torch.randn(300, 64, device="cuda", dtype=BF16), torch.randn(3001, 64, device="cuda", dtype=BF16)
+    tk = torch.randint(0, 3001, (300,), device="cuda")
+
+    def work(i):
+        x, t, old, ref, _ = made[i]
+        x = x.detach().requires_grad_(True)
+        r = F.policy_loss(x, t, old, adv[i], ref, kl_coef=0.1, vocab=3001)
+        (r.loss * 0.5).backward()
+        hh, ww = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        g = torch.autograd.grad(F.linear_logprobs(hh, ww, tk).sum(), (hh, ww))
+        gs = [x.grad.clone(), g[0].float()]
+        n = F.clip_grad_norm_(gs, 0.1)
+        return r.loss.detach(), x.grad, *g, n, *gs
+
+    plain = [work(i) for i in range(4)]
+    torch.cuda.synchronize()
+
+    def aside(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                out = work(i)
+        s.synchronize()
+        return out
+
+    with ThreadPoolExecutor(4) as ex:
+        for out, want in zip(ex.map(aside, range(4)), plain):
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
 def test_no_gradient_asked():
