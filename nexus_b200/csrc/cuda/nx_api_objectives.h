@@ -24,7 +24,8 @@ typedef struct NxTokenRows {
 // logp [rows] = log-probability of the target (0 where ignored); stats [rows] pairs: a logit x, and log2 of the sum of
 // exp((logit - x) * inv_temp).
 // status: device int, receives a non-zero nx::StatusCode when a wait timed out.
-int nx_token_logprobs(const NxTokenRows* rows, float* logp, float* stats, int* status, nx_stream_t stream);
+// wide [rows], may be null: logp before it is rounded to FP32.
+int nx_token_logprobs(const NxTokenRows* rows, float* logp, float* stats, double* wide, int* status, nx_stream_t stream);
 // A gradient has the layout and type of the logits and starts at the same place of a 16-byte line.
 // grad = coef (delta_target - p) * inv_temp (zeros in ignored rows and behind the vocabulary);
 // coef of row r: coef[r / coef_per] * *factor (factor: device scalar, may be null)
@@ -53,7 +54,7 @@ int nx_scale_unless_one(void* x, const float* factor, int dtype, int64_t n, nx_s
 
 enum NxPreferenceKind { NX_PREF_SIGMOID = 0, NX_PREF_HINGE = 1, NX_PREF_IPO = 2 };
 typedef struct NxPreferenceArgs {
-  const float* logp;       // [2 * pairs, seq_len] per token, chosen sequences first
+  const double* logp;      // [2 * pairs, seq_len] per token, chosen sequences first
   const void* targets;     // [2 * pairs, seq_len]
   const float* ref_logp;   // [2 * pairs], may be null
   int64_t pairs, seq_len, ignore_index;

@@ -496,6 +496,7 @@ __device__ __forceinline__ float4 join_all(float4 v, float k, RingSpace<S>* sp, 
 struct RingOut {
   float* logp;
   float2* stats;     // token log-probabilities: a logit x, log2 of the sum of exp((logit - x) inv_temp)
+  double* wide;      // and, where given, logp before it is rounded to FP32
   float* kl;
   float* entropy;
   float* row_loss;
@@ -641,8 +642,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         if (rank == 0 && tid == 0) {
           const float v = tg == -1 ? 0.0f : NAN;
           o.logp[row] = v;
-          if (kPolicy) o.kl[row] = o.entropy[row] = o.row_loss[row] = v;
-          else o.stats[row] = make_float2(0.0f, 0.0f);
+          if constexpr (kPolicy) {
+            o.kl[row] = o.entropy[row] = o.row_loss[row] = v;
+          } else {
+            o.stats[row] = make_float2(0.0f, 0.0f);
+            if (o.wide != nullptr) o.wide[row] = v;
+          }
         }
         if (second) {
           T* gr = grad + at;
@@ -715,6 +720,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
           if (rank == 0 && lane == 0) {
             o.logp[row] = lp;
             o.stats[row] = make_float2(careful ? v.x : xt, log2_s - (careful ? 0.0f : coarse));
+            if (o.wide != nullptr)
+              o.wide[row] = (careful ? (static_cast<double>(xt) - v.x) * a.inv_temp : coarse * 0.6931471805599453) - log(static_cast<double>(v.y));
           }
         } else {
           const float ent = careful ? ln_s - v.z / v.y * a.inv_temp : ln_s - v.z / v.y * kLn2;
@@ -947,7 +954,8 @@ __global__ void __launch_bounds__(256) scale_unless_one_kernel(T* __restrict__ x
 }
 
 // ------------------------------------------------------------------------------------------------ preference loss
-// A pair's sums in FP64 by a block (long sequences) or a warp; ln(1 + e^-|z|) and the sigmoid from one exponential.
+// A pair's sums in FP64, of log-probabilities in FP64 (the margin is a difference of sums that are near each other), by a block (long sequences)
+// or a warp; ln(1 + e^-|z|) and the sigmoid from one exponential.
 __global__ void __cluster_dims__(kJoinBlocks, 1, 1) __launch_bounds__(kJoinThreads)
 preference_kernel(const NxPreferenceArgs a, float* __restrict__ seq_logp, float* __restrict__ margin, float* __restrict__ coef,
                   float* __restrict__ loss) {
@@ -1046,12 +1054,15 @@ bool same_lines(const void* a, const void* b) { return ((reinterpret_cast<uintpt
       return -1;                             \
   }
 
-extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats, int* status, nx_stream_t stream) {
-  if (!rows_ok(a) || logp == nullptr || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 7) != 0 || status == nullptr) return -1;
+extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats, double* wide, int* status, nx_stream_t stream) {
+  if (!rows_ok(a) || logp == nullptr || stats == nullptr || ((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(wide)) & 7) != 0 ||
+      status == nullptr)
+    return -1;
   if (a->rows == 0) return 0;
   RingOut o{};
   o.logp = logp;
   o.stats = reinterpret_cast<float2*>(stats);
+  o.wide = wide;
   o.status = status;
   NX_BY_TYPE(a->dtype, return launch_ring<T, false>(*a, NxPolicyArgs{}, o, nullptr, static_cast<cudaStream_t>(stream)))
 }

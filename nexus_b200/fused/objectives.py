@@ -320,9 +320,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
 def _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options):
     with _on(logits):
         logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
-        pairs, n = targets.shape[0] // 2, rows.rows
-        logp, stats = O.token_logprobs(rows, targets, 2 * pairs)      # the slopes lie behind the statistics
-        return (logits, targets, stats, *O.preference_loss(logp, targets, ref, pairs, ignore_index, stats.data_ptr() + 8 * n, **options))
+        return (logits, targets, *O.preference_loss(rows, targets, ref, targets.shape[0] // 2, ignore_index, **options))
 
 
 class _PreferenceLoss(torch.autograd.Function):
@@ -330,8 +328,8 @@ class _PreferenceLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, vocab, ignore_index, temperature, ref, options):
-        logits, targets, stats, loss, seq, margin = _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options)
-        ctx.save_for_backward(logits, targets, stats)
+        logits, targets, loss, seq, margin, kept = _preference_forward(logits, targets, vocab, ignore_index, temperature, ref, options)
+        ctx.save_for_backward(logits, targets, kept)
         ctx.cfg = (vocab, ignore_index, temperature)
         ctx.mark_non_differentiable(seq, margin)
         ctx.set_materialize_grads(False)
@@ -342,12 +340,12 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 7
-        logits, targets, stats = ctx.saved_tensors
+        logits, targets, kept = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         with _on(logits):
             logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
             grad = O.empty_grad(logits)
-            O.token_logprobs_grad(rows, stats, stats.data_ptr() + 8 * rows.rows, targets.shape[1], dloss.float(), grad)
+            O.token_logprobs_grad(rows, kept, kept.data_ptr() + 8 * rows.rows, targets.shape[1], dloss.float(), grad)
         return (grad, *(None,) * 6)
 
 
@@ -379,7 +377,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optio
         options = dict(kind=kind, average=bool(average), beta=beta, smoothing=label_smoothing, target_margin=target_margin)
         if _wants(logits):
             return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, V, ignore_index, float(temperature), ref, options))
-        return PreferenceLoss(*_preference_forward(logits, targets, V, ignore_index, temperature, ref, options)[3:6])
+        return PreferenceLoss(*_preference_forward(logits, targets, V, ignore_index, temperature, ref, options)[2:5])
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     seq = logp.double().view(targets.shape).sum(-1)
     if average:

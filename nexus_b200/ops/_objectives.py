@@ -16,7 +16,7 @@ _functions = {}
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the current stream's handle, without an object around it
 _P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 _SIGNATURES = {
-    "nx_token_logprobs": [_P, _P, _P, _P, _P],
+    "nx_token_logprobs": [_P, _P, _P, _P, _P, _P],
     "nx_token_logprobs_grad": [_P, _P, _P, _L, _P, _P, _P],
     "nx_policy_loss": [_P] * 11 + [_P],
     "nx_scale_unless_one": [_P, _P, _I, _L, _P],
@@ -113,11 +113,11 @@ def empty_grad(logits: torch.Tensor) -> torch.Tensor:
     return buf.as_strided(logits.shape, logits.stride(), off)
 
 
-def token_logprobs(rows: TokenRows, like: torch.Tensor, more: int = 0):
-    """FP32 (logp of the shape of `like` (the contiguous targets), stats: two values per row, and `more` values behind them for the caller)."""
+def token_logprobs(rows: TokenRows, like: torch.Tensor):
+    """FP32 (logp of the shape of `like` (the contiguous targets), stats: two values per row)."""
     logp = torch.empty_like(like, dtype=torch.float32)
-    stats = torch.empty(2 * rows.rows + more, dtype=torch.float32, device=like.device)
-    _call("nx_token_logprobs", C.byref(rows), logp.data_ptr(), stats.data_ptr(), K.status_word(like.device).data_ptr())
+    stats = torch.empty(2 * rows.rows, dtype=torch.float32, device=like.device)
+    _call("nx_token_logprobs", C.byref(rows), logp.data_ptr(), stats.data_ptr(), None, K.status_word(like.device).data_ptr())
     return logp, stats
 
 
@@ -147,15 +147,20 @@ def scale_unless_one_(x: torch.Tensor, factor: torch.Tensor) -> None:
     _call("nx_scale_unless_one", x.data_ptr(), factor.data_ptr(), K._DT[x.dtype], n)
 
 
-def preference_loss(logp, targets, ref_logp, pairs: int, ignore_index: int, coef: int, *, kind: str, average: bool, beta: float,
+def preference_loss(rows: TokenRows, targets, ref_logp, pairs: int, ignore_index: int, *, kind: str, average: bool, beta: float,
                     smoothing: float, target_margin: float):
-    """FP32 (loss, logp of the sequences [2 * pairs], margin [pairs]); the 2 * pairs slopes go to the address `coef`."""
-    a = PreferenceArgs(logp.data_ptr(), targets.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(), pairs,
-                       targets.numel() // (2 * pairs), ignore_index, targets.dtype == torch.int64, PREFERENCE[kind], average, beta, smoothing,
-                       target_margin)
-    loss, seq_logp, margin = logp.new_empty(()), logp.new_empty(2 * pairs), logp.new_empty(pairs)
-    _call("nx_preference_loss", C.byref(a), seq_logp.data_ptr(), margin.data_ptr(), coef, loss.data_ptr())
-    return loss, seq_logp, margin
+    """FP32 (loss, logp of the sequences [2 * pairs], margin [pairs]), and what the gradient needs: two values per row, behind them a slope per
+    sequence."""
+    n, dev = rows.rows, targets.device
+    kept = torch.empty(2 * n + 2 * pairs, dtype=torch.float32, device=dev)
+    loss, seq_logp, margin = kept.new_empty(()), kept.new_empty(2 * pairs), kept.new_empty(pairs)
+    scratch = torch.empty(12 * n, dtype=torch.uint8, device=dev)        # log-probabilities in FP64 and in FP32
+    wide, at = scratch.data_ptr(), kept.data_ptr()
+    _call("nx_token_logprobs", C.byref(rows), wide + 8 * n, at, wide, K.status_word(dev).data_ptr())
+    a = PreferenceArgs(wide, targets.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(), pairs, n // (2 * pairs), ignore_index,
+                       targets.dtype == torch.int64, PREFERENCE[kind], average, beta, smoothing, target_margin)
+    _call("nx_preference_loss", C.byref(a), seq_logp.data_ptr(), margin.data_ptr(), at + 8 * n, loss.data_ptr())
+    return loss, seq_logp, margin, kept
 
 
 # ------------------------------------------------------------------------------------------- log-probabilities from hidden states
