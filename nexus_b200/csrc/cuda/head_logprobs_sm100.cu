@@ -1190,7 +1190,7 @@ extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* tlogit,
 }
 
 extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, nx_stream_t stream) {
-  if (!args_ok(a) || g == nullptr || g->coef == nullptr || g->logit_grad == nullptr || g->chunk < kTile || g->chunk % kTile != 0 ||
+  if (!args_ok(a) || a->index == nullptr || g == nullptr || g->coef == nullptr || g->logit_grad == nullptr || g->chunk < kTile || g->chunk % kTile != 0 ||
       g->ld_logit_grad < a->vocab || g->ld_logit_grad % 64 != 0 || (reinterpret_cast<uintptr_t>(g->logit_grad) & 15) != 0 ||
       (a->dtype == NX_F16 && g->scale == nullptr) || g->slices < 1 || (g->slices > 1 && g->slice_sums == nullptr) ||
       (reinterpret_cast<uintptr_t>(g->d_hidden) & 15) != 0 || (reinterpret_cast<uintptr_t>(g->d_weight) & 15) != 0 ||
@@ -1201,9 +1201,9 @@ extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, n
   int rc;
   const bool half = a->dtype == NX_F16;
   if (half) NX_PDL(coef_scale_kernel, 1, 1024, 0, st, g->coef, a->targets, a->targets_wide, a->ignore_index, a->rows, a->inv_temp, g->scale);
-  if (a->index != nullptr && (rc = gather(a, st)) != 0) return rc;
-  const void* h = a->index != nullptr ? a->gathered : a->hidden;
-  const int64_t ldh = a->index != nullptr ? a->width : a->ld_hidden;
+  if (a->weights == nullptr && (rc = gather(a, st)) != 0) return rc;
+  const void* h = a->gathered;
+  const int64_t ldh = a->width;
   if (g->d_hidden != nullptr)
     NX_PDL(clear_rows_kernel, static_cast<unsigned>(std::min<int64_t>(a->rows, kNumSmsB200 * 16)), 128, 0, st, a->targets, a->targets_wide, a->rows,
            a->ignore_index, a->vocab, reinterpret_cast<uint4*>(g->d_hidden), static_cast<int64_t>(a->width / 8), a->width / 8);

@@ -171,21 +171,21 @@ class _LinearLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, vocab, ignore_index, temperature, recompute):
-        t, logp, stats, index, part, weights = _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, True, recompute)
-        ctx.save_for_backward(hidden, weight, t, stats, index, part, weights)
+        t, logp, block, weights = _linear_forward(hidden, weight, targets, vocab, ignore_index, temperature, True, recompute)
+        ctx.save_for_backward(hidden, weight, t, block, weights)
         ctx.cfg = (vocab, ignore_index, temperature)
         return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
-        hidden, weight, t, stats, index, part, weights = ctx.saved_tensors
+        hidden, weight, t, block, weights = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         again = torch._C._autograd._get_current_graph_task_keep_graph()
         with _on(hidden):
             h, w = O.head_rows(hidden.reshape(-1, hidden.shape[-1])), O.head_rows(weight)
-            dh, dw = O.head_logprobs_grad(h, w, t, vocab, ignore_index, 1.0 / temperature, stats, index, part, weights,
-                                          dlogp.float().contiguous(), ctx.needs_input_grad[0], ctx.needs_input_grad[1], again)
+            dh, dw = O.head_logprobs_grad(h, w, t, vocab, ignore_index, 1.0 / temperature, block, weights, dlogp.float().contiguous(),
+                                          ctx.needs_input_grad[0], ctx.needs_input_grad[1], again)
         return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None, None
 
 

@@ -195,53 +195,67 @@ def head_rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _head_args(hidden, weight, targets, index, moved, stats: int, part: int, weights, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
+def _head_args(hidden, weight, targets, index, moved, stats: int, part, weights, vocab: int, ignore_index: int, inv_temp: float) -> HeadArgs:
+    """`index` (the rows that count and behind them their number), `moved`, `stats`, `part`: addresses."""
     rows, width = hidden.shape
-    at = (None, None, None) if index is None else (index.data_ptr(), index.data_ptr() + 4 * rows, moved.data_ptr())
     held, ld = (None, 0) if weights is None else (weights.data_ptr(), weights.stride(0))
-    return HeadArgs(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), *at, stats, part, held, K.status_word(hidden.device).data_ptr(),
-                    _part_rows(rows), ld, rows, hidden.stride(0), weight.stride(0), ignore_index, vocab, width, K._DT[hidden.dtype], targets.dtype == torch.int64,
-                    inv_temp, 0)
+    return HeadArgs(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), index, None if index is None else index + 4 * rows, moved, stats, part,
+                    held, K.status_word(hidden.device).data_ptr(), _part_rows(rows), ld, rows, hidden.stride(0), weight.stride(0), ignore_index,
+                    vocab, width, K._DT[hidden.dtype], targets.dtype == torch.int64, inv_temp, 0)
 
 
 def _part_rows(rows: int) -> int:
     return min(HEAD_ROWS, -(-rows // HEAD_TILE) * HEAD_TILE)
 
 
-def _gathered(hidden) -> torch.Tensor:
-    return torch.empty(((hidden.shape[0] + 63) // 64 * 64, hidden.shape[1]), dtype=hidden.dtype, device=hidden.device)
-
-
 def _head_pitch(vocab: int) -> int:
     return (vocab + 63) // 64 * 64
 
 
+class _Block:
+    """Places of a scratch block: 256-byte boundaries, handed out before the block is allocated."""
+
+    def __init__(self):
+        self.size = 0
+
+    def take(self, nbytes: int) -> int:
+        at, self.size = self.size, self.size + (nbytes + 255) // 256 * 256
+        return at
+
+    def allocate(self, device) -> torch.Tensor:
+        return torch.empty(self.size, dtype=torch.uint8, device=device)
+
+
 def head_logprobs(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, want_grad: bool, recompute: bool = False):
     """FP32 logp (of the shape of `targets`) for hidden [rows, width] and weight [>= vocab, width] (`head_rows` of both), and what the gradient
-    needs (all None where it is not wanted): stats, index of the rows that count, with their number behind it, and the column tiles' maxima and
-    the logits' exponentials where these are held."""
-    rows, dev = hidden.shape[0], hidden.device
-    logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-    parts = 2 * HEAD_PARTS * -(-vocab // HEAD_TILE) * _part_rows(rows)
-    if not want_grad:    # one block of scratch: column tiles and statistics (pairs), targets' logits
-        scratch = torch.empty(parts + 3 * rows, dtype=torch.float32, device=dev)
-        at = scratch.data_ptr()
-        index = torch.empty(rows + 1, dtype=torch.int32, device=dev) if rows > HEAD_TILE else None
-        moved = None if index is None else _gathered(hidden)
-        a = _head_args(hidden, weight, targets, index, moved, at + 4 * parts, at, None, vocab, ignore_index, inv_temp)
-        _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), at + 4 * (parts + 2 * rows))
-        return logp, None, None, None, None
-    index = torch.empty(rows + 1, dtype=torch.int32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    part = torch.empty(parts, dtype=torch.float32, device=dev)
-    tlogit = torch.empty(rows, dtype=torch.float32, device=dev)
+    needs, None where it is not wanted: a block with the statistics and the rows that count, and the logits' exponentials where these are held
+    (the block then has their column tiles' maxima and the gathered rows too)."""
+    rows, width = hidden.shape
+    dev = hidden.device
+    logp = torch.empty_like(targets, dtype=torch.float32)
     full, ld = -(-rows // HEAD_TILE) * HEAD_TILE, _head_pitch(vocab)
-    keep = not recompute and rows <= HEAD_ROWS and hidden.shape[1] >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
+    keep = want_grad and not recompute and rows <= HEAD_ROWS and width >= HEAD_KEEP_WIDTH and full * ld <= HEAD_GRAD_ELEMENTS
+    parts, gathered = 8 * HEAD_PARTS * -(-vocab // HEAD_TILE) * _part_rows(rows), (rows + 63) // 64 * 64 * width * 2
+    kept, scratch = _Block(), _Block()
+    stats = kept.take(8 * rows)
+    index = kept.take(4 * rows + 4) if want_grad or rows > HEAD_TILE else None
+    part = (kept if keep else scratch).take(parts)
+    moved = None if index is None else (kept if keep else scratch).take(gathered)
+    tlogit = scratch.take(4 * rows)
+    if not want_grad:                     # one block
+        shift = scratch.take(kept.size)
+        block = scratch.allocate(dev)
+        at = block.data_ptr()
+        base = at + shift
+    else:
+        block, rest = kept.allocate(dev), scratch.allocate(dev)
+        base, at = block.data_ptr(), rest.data_ptr()
+    other = base if keep else at
     weights = torch.empty((full, ld), dtype=hidden.dtype, device=dev) if keep else None
-    moved = _gathered(hidden)
-    a = _head_args(hidden, weight, targets, index, moved, stats.data_ptr(), part.data_ptr(), weights, vocab, ignore_index, inv_temp)
-    _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), tlogit.data_ptr())
-    return logp, stats, index, (part if keep else None), weights
+    a = _head_args(hidden, weight, targets, None if index is None else base + index, None if moved is None else other + moved, base + stats,
+                   other + part, weights, vocab, ignore_index, inv_temp)
+    _call("nx_head_logprobs", C.byref(a), logp.data_ptr(), at + tlogit)
+    return logp, (block if want_grad else None), weights
 
 
 def head_slices(rows: int, width: int) -> int:
@@ -253,34 +267,38 @@ def head_slices(rows: int, width: int) -> int:
     return max(1, min(16, (1 << 25) // (-(-rows // HEAD_TILE) * HEAD_TILE * width)))
 
 
-def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, stats, index, part, weights, coef,
-                       want_hidden: bool, want_weight: bool, again: bool = False):
+def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, inv_temp: float, block, weights, coef, want_hidden: bool,
+                       want_weight: bool, again: bool = False):
     """(d_hidden [rows, width], d_weight [all rows of weight, width]), either None where not wanted.  The exponentials become the gradient of the
     logits in place, unless they are needed `again`."""
     rows, width = hidden.shape
     dev, dtype = hidden.device, hidden.dtype
-    moved = _gathered(hidden)
-    a = _head_args(hidden, weight, targets, index, moved, stats.data_ptr(), None if part is None else part.data_ptr(), weights, vocab, ignore_index,
-                   inv_temp)
-    g = HeadGrad()
-    ld = _head_pitch(vocab)
-    chunk = -(-rows // HEAD_TILE) * HEAD_TILE
+    kept, scratch = _Block(), _Block()
+    stats, index = kept.take(8 * rows), kept.take(4 * rows + 4)
+    parts, gathered = 8 * HEAD_PARTS * -(-vocab // HEAD_TILE) * _part_rows(rows), (rows + 63) // 64 * 64 * width * 2
+    base, ld, chunk = block.data_ptr(), _head_pitch(vocab), -(-rows // HEAD_TILE) * HEAD_TILE
     if weights is not None:
-        logit_grad = torch.empty_like(weights) if again else weights
+        part, moved = base + kept.take(parts), base + kept.take(gathered)
+        grad_at = scratch.take(2 * chunk * ld) if again else None
     else:
         chunk = min(chunk, max(HEAD_TILE, HEAD_GRAD_ELEMENTS // ld // HEAD_TILE * HEAD_TILE))
-        logit_grad = torch.empty((chunk, ld), dtype=dtype, device=dev)
-    scale = torch.empty(2, dtype=torch.float32, device=dev)
-    g.coef, g.logit_grad, g.chunk, g.ld_logit_grad, g.scale = coef.data_ptr(), logit_grad.data_ptr(), chunk, ld, scale.data_ptr()
+        part, moved, grad_at = None, scratch.take(gathered), scratch.take(2 * chunk * ld)
+    scale = scratch.take(8)
+    slices = head_slices(min(rows, chunk), width) if want_hidden else 1
+    slice_sums = scratch.take(4 * slices * chunk * width) if slices > 1 else None
+    weight_sums = scratch.take(4 * vocab * width) if want_weight and chunk < rows else None
+    rest = scratch.allocate(dev)
+    at = rest.data_ptr()
+    if weights is None:
+        moved += at
     dh = torch.empty((rows, width), dtype=dtype, device=dev) if want_hidden else None
     dw = torch.empty((weight.shape[0], width), dtype=dtype, device=dev) if want_weight else None
     if want_weight and weight.shape[0] > vocab:
         dw[vocab:].zero_()
-    g.slices = head_slices(min(rows, chunk), width) if want_hidden else 1
-    slice_sums = torch.empty((g.slices, chunk, width), dtype=torch.float32, device=dev) if g.slices > 1 else None
-    weight_sums = torch.empty((vocab, width), dtype=torch.float32, device=dev) if want_weight and chunk < rows else None
-    for name, t in (("d_hidden", dh), ("d_weight", dw), ("slice_sums", slice_sums), ("weight_sums", weight_sums)):
-        setattr(g, name, None if t is None else t.data_ptr())
+    a = _head_args(hidden, weight, targets, base + index, moved, base + stats, part, weights, vocab, ignore_index, inv_temp)
+    g = HeadGrad(coef.data_ptr(), weights.data_ptr() if grad_at is None else at + grad_at, chunk, ld, at + scale, None if dh is None else dh.data_ptr(),
+                 None if dw is None else dw.data_ptr(), None if slice_sums is None else at + slice_sums,
+                 None if weight_sums is None else at + weight_sums, slices, 0)
     _call("nx_head_logprobs_grad", C.byref(a), C.byref(g))
     return dh, dw
 
