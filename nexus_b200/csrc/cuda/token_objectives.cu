@@ -296,9 +296,11 @@ using LongShape = Shape<512, 13, 1>;
 // base is the same for every thread and block, so joining is adding and no maximum is kept; the product is inside the fused multiply-add, so t
 // is exact to its own last bit, and results are taken relative to B itself.  The target's own term makes s at least 1.  A row where a logit lies
 // so far above its target's that the sums overflow (t of 120 and more), or where B would be too coarse (|x_t| above kFastLimit, -inf, NaN), is
-// done again in the form with running maxima and the difference first.
+// done again in the form with running maxima and the difference first; and so is, where t is multiplied, one where the finite value that stands
+// for -inf (an FP16 piece holds none below -65504) comes so near the target's logit, or is scaled down so far, that its weight is not zero.
 constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f;
 constexpr float kFloor = -1.0e30f;  // stands for -inf where t is multiplied: the weight is zero either way, and zero times it is zero
+constexpr float kNoWeight = -160.0f;  // 2^t is zero
 
 struct Pair {
   uint64_t v;
@@ -331,6 +333,7 @@ struct PieceOf;
 template <>
 struct PieceOf<__nv_bfloat16> {
   static constexpr int kPairs = 4;
+  static constexpr float kLowest = kFloor;
   template <bool kFloored>
   static __device__ __forceinline__ void get(const uint4& q, Pair (&p)[4]) {
     uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -344,6 +347,7 @@ struct PieceOf<__nv_bfloat16> {
 template <>
 struct PieceOf<__half> {
   static constexpr int kPairs = 4;
+  static constexpr float kLowest = -65504.0f;
   template <bool kFloored>
   static __device__ __forceinline__ void get(const uint4& q, Pair (&p)[4]) {
     uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -358,6 +362,7 @@ struct PieceOf<__half> {
 template <>
 struct PieceOf<float> {
   static constexpr int kPairs = 2;
+  static constexpr float kLowest = kFloor;
   template <bool kFloored>
   static __device__ __forceinline__ void get(const uint4& q, Pair (&p)[2]) {
     float v[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
@@ -745,7 +750,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         }
       };
       if (warp == 0) {
-        const bool careful = !(fabsf(xt) <= kFastLimit && st.y <= kFastSum);
+        const bool careful = !(fabsf(xt) <= kFastLimit && st.y <= kFastSum && (!kPolicy || fmaf(PieceOf<T>::kLowest, k, -base) <= kNoWeight));
         if (!careful) end_row(st, false);
         else if (lane == 0) sp->end.careful = 1;
         if (!kPolicy && !careful && lane == 0) sp->end.careful = 0;

@@ -62,8 +62,8 @@ def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature:
 
 
 def _check_temperature(name: str, temperature: float) -> None:
-    if not 0.0 < temperature < math.inf:
-        raise ValueError(f"{name}: temperature must be positive, got {temperature}")
+    if not 1e-8 <= temperature <= 1e8:     # its inverse times a logit is an FP32 number, and -inf stays far below every logit
+        raise ValueError(f"{name}: temperature must be between 1e-8 and 1e8, got {temperature}")
 
 
 def _check_values(name: str, what: str, t, shapes, device) -> torch.Tensor:

@@ -184,6 +184,39 @@ def test_masked_vocabulary(dtype):
         close(x.grad, gw, grad_error(gw, p, size, dtype, vocab, coef_rel=64 * U) + {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: U}[dtype] * gw.abs())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("temperature", [1.0, 2.0 ** 14, 1.0e8])
+@pytest.mark.parametrize("ent", [0.0, 0.05])
+def test_masks_beside_the_lowest_value_and_at_high_temperatures(dtype, temperature, ent):
+    """-inf has no weight where the target itself holds the type's lowest value (or lies next to it), nor where a high temperature brings all
+    finite logits together."""
+    vocab, low = 2000, torch.finfo(dtype).min
+    x, t, _ = make((1, 4), vocab, dtype, seed=4)
+    x[0, 0] = -math.inf
+    x[0, 0, [3, 50, 700, 1999]] = low
+    x[0, 1] = -math.inf
+    x[0, 1, [3, 50]] = torch.tensor([-65472.0, -65504.0], dtype=dtype, device="cuda")
+    x[0, 2, ::2] = -math.inf
+    x[0, 3, 1:] = -math.inf
+    t[0] = torch.tensor([700, 3, 7, 0])
+    lp = softmax64(x, vocab, temperature)
+    p = lp.exp()
+    want = lp.gather(2, t[..., None])[..., 0]
+    H = -torch.where(p > 0, p * lp.clamp(min=-1e30), 0.0).sum(-1)
+    x.requires_grad_(True)
+    r = F.policy_loss(x, t, want.float(), torch.ones(1, 4, device="cuda"), entropy_coef=ent, reduction="sum", temperature=temperature)
+    r.loss.backward()
+    close(r.logp, want, logp_error(want, vocab))
+    close(F.token_logprobs(x.detach(), t, temperature=temperature), want, logp_error(want, vocab))
+    close(r.entropy, H, U * (8 * H + 40 + chain(vocab)))
+    delta = torch.nn.functional.one_hot(t, vocab).double()
+    gw = (-(delta - p) + ent * torch.where(p > 0, p * (lp.clamp(min=-1e30) + H[..., None]), 0.0)) / temperature
+    assert bool((x.grad[torch.isinf(x.detach())] == 0).all())
+    size = (1.0 + ent * (H[..., None] + 20.0)) / temperature
+    step = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: U}[dtype]
+    close(x.grad, gw, grad_error(gw, p, size, dtype, vocab, coef_rel=64 * U) + step * gw.abs())
+
+
 def test_ignored_rows_are_not_read_and_bad_targets_are_nan():
     x, t, _ = make((2, 3), 64, F32)
     x[0, 0] = math.nan

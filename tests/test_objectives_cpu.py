@@ -74,6 +74,18 @@ def test_refusals():
             call()
 
 
+def test_refuses_temperatures_whose_inverse_is_no_scale():
+    x, t, old, _, adv = inputs()
+    h, w = torch.randn(*t.shape, 16), torch.randn(x.shape[-1], 16)
+    for temperature in (1e-45, 9e-9, 1.1e8, 1e39, math.nan):
+        for call in (lambda: F.token_logprobs(x, t, temperature=temperature), lambda: F.linear_logprobs(h, w, t, temperature=temperature),
+                     lambda: F.policy_loss(x, t, old, adv, temperature=temperature), lambda: F.preference_loss(x, t, temperature=temperature)):
+            with pytest.raises(ValueError, match="temperature"):
+                call()
+    for temperature in (1e-8, 1e8):
+        assert bool(torch.isfinite(F.token_logprobs(x, t, temperature=temperature)).all())
+
+
 def test_row_layouts():
     """The rows of these views are read where they are; the others are copied first."""
     from nexus_b200.ops._objectives import row_layout
