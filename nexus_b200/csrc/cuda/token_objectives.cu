@@ -44,17 +44,18 @@ struct RowSplit {
   }
 };
 
-// Running maximum, sum of exponentials and, where asked for, sum of exponentials times differences, of one thread's elements.
-template <bool kEntropy>
+constexpr float kFarBelow = -1.0e30f;  // stands for a difference of -inf where a weight of zero multiplies it
+
+// Running maximum, sum of exponentials and sum of exponentials times differences, of one thread's elements.
 struct Online {
   float m = -INFINITY, s = 0.0f, h = 0.0f;
   __device__ __forceinline__ void raise(float to, float k) {  // a larger maximum: the sums so far are taken down to it
     const float old = m;
     m = to;
     if (old == -INFINITY) return;  // nothing but -inf so far: the sums are zero (or NaN) as they are
-    const float d = fmaxf(old - to, -1e30f);  // finite beside a masked lowest value, so that its weight of zero makes it zero
+    const float d = fmaxf(old - to, kFarBelow);  // finite beside a masked lowest value, so that its weight of zero makes it zero
     const float f = ex2_approx(d * k);
-    if (kEntropy) h = (h + d * s) * f;
+    h = (h + d * s) * f;
     s *= f;
   }
   template <int N>
@@ -68,10 +69,10 @@ struct Online {
     for (int j = 0; j < N; ++j) {
       float d = v[j] - base;
       // a masked -inf has the weight 0 and must not make 0 * -inf of it; NaN stays NaN
-      if (kEntropy) asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(-1e30f));
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(kFarBelow));
       const float e = ex2_approx(d * k);
       s += e;
-      if (kEntropy) h = fmaf(e, d, h);
+      h = fmaf(e, d, h);
     }
   }
 };
@@ -299,7 +300,9 @@ using LongShape = Shape<512, 13, 1>;
 // done again in the form with running maxima and the difference first; and so is, where t is multiplied, one where the finite value that stands
 // for -inf (an FP16 piece holds none below -65504) comes so near the target's logit, or is scaled down so far, that its weight is not zero.
 constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f;
-constexpr float kFloor = -1.0e30f;  // stands for -inf where t is multiplied: the weight is zero either way, and zero times it is zero
+// Stands for -inf (and all below it) where t is multiplied: the weight is zero either way, and zero times a finite product is zero.  Representable in
+// BF16; no lower than it must be, so that k (up to 1.5e8) and the entropy's factors keep the products finite.
+constexpr float kFloor = -998244352.0f;
 constexpr float kNoWeight = -160.0f;  // 2^t is zero
 
 struct Pair {
@@ -339,7 +342,7 @@ struct PieceOf<__nv_bfloat16> {
     uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (kFloored) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xf149f149u));  // -1e30
+      if (kFloored) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0xce6ece6eu));  // kFloor
       p[i] = pair_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
   }
@@ -434,7 +437,7 @@ __device__ __forceinline__ void workers_sync() {
 // s and h are relative to a maximum m: brings them to `top`, differences in units of the logits
 __device__ __forceinline__ void weigh(float4& v, float top, float k) {
   if (v.x == -INFINITY) return;  // nothing but -inf: zero (or NaN) as it is
-  const float d = fmaxf(v.x - top, kFloor), f = ex2_approx(d * k);
+  const float d = fmaxf(v.x - top, kFarBelow), f = ex2_approx(d * k);
   v.z = fmaf(d, v.y, v.z) * f;
   v.y *= f;
 }
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
       }
       workers_sync<S>();
       if (sp->end.careful) {  // the same in every block of the cluster; from memory, with maxima and the difference first
-        Online<true> on2;
+        Online on2;
         const T* body = p + r.head + static_cast<int64_t>(lo) * VN;
         for (int i = tid; i < n; i += kWorkers) {
           float v[VN];
@@ -777,9 +780,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         T* gr = grad + at;
         const int col0 = r.head + lo * VN;
         if (e.careful) {
+          const float least = 2.0f * kNoWeight / k;  // no weight from here on (log2_s is not negative), and small enough to be multiplied
           auto one = [&](float v) {
             float d = v - e.m;
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(kFloor));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(least));
             return ex2_approx(fmaf(d, k, -e.log2_s)) * (g.entropy_coef != 0.0f ? fmaf(d, e.slope, e.off) : e.off);
           };
           for (int i = tid; i < n; i += kWorkers) {

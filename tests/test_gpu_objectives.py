@@ -430,6 +430,33 @@ def test_policy_gradient_of_a_scaled_loss():
         torch.autograd.grad(torch.autograd.grad(call(), x, create_graph=True)[0].sum(), x)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("temperature", [1e-8, 1e-4, 1e4, 1e8])
+def test_entropy_gradient_of_masked_rows_at_extreme_temperatures(dtype, temperature):
+    """Entries of -inf have no gradient, and the others a finite one, at both ends of the temperatures that are allowed."""
+    vocab = 700
+    x, t, _ = make((2, 3), vocab, dtype, seed=8)
+    x[0, :, 1::2] = -math.inf
+    x[1, :, 1::2] = torch.finfo(dtype).min
+    x[1, 1, 2] = -math.inf
+    t -= t % 2
+    t[1, 1] = 4
+    x.requires_grad_(True)
+    r = F.policy_loss(x, t, torch.zeros(2, 3, device="cuda"), torch.zeros(2, device="cuda"), entropy_coef=0.05, reduction="sum", temperature=temperature)
+    r.loss.backward()
+    lp = softmax64(x, vocab, temperature)
+    p = lp.exp()
+    H = -torch.where(p > 0, p * lp.clamp(min=-1e30), 0.0).sum(-1, keepdim=True)
+    gw = 0.05 / temperature * torch.where(p > 0, p * (lp.clamp(min=-1e30) + H), 0.0)
+    assert bool(torch.isfinite(x.grad).all())
+    assert bool((x.grad[torch.isinf(x.detach())] == 0).all())
+    if dtype != F16 or temperature >= 1e4:     # elsewhere FP16 cannot hold an element of the gradient
+        # t = (x - x0) k is off by two roundings of itself (z in `grad_error`), and log p + H by as much, absolutely: 20 covers both below
+        size = 0.05 / temperature * (H + 20.0)
+        step = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: U}[dtype]
+        close(x.grad, gw, grad_error(gw, p, size, dtype, vocab, coef_rel=64 * U) + step * gw.abs())
+
+
 @pytest.mark.parametrize("B,T", [(1, 1), (1, 300), (300, 1), (40, 7)])
 @pytest.mark.parametrize("reduction", ["token", "sequence"])
 def test_policy_shapes(B, T, reduction):
