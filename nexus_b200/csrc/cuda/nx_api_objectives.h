@@ -44,12 +44,18 @@ typedef struct NxPolicyArgs {
   int32_t kl, mean;
   int32_t write_grad;
 } NxPolicyArgs;
+// What a row's gradient is made of: p_j (slope (logit_j - x) + off) with p_j = 2^((logit_j - x) inv_temp log2 e - log2_s), and c more at the target.
+typedef struct NxPolicySlope {
+  float x, log2_s, c, slope, off;
+} NxPolicySlope;
 // Clipped policy loss with KL and entropy terms.  logp, kl, entropy, row_loss: [rows]; totals: three doubles, counts: [rows / seq_len],
 // both scratch; loss: one float; at least one row;
-// grad (write_grad): d loss / d logits in the layout and type of the logits.
+// grad (write_grad; BF16, FP32): d loss / d logits in the layout and type of the logits; slopes [rows], may be null: for nx_policy_loss_grad.
 int nx_policy_loss(const NxTokenRows* rows, const NxPolicyArgs* args, double* totals, int32_t* counts, float* logp, float* kl, float* entropy,
-                   float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream);
-// x *= *factor in place, n elements; nothing is read or written where the factor is 1
+                   float* row_loss, float* loss, void* grad, NxPolicySlope* slopes, int* status, nx_stream_t stream);
+// grad = *factor (device scalar) * d loss / d logits, FP16 logits only: a loss scale has to be in the gradient before it is rounded
+int nx_policy_loss_grad(const NxTokenRows* rows, const NxPolicySlope* slopes, const float* factor, void* grad, nx_stream_t stream);
+// x *= *factor in place, n elements (BF16, FP32); nothing is read or written where the factor is 1
 int nx_scale_unless_one(void* x, const float* factor, int dtype, int64_t n, nx_stream_t stream);
 
 enum NxPreferenceKind { NX_PREF_SIGMOID = 0, NX_PREF_HINGE = 1, NX_PREF_IPO = 2 };

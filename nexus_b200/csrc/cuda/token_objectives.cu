@@ -44,6 +44,7 @@ struct RowSplit {
   }
 };
 
+constexpr float kNoWeight = -160.0f;    // 2^t is zero
 constexpr float kFarBelow = -1.0e30f;  // stands for a difference of -inf where a weight of zero multiplies it
 
 // Running maximum, sum of exponentials and sum of exponentials times differences, of one thread's elements.
@@ -146,6 +147,32 @@ __global__ void __launch_bounds__(kThreads) token_grad_kernel(const NxTokenRows 
   const float k = a.inv_temp * kLog2e;
   write_row(reinterpret_cast<const T*>(a.logits) + at, g, a.vocab, a.width, static_cast<int>(tg), c,
             [&](float v) { return -c * ex2_approx(fmaf(v - st.x, k, -st.y)); });
+}
+
+// Gradient of the policy loss from what its forward pass left of each row: g = p (slope (v - x) + off) and c at the target, times the loss's own
+// gradient before anything is rounded.  FP16 only, where a gradient that is rounded first and multiplied by a loss scale afterwards has lost all
+// below 2^-25: one more read of the logits than writing it forward.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) policy_grad_kernel(const NxTokenRows a, const NxPolicySlope* __restrict__ slopes,
+                                                               const float* __restrict__ factor, T* __restrict__ grad) {
+  pdl_dependency();
+  pdl_trigger();
+  const int64_t row = gridDim.x - 1 - blockIdx.x;  // the last rows first: the sums have left them in L2
+  const int64_t tg = target_at(a.targets, a.targets_wide, row);
+  const int64_t at = row_offset(a, row);
+  T* g = grad + at;
+  if (tg == a.ignore_index || tg < 0 || tg >= a.vocab) {
+    clear_row(g, a.width);
+    return;
+  }
+  const NxPolicySlope st = slopes[row];
+  const float f = *factor, k = a.inv_temp * kLog2e;
+  const float slope = st.slope * f, off = st.off * f, least = 2.0f * kNoWeight / k;
+  write_row(reinterpret_cast<const T*>(a.logits) + at, g, a.vocab, a.width, static_cast<int>(tg), st.c * f, [&](float v) {
+    float d = v - st.x;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(least));  // no weight from here on, and small enough to be multiplied
+    return ex2_approx(fmaf(d, k, -st.log2_s)) * fmaf(d, slope, off);
+  });
 }
 
 // ------------------------------------------------------------------------------------------------ policy loss
@@ -284,14 +311,15 @@ __device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, const Pol
 constexpr int kSlotBytes = 16384, kSlotPieces = kSlotBytes / 16;
 constexpr int kMaxCuts = 8;
 
-template <int WORKERS, int SLOTS, int RESIDENT>
+template <int WORKERS, int SLOTS, int RESIDENT, bool WRITES>
 struct Shape {
+  static constexpr bool kWrites = WRITES;                            // a second pass writes the gradient
   static constexpr int kWorkers = WORKERS, kThreads = WORKERS + 32;  // and the warp that copies
   static constexpr int kSlots = SLOTS, kResident = RESIDENT;         // blocks per SM
 };
-using SumsShape = Shape<128, 4, 3>;
-using ShortShape = Shape<256, 7, 2>;
-using LongShape = Shape<512, 13, 1>;
+using SumsShape = Shape<128, 4, 3, false>;
+using ShortShape = Shape<256, 7, 2, true>;
+using LongShape = Shape<512, 13, 1, true>;
 
 // A row's sums relative to its target's logit:  s = sum 2^t,  h = sum t 2^t  with  t = v k - B,  B = x_t k rounded,  k = log2(e) inv_temp.  The
 // base is the same for every thread and block, so joining is adding and no maximum is kept; the product is inside the fused multiply-add, so t
@@ -303,7 +331,6 @@ constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f;
 // Stands for -inf (and all below it) where t is multiplied: the weight is zero either way, and zero times a finite product is zero.  Representable in
 // BF16; no lower than it must be, so that k (up to 1.5e8) and the entropy's factors keep the products finite.
 constexpr float kFloor = -998244352.0f;
-constexpr float kNoWeight = -160.0f;  // 2^t is zero
 
 struct Pair {
   uint64_t v;
@@ -508,6 +535,7 @@ struct RingOut {
   float* kl;
   float* entropy;
   float* row_loss;
+  NxPolicySlope* slopes;  // policy: where given, what a row's gradient is made of later
   const double* totals;
   const int32_t* counts;
   int* ended;        // policy: blocks that have ended, zero before; the last one adds up the rows' losses
@@ -544,7 +572,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
   pdl_dependency();
   pdl_trigger();
 
-  const bool second = kPolicy && g.write_grad;
+  constexpr bool second = S::kWrites;
+  static_assert(kPolicy || !second);
   // slots of `n` pieces that are freed in the first pass: all without a second one; with one, those that the ring has no room for (and of a long
   // row two more, so that copies go on while the sums are joined)
   auto freed = [&](int n) {
@@ -739,6 +768,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
             o.kl[row] = pr.kl;
             o.entropy[row] = ent;
             o.row_loss[row] = pr.loss;
+            if (o.slopes != nullptr) {  // relative to the same logit as `stats` above; logp at it is -ln_s or lp
+              const float c = pr.c * a.inv_temp, e0 = pr.ent * a.inv_temp;
+              NxPolicySlope& to = o.slopes[row];
+              to.x = careful ? v.x : xt;
+              to.log2_s = log2_s - (careful ? 0.0f : coarse);
+              to.c = c;
+              to.slope = e0 * a.inv_temp;
+              to.off = g.entropy_coef != 0.0f ? e0 * (ent + (careful ? -ln_s : lp)) - c : -c;
+            }
           }
           const float inv_s = 1.0f / v.y, e1 = pr.ent * a.inv_temp;
           e.c = pr.c * a.inv_temp;
@@ -775,7 +813,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         if (warp == 0) end_row(st, true);
         workers_sync<S>();
       }
-      if (kPolicy && second) {
+      if constexpr (second) {
         const RowEnd e = sp->end;
         T* gr = grad + at;
         const int col0 = r.head + lo * VN;
@@ -939,8 +977,9 @@ int launch_ring(const NxTokenRows& a, const NxPolicyArgs& g, RingOut o, T* grad,
     return launch_shape<T, false, SumsShape>(a, g, o, grad, st);
   } else {
     if (!g.write_grad) return launch_shape<T, true, SumsShape>(a, g, o, grad, st);
-    if ((pieces + o.cuts - 1) / o.cuts + 1 <= ShortShape::kSlots * kSlotPieces) return launch_shape<T, true, ShortShape>(a, g, o, grad, st);
-    return launch_shape<T, true, LongShape>(a, g, o, grad, st);
+    if constexpr (std::is_same_v<T, __half>) return -1;  // nx_policy_loss_grad
+    else if ((pieces + o.cuts - 1) / o.cuts + 1 <= ShortShape::kSlots * kSlotPieces) return launch_shape<T, true, ShortShape>(a, g, o, grad, st);
+    else return launch_shape<T, true, LongShape>(a, g, o, grad, st);
   }
 }
 
@@ -1087,8 +1126,8 @@ extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, 
 }
 
 extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, double* totals, int32_t* counts, float* logp, float* kl,
-                              float* entropy, float* row_loss, float* loss, void* grad, int* status, nx_stream_t stream) {
-  if (!rows_ok(a) || a->rows == 0 || g == nullptr || totals == nullptr || (reinterpret_cast<uintptr_t>(totals) & 7) != 0 || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
+                              float* entropy, float* row_loss, float* loss, void* grad, NxPolicySlope* slopes, int* status, nx_stream_t stream) {
+  if (!rows_ok(a) || a->rows == 0 || g == nullptr || (reinterpret_cast<uintptr_t>(slopes) & 3) != 0 || totals == nullptr || (reinterpret_cast<uintptr_t>(totals) & 7) != 0 || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
       g->seq_len < 1 || g->seq_len > 0x7fffffff ||
       a->rows % g->seq_len != 0 || (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
     return -1;
@@ -1100,6 +1139,7 @@ extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, doubl
   o.kl = kl;
   o.entropy = entropy;
   o.row_loss = row_loss;
+  o.slopes = slopes;
   o.totals = totals;
   o.counts = counts;
   o.ended = reinterpret_cast<int*>(totals + 2);
@@ -1108,12 +1148,23 @@ extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, doubl
   NX_BY_TYPE(a->dtype, return (launch_ring<T, true>(*a, *g, o, static_cast<T*>(grad), st)))
 }
 
+extern "C" int nx_policy_loss_grad(const NxTokenRows* a, const NxPolicySlope* slopes, const float* factor, void* grad, nx_stream_t stream) {
+  if (!rows_ok(a) || a->dtype != NX_F16 || slopes == nullptr || (reinterpret_cast<uintptr_t>(slopes) & 3) != 0 || factor == nullptr ||
+      grad == nullptr || !same_lines(a->logits, grad))
+    return -1;
+  if (a->rows == 0) return 0;
+  NX_PDL((policy_grad_kernel<__half>), a->rows, kThreads, 0, static_cast<cudaStream_t>(stream), *a, slopes, factor, static_cast<__half*>(grad));
+  return 0;
+}
+
 extern "C" int nx_scale_unless_one(void* x, const float* factor, int dtype, int64_t n, nx_stream_t stream) {
-  if (n < 0 || factor == nullptr || (n > 0 && x == nullptr)) return -1;
+  if (n < 0 || factor == nullptr || (n > 0 && x == nullptr) || (dtype != NX_BF16 && dtype != NX_F32)) return -1;
   if (n == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  NX_BY_TYPE(dtype, const int64_t vec = (reinterpret_cast<uintptr_t>(x) & 15) ? 0 : n / RowVec<T>::kN;
-             NX_PDL((scale_unless_one_kernel<T>), blocks_for(std::max<int64_t>(vec, 1), 256), 256, 0, st, static_cast<T*>(x), factor, n, vec))
+  const int64_t vec = (reinterpret_cast<uintptr_t>(x) & 15) ? 0 : n / (dtype == NX_BF16 ? 8 : 4);
+  const int blocks = blocks_for(std::max<int64_t>(vec, 1), 256);
+  if (dtype == NX_BF16) NX_PDL((scale_unless_one_kernel<__nv_bfloat16>), blocks, 256, 0, st, static_cast<__nv_bfloat16*>(x), factor, n, vec);
+  else NX_PDL((scale_unless_one_kernel<float>), blocks, 256, 0, st, static_cast<float*>(x), factor, n, vec);
   return 0;
 }
 

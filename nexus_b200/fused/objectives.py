@@ -231,6 +231,36 @@ def _policy_forward(logits, targets, vocab, ignore_index, temperature, old, args
         return O.policy_loss(rows, args, old, grad), grad
 
 
+class _PolicyLossHalf(torch.autograd.Function):
+    """FP16: a loss scale has to be in the gradient before it is rounded, so the gradient is made in the backward pass, from the logits and five
+    values per row."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, vocab, ignore_index, temperature, old, args):
+        with _on(logits):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            slopes = old.new_empty(O.POLICY_SLOPE * rows.rows)
+            loss, logp, kl, entropy = O.policy_loss(rows, args, old, None, slopes)
+        ctx.save_for_backward(logits, targets, slopes)
+        ctx.cfg = (vocab, ignore_index, temperature)
+        ctx.mark_non_differentiable(logp, kl, entropy)
+        ctx.set_materialize_grads(False)
+        return loss, logp, kl, entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, *_):
+        if dloss is None:
+            return (None,) * 7
+        logits, targets, slopes = ctx.saved_tensors
+        vocab, ignore_index, temperature = ctx.cfg
+        with _on(logits):
+            logits, targets, rows = O.prepare_rows(logits, targets, vocab, ignore_index, 1.0 / temperature)
+            grad = O.empty_grad(logits)
+            O.policy_loss_grad(rows, slopes, dloss.float(), grad)
+        return (grad, *(None,) * 6)
+
+
 class _PolicyLoss(torch.autograd.Function):
     """Loss and gradient from one pass; the backward pass multiplies the gradient where the loss's own is not 1."""
 
@@ -269,7 +299,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     ``old_logp``, ``ref_logp`` and the advantages are constants.
 
     The gradient is made together with the loss, in one read of the logits; where the gradient of the loss itself is not 1 it is
-    multiplied afterwards, so the factor of an accumulated micro-batch is better given as ``scale``."""
+    multiplied afterwards, so the factor of an accumulated micro-batch is better given as ``scale``.  With FP16 logits it is made in the
+    backward pass, with a second read of them: a loss scale must be in it before it is rounded."""
     name = "policy_loss"
     V = _check_logits(name, logits, targets, vocab, temperature)
     if targets.dim() != 2:
@@ -293,7 +324,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
         a = O.PolicyArgs(old.data_ptr(), None if ref is None else ref.data_ptr(), adv.data_ptr(), T if adv.dim() == 1 else 1, T, clip_low, clip_high,
                          kl_coef, entropy_coef, scale, O.KL[kl], O.MEAN[reduction], 0)
         if _wants(logits):
-            return PolicyLoss(*_PolicyLoss.apply(logits, targets, V, ignore_index, float(temperature), old, a))
+            return PolicyLoss(*(_PolicyLossHalf if logits.dtype == torch.float16 else _PolicyLoss).apply(logits, targets, V, ignore_index, float(temperature), old, a))
         return PolicyLoss(*_policy_forward(logits, targets, V, ignore_index, temperature, old, a, False)[0])
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     zero = torch.zeros((), dtype=lp.dtype, device=lp.device)

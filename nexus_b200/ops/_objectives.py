@@ -18,7 +18,8 @@ _P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 _SIGNATURES = {
     "nx_token_logprobs": [_P, _P, _P, _P, _P, _P],
     "nx_token_logprobs_grad": [_P, _P, _P, _L, _P, _P, _P],
-    "nx_policy_loss": [_P] * 11 + [_P],
+    "nx_policy_loss": [_P] * 12 + [_P],
+    "nx_policy_loss_grad": [_P] * 5,
     "nx_scale_unless_one": [_P, _P, _I, _L, _P],
     "nx_preference_loss": [_P, _P, _P, _P, _P, _P],
     "nx_head_logprobs": [_P, _P, _P, _P],
@@ -127,8 +128,11 @@ def token_logprobs_grad(rows: TokenRows, stats, coef: int, coef_per: int, factor
           grad.data_ptr())
 
 
-def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad):
-    """FP32 (loss, logp, kl, entropy) of the shape of `like` (contiguous FP32, a value per token); `grad` (or None) is written."""
+POLICY_SLOPE = 5                 # FP32 values of a row that its gradient is made of
+
+
+def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad, slopes=None):
+    """FP32 (loss, logp, kl, entropy) of the shape of `like` (contiguous FP32, a value per token); `grad` and `slopes` (or None) are written."""
     n, dev = rows.rows, like.device
     loss = like.new_empty(())
     logp, kl, entropy = torch.empty_like(like), torch.empty_like(like), torch.empty_like(like)
@@ -136,8 +140,13 @@ def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad):
     at = scratch.data_ptr()
     args.write_grad = grad is not None
     _call("nx_policy_loss", C.byref(rows), C.byref(args), at, at + 24, logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
-          at + 24 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(), K.status_word(dev).data_ptr())
+          at + 24 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(), None if slopes is None else slopes.data_ptr(),
+          K.status_word(dev).data_ptr())
     return loss, logp, kl, entropy
+
+
+def policy_loss_grad(rows: TokenRows, slopes, factor, grad) -> None:
+    _call("nx_policy_loss_grad", C.byref(rows), slopes.data_ptr(), factor.data_ptr(), grad.data_ptr())
 
 
 def scale_unless_one_(x: torch.Tensor, factor: torch.Tensor) -> None:

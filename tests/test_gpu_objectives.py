@@ -430,6 +430,33 @@ def test_policy_gradient_of_a_scaled_loss():
         torch.autograd.grad(torch.autograd.grad(call(), x, create_graph=True)[0].sum(), x)
 
 
+@pytest.mark.parametrize("vocab", [333, 50257])
+@pytest.mark.parametrize("ent", [0.0, 0.02])
+@pytest.mark.parametrize("keep_graph", [False, True])
+def test_fp16_gradient_under_loss_scaling(vocab, ent, keep_graph):
+    """A loss times 2^14 keeps the gradients that FP16 could not hold without the factor."""
+    B, T, factor = 4, 64, 2.0 ** 14
+    x, t, old, ref, g = policy_inputs(B, T, vocab, F16, vocab + 7)
+    t[1, 40:] = -100
+    adv = (1e-3 * torch.randn(B, generator=g)).cuda()
+    want = policy64(x, t, old, adv, ref, vocab, "k3", "token", 1e-3, 1e-3 * ent, 0.2, 0.28)
+    x.requires_grad_(True)
+    r = F.policy_loss(x, t, old, adv, ref, clip_low=0.2, clip_high=0.28, kl_coef=1e-3, entropy_coef=1e-3 * ent, vocab=vocab)
+    (got,) = torch.autograd.grad(r.loss * factor, x, retain_graph=keep_graph)
+    if keep_graph:
+        (again,) = torch.autograd.grad(r.loss * factor, x)
+        assert torch.equal(got, again)
+    keep = (t != -100)[..., None]
+    p = softmax64(x, vocab, 1.0).exp()
+    gw = factor * want[4]
+    n = float((t != -100).sum())
+    size = factor / n * 1e-3 * (2 * adv.abs().max().double() * 1e3 + float(want[2].abs().max()) + 1 + ent * 40) * keep
+    err = grad_error(gw[..., :vocab], p, size, F16, vocab, coef_rel=float(4 * logp_error(want[1], vocab).max() + 32 * U))
+    close(got[..., :vocab], gw[..., :vocab], err * keep)
+    assert bool((got[..., vocab:] == 0).all())
+    assert float((got[..., :vocab] != 0).float().mean()) > float(((gw[..., :vocab].abs() > 2.0 ** -24)).float().mean()) - 1e-3
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("temperature", [1e-8, 1e-4, 1e4, 1e8])
 def test_entropy_gradient_of_masked_rows_at_extreme_temperatures(dtype, temperature):
