@@ -4,7 +4,8 @@
 // arguments, so nothing is uploaded and a captured graph carries its own.  A block walks over pieces of kPiece elements, whatever tensors they
 // belong to.  The second kernel's blocks each add up the first one's partial sums, in the same order, instead of a launch in between.
 // Bound by bytes: every gradient is read twice and written once; the second pass walks backwards, so that it begins with what the first one
-// left in L2.
+// left in L2.  8 x [4096, 4096] FP32: norm 82 us (6.5 TB/s), both passes to other memory 293 us (5.5 TB/s of two reads and a write); in place with a norm
+// that is small enough 107.  Other shapes of blocks (256, 1024 threads; two or four pieces in flight) and stores past L2 were no faster.
 #include "common.cuh"
 #include "nx_api_objectives.h"
 #include "row_vec.cuh"

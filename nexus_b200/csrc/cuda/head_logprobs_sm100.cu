@@ -10,6 +10,9 @@
 //   grad    otherwise h W^T again, whose epilogue turns the logits into G in 16 bits: one product more, and G of a bounded number of rows is
 //           all that is ever in memory
 //   dh, dW  G W and G^T h
+// Bound by the tensor cores: 2048 x 2048 x 32000 BF16 at 86 (statistics, exponentials written) and 87 % (dh) of their pipe, 180 us each, 1.49 PFLOP/s; at
+// 5376 x 4096 x 32000 1.05 ms for each of the three products, 1.33 PFLOP/s (to 1.43 in other runs), under
+// the power cap.
 // Rows whose target does not count are left out before the first product: the others are brought together in order (their number stays on the
 // device and bounds every loop), so that prompts and padding cost no tensor-core time.  A tile is 256 rows: without a gradient, up to that
 // many rows stay where they are (with one they would put 0 * h of a row that does not count into dW, and h may hold anything there).
@@ -80,7 +83,7 @@ struct Extent {
   int slices, per;          // input gradient: pieces of the vocabulary, and blocks of a piece
 };
 // Pieces of `blocks` 64-deep blocks for each of `tiles` tiles, so that the CTA pairs finish together: rounds times (blocks of a piece and six for
-// handing a tile over).  Chosen here, from the number of rows that count: by all rows, 380 of 609 kept 48 of the 74 pairs busy (154 us, not 105).
+// handing a tile over).  Chosen here, from the number of rows that count: by all rows, 380 of 609 kept 48 of the 74 pairs busy (156 us; now 130 to 141).
 __device__ __forceinline__ void cut(Extent& e, int tiles, int blocks, int most) {
   int best = 0x7fffffff;
   e.slices = 1;
@@ -570,7 +573,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 // Scoring beside decoding: the time is that of reading the weight once.  The weight's rows are the tall operand here: every SM takes one run of
 // the vocabulary, in groups of 32 rows so that the runs differ by at most one group (with 256 x 256 tiles 50257 rows were 197 tiles for 74 pairs,
 // three rounds for 2.7), and a lane of the epilogue keeps maximum and sum of one row of a tile for every token, over all tiles of the run; lanes
-// meet once, at its end.  8 x 50257 x 1600 BF16: 30 us (5.3 TB/s of weights), 256 x 256 tiles 44.
+// meet once, at its end.  8 x 50257 x 1600 BF16: 35 us (4.6 TB/s of weights), 256 x 256 tiles 44.
 constexpr int kFewRows = 64, kFewThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2..5: a quarter of the 128 lanes each
 constexpr int kGroupBytes = 32 * kBK * 2, kFewAccumulators = 4;
 template <int NT>
@@ -838,7 +841,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* __restric
 }
 
 // Joins the column tiles' maxima and sums of a row.  Eight rows per block (64 contiguous bytes of every tile), a quarter of a warp's lanes per row
-// and four loads of each in flight: 1188 tiles of 380 rows took 24 us with 32 rows per block and a load at a time.
+// and four loads of each in flight: 1188 tiles of 380 rows took 24 us with 32 rows per block and a load at a time, 9 now.
 constexpr int kJoinRows = 8;
 __global__ void __launch_bounds__(1024) join_kernel(const Params p, int parts, float* __restrict__ logp, float2* __restrict__ stats) {
   __shared__ float2 share[32][kJoinRows + 1];
@@ -937,6 +940,7 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 
 // Exponentials relative to the largest logit of their row and 128 columns -> gradient of the logits: each times the row's coefficient and the
 // 128 columns' share, the target's c more.  Rows up to the next multiple of 256 are cleared: the products read them.  from and to may be the same.
+// 5376 x 32000 BF16 in place: 125 to 143 us, 4.8 to 5.5 TB/s, bound by these bytes.
 template <bool BF>
 __global__ void __launch_bounds__(256) weigh_kernel(const Params p, const uint4* from, uint4* to, int64_t ld) {
   pdl_dependency();
@@ -1109,12 +1113,14 @@ int map_store(CUtensorMap* m, const NxHeadArgs* a, const void* base, int64_t col
 bool args_ok(const NxHeadArgs* a) {
   auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
   auto split = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) != 0; };  // pairs of floats
-  return a != nullptr && !split(a->stats) && !split(a->part) && (a->dtype == NX_BF16 || a->dtype == NX_F16) && a->rows > 0 && a->rows <= (1 << 30) && a->width > 0 && a->width % 8 == 0 &&
+  return a != nullptr && !split(a->stats) && !split(a->part) && (a->dtype == NX_BF16 || a->dtype == NX_F16) && a->rows > 0 &&
+         a->rows <= (1 << 30) && a->width > 0 && a->width % 8 == 0 &&
          a->vocab > 0 && a->vocab <= (1 << 30) && a->hidden != nullptr && a->weight != nullptr && a->targets != nullptr && !off(a->hidden) &&
          !off(a->weight) && a->ld_hidden % 8 == 0 && a->ld_weight % 8 == 0 && a->ld_hidden >= a->width && a->ld_weight >= a->width &&
          a->stats != nullptr && a->status != nullptr && (a->index == nullptr) == (a->count == nullptr) &&
          (a->index == nullptr) == (a->gathered == nullptr) && !off(a->gathered) &&
-         a->part_rows > 0 && a->part_rows % kTile == 0 && (a->weights == nullptr || (!off(a->weights) && a->part_rows >= a->rows && a->ld_weights >= a->vocab && a->ld_weights % 64 == 0));
+         a->part_rows > 0 && a->part_rows % kTile == 0 &&
+         (a->weights == nullptr || (!off(a->weights) && a->part_rows >= a->rows && a->ld_weights >= a->vocab && a->ld_weights % 64 == 0));
 }
 
 Params base_params(const NxHeadArgs* a) {

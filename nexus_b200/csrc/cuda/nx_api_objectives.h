@@ -71,9 +71,10 @@ typedef struct NxPreferenceArgs {
 int nx_preference_loss(const NxPreferenceArgs* args, float* seq_logp, float* margin, float* coef, float* loss, nx_stream_t stream);
 
 // Log-probabilities of `targets` [rows] under softmax(hidden weight^T * inv_temp), hidden [rows, width] of pitch ld_hidden, weight
-// [vocab, width] of pitch ld_weight, BF16 or FP16 (16-byte bases; width and pitches multiples of 8).  `index` [rows], `count` [1] and `gathered`
-// [rows rounded up to 64, width], all three or none (the gradient wants them): the rows that count are brought together before the products (the forward
-// call fills index and count; `gathered` is filled by both, with `weights` by the forward call for the gradient too).  stats [rows] pairs, written by the forward call, read by the gradient.
+// [vocab, width] of pitch ld_weight, BF16 or FP16 (16-byte bases; width and pitches multiples of 8).  `index` [rows], `count` [1] and
+// `gathered` [rows rounded up to 64, width], all three or none (the gradient wants them): the rows that count are brought together before
+// the products (the forward call fills index and count; `gathered` is filled by both, with `weights` by the forward call for the gradient
+// too).  stats [rows] pairs, written by the forward call, read by the gradient.
 typedef struct NxHeadArgs {
   const void* hidden;
   const void* weight;

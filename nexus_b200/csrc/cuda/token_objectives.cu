@@ -128,6 +128,7 @@ __device__ __forceinline__ void clear_row(T* g, int width) {
     Num<T>::store(g + sp.head + static_cast<int64_t>(sp.pieces) * VN + threadIdx.x - 32, 0.0f);
 }
 
+// c (delta - p) of each row.  8192 x 50304 BF16 or FP16: 262 us, 6.3 TB/s read and written, bound by these bytes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) token_grad_kernel(const NxTokenRows a, const float2* __restrict__ stats,
                                                               const float* __restrict__ coef, int64_t coef_per,
@@ -151,7 +152,8 @@ __global__ void __launch_bounds__(kThreads) token_grad_kernel(const NxTokenRows 
 
 // Gradient of the policy loss from what its forward pass left of each row: g = p (slope (v - x) + off) and c at the target, times the loss's own
 // gradient before anything is rounded.  FP16 only, where a gradient that is rounded first and multiplied by a loss scale afterwards has lost all
-// below 2^-25: one more read of the logits than writing it forward.
+// below 2^-25: one more read of the logits than writing it forward.  8192 x 50304: 264 us (6.2 TB/s) behind 166 of the forward pass; BF16, which has
+// the range of FP32 and writes it forward, 299 for both.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) policy_grad_kernel(const NxTokenRows a, const NxPolicySlope* __restrict__ slopes,
                                                                const float* __restrict__ factor, T* __restrict__ grad) {
@@ -304,10 +306,10 @@ __device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, const Pol
 //
 // Three shapes (BF16, B200; bytes read and written over the time):
 //   sums only                 three blocks of four warps per SM      8192 x 50304: 146 us, 5.6 TB/s; two of eight warps 156, one of sixteen 180
-//   gradient, rows to 112 KiB two blocks of eight warps              8192 x 50304: 283 us, 5.8 TB/s; one of sixteen 336, three of four 332
+//   gradient, rows to 112 KiB two blocks of eight warps              8192 x 50304: 283 us, 5.8 TB/s (to 304 in other runs); one of sixteen 336
 //   gradient, longer rows     one block of sixteen warps, 208 KiB    2368 x 32000 FP32: 101 us, 6.0 TB/s; two of eight 114
 // With sums and maxima kept per thread instead of a common base, 64-bit divisions per row in every thread and each row's target and constants
-// loaded at its beginning, the same ring took 465 us for 8192 x 50304 (11 instructions per element and pass instead of 5).
+// loaded at its beginning, the same ring took 465 us for 8192 x 50304 (11 instructions per element and pass instead of 7).
 constexpr int kSlotBytes = 16384, kSlotPieces = kSlotBytes / 16;
 constexpr int kMaxCuts = 8;
 
@@ -1117,7 +1119,9 @@ extern "C" int nx_token_logprobs(const NxTokenRows* a, float* logp, float* stats
 
 extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, const float* coef, int64_t coef_per, const float* factor,
                                       void* grad, nx_stream_t stream) {
-  if (!rows_ok(a) || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 7) != 0 || coef == nullptr || coef_per < 1 || coef_per > 0x7fffffff || grad == nullptr || !same_lines(a->logits, grad)) return -1;
+  if (!rows_ok(a) || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 7) != 0 || coef == nullptr || coef_per < 1 || coef_per > 0x7fffffff ||
+      grad == nullptr || !same_lines(a->logits, grad))
+    return -1;
   if (a->rows == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   NX_BY_TYPE(a->dtype, NX_PDL((token_grad_kernel<T>), a->rows, kThreads, 0, st, *a, reinterpret_cast<const float2*>(stats), coef, coef_per,
@@ -1127,9 +1131,9 @@ extern "C" int nx_token_logprobs_grad(const NxTokenRows* a, const float* stats, 
 
 extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, double* totals, int32_t* counts, float* logp, float* kl,
                               float* entropy, float* row_loss, float* loss, void* grad, NxPolicySlope* slopes, int* status, nx_stream_t stream) {
-  if (!rows_ok(a) || a->rows == 0 || g == nullptr || (reinterpret_cast<uintptr_t>(slopes) & 3) != 0 || totals == nullptr || (reinterpret_cast<uintptr_t>(totals) & 7) != 0 || counts == nullptr || loss == nullptr || status == nullptr || g->adv_per < 1 || g->adv_per > 0x7fffffff ||
-      g->seq_len < 1 || g->seq_len > 0x7fffffff ||
-      a->rows % g->seq_len != 0 || (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
+  if (!rows_ok(a) || a->rows == 0 || g == nullptr || (reinterpret_cast<uintptr_t>(slopes) & 3) != 0 ||
+      totals == nullptr || (reinterpret_cast<uintptr_t>(totals) & 7) != 0 || counts == nullptr || loss == nullptr || status == nullptr ||
+      g->adv_per < 1 || g->adv_per > 0x7fffffff || g->seq_len < 1 || g->seq_len > 0x7fffffff || a->rows % g->seq_len != 0 || (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   NX_PDL(token_count_kernel, kJoinBlocks, kJoinThreads, 0, st, a->targets, a->targets_wide, g->mean != NX_MEAN_NONE ? a->rows / g->seq_len : 0,
