@@ -325,10 +325,11 @@ using LongShape = Shape<512, 13, 1, true>;
 
 // A row's sums relative to its target's logit:  s = sum 2^t,  h = sum t 2^t  with  t = v k - B,  B = x_t k rounded,  k = log2(e) inv_temp.  The
 // base is the same for every thread and block, so joining is adding and no maximum is kept; the product is inside the fused multiply-add, so t
-// is exact to its own last bit, and results are taken relative to B itself.  The target's own term makes s at least 1.  A row where a logit lies
-// so far above its target's that the sums overflow (t of 120 and more), or where B would be too coarse (|x_t| above kFastLimit, -inf, NaN), is
-// done again in the form with running maxima and the difference first; and so is, where t is multiplied, one where the finite value that stands
-// for -inf (an FP16 piece holds none below -65504) comes so near the target's logit, or is scaled down so far, that its weight is not zero.
+// is exact to its own last bit, and results are taken relative to B itself.  The target's own term is 2^(x_t k - B): with |B| up to kFastLimit, B is
+// rounded by 2^-5 at most, and s is at least 0.97.  A row where a logit lies so far above its target's that the sums overflow (t of 120 and more), or
+// where B would be too coarse (|x_t| or |B| above kFastLimit: at temperatures of 1e-8 the second from logits of 0.007 on; -inf, NaN), is done again
+// in the form with running maxima and the difference first; and so is, where t is multiplied, one where the finite value that stands for -inf (an
+// FP16 piece holds none below -65504) comes so near the target's logit, or is scaled down so far, that its weight is not zero.
 constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f;
 // Stands for -inf (and all below it) where t is multiplied: the weight is zero either way, and zero times a finite product is zero.  Representable in
 // BF16; no lower than it must be, so that k (up to 1.5e8) and the entropy's factors keep the products finite.
@@ -793,7 +794,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         }
       };
       if (warp == 0) {
-        const bool careful = !(fabsf(xt) <= kFastLimit && st.y <= kFastSum && (!kPolicy || fmaf(PieceOf<T>::kLowest, k, -base) <= kNoWeight));
+        const bool careful = !(fabsf(xt) <= kFastLimit && fabsf(base) <= kFastLimit && st.y <= kFastSum && (!kPolicy || fmaf(PieceOf<T>::kLowest, k, -base) <= kNoWeight));
         if (!careful) end_row(st, false);
         else if (lane == 0) sp->end.careful = 1;
         if (!kPolicy && !careful && lane == 0) sp->end.careful = 0;

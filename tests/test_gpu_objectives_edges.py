@@ -1,0 +1,95 @@
+"""Ends of the ranges that the fine-tuning operators take, on the GPU: temperatures, rows far below their maximum, infinite margins, derivatives
+that are asked for in other ways.  Tolerances as in `test_gpu_objectives.py`, whose helpers are used."""
+import math
+
+import pytest
+import torch
+from test_gpu_objectives import BF16, F16, F32, U, close, grad_error, logp_error, softmax64
+
+from nexus_b200.fused import ops as F
+
+pytestmark = pytest.mark.gpu
+STEP = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: U}
+
+
+# ------------------------------------------------------------------------------------------------ low temperatures
+# target logits from which (target / temperature) log2 e is rounded by more than one
+LOW = [(1e-8, 4.0, 60.0), (1e-7, 200.0, 600.0), (1e-6, 1500.0, 6000.0), (1e-5, 15000.0, 60000.0), (1e-4, 30000.0, 64000.0)]
+
+
+def low_rows(dtype, lo, hi, vocab=300):
+    """[3, 64] rows at 64 values of the target's logit: alone above all others; beside another of the same value; a step below the largest."""
+    g = torch.Generator().manual_seed(int(lo))
+    top = torch.linspace(lo, hi, 64).to(dtype)
+    x = torch.randn(3, 64, vocab, generator=g).to(dtype)
+    t = torch.randint(1, vocab, (3, 64), generator=g)
+    x.scatter_(2, t[..., None], top[None, :, None].expand(3, 64, 1))
+    x[1:, :, 0] = top
+    below = top * (1 - 2 * torch.finfo(dtype).eps)
+    x[2].scatter_(1, t[2][:, None], below[:, None])
+    return x.cuda(), t.cuda()
+
+
+def low_expected(x, t, temperature):
+    lp = softmax64(x, x.shape[-1], temperature)
+    p = lp.exp()
+    return lp.gather(2, t[..., None])[..., 0], p, -torch.where(p > 0, p * lp.clamp(min=-1e30), 0.0).sum(-1), torch.where(p > 0, lp, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("temperature,lo,hi", LOW)
+def test_token_logprobs_at_low_temperatures(dtype, temperature, lo, hi):
+    x, t = low_rows(dtype, lo, hi)
+    want, p, _, _ = low_expected(x, t, temperature)
+    x.requires_grad_(True)
+    logp = F.token_logprobs(x, t, temperature=temperature)
+    close(logp.detach(), want, logp_error(want, 300))
+    logp.backward(torch.full_like(logp, temperature))
+    delta = torch.nn.functional.one_hot(t, 300).double()
+    one = torch.ones(3, 64, 1, dtype=torch.float64, device="cuda")
+    # the coefficient is a product with the rounded inverse of the temperature
+    close(x.grad, delta - p, grad_error(delta - p, p, one, dtype, 300, coef_rel=4 * U))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("temperature,lo,hi", LOW)
+@pytest.mark.parametrize("ent", [0.0, 0.05])
+def test_policy_loss_at_low_temperatures(dtype, temperature, lo, hi, ent):
+    x, t = low_rows(dtype, lo, hi)
+    want, p, H, lp = low_expected(x, t, temperature)
+    old = want.float()
+    old[2] = 0.0        # far from the old log-probability: the ratio is exp(logp), mostly zero
+    adv = torch.ones(3, device="cuda")
+    x.requires_grad_(True)
+    r = F.policy_loss(x, t, old, adv, entropy_coef=ent, temperature=temperature, reduction="sum", scale=temperature)
+    r.loss.backward()
+    close(r.logp, want, logp_error(want, 300))
+    close(r.entropy, H, U * (8 * H + 40 + 32))
+    c = torch.ones(3, 64, 1, dtype=torch.float64, device="cuda")
+    c[2] = torch.exp(want[2])[:, None]      # off by logp's own error, of itself
+    delta = torch.nn.functional.one_hot(t, 300).double()
+    gw = -c * (delta - p) + ent * torch.where(p > 0, p * (lp + H[..., None]), 0.0)
+    size = c + ent * (H[..., None] + 20.0)
+    rel = 64 * U + logp_error(want, 300)[..., None]
+    close(x.grad, gw, grad_error(gw, p, size, dtype, 300, coef_rel=rel) + STEP[dtype] * gw.abs())
+    loss = temperature * float((-c[..., 0] - ent * H).sum())
+    assert float(r.loss.detach()) == pytest.approx(loss, rel=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("temperature,lo,hi", LOW)
+def test_preference_loss_at_low_temperatures(dtype, temperature, lo, hi):
+    x, t = low_rows(dtype, lo, hi)
+    x, t = x[:2].contiguous(), t[:2]          # targets that share the largest value against ones that have it alone
+    want, p, _, _ = low_expected(x, t, temperature)
+    x.requires_grad_(True)
+    r = F.preference_loss(x, t, beta=0.1, temperature=temperature)
+    (r.loss * temperature).backward()
+    h = float(want[0].sum() - want[1].sum())
+    assert h == pytest.approx(64 * math.log(2), rel=1e-6) and float(r.margin) == pytest.approx(h, rel=1e-5)
+    assert float(r.loss.detach()) == pytest.approx(math.log1p(math.exp(-0.1 * h)), rel=1e-5)
+    slope = 0.1 / (1.0 + math.exp(0.1 * h))
+    delta = torch.nn.functional.one_hot(t, 300).double()
+    gw = slope * torch.tensor([-1.0, 1.0], device="cuda", dtype=torch.float64)[:, None, None] * (delta - p)
+    size = torch.full((2, 64, 1), slope, dtype=torch.float64, device="cuda")
+    close(x.grad, gw, grad_error(gw, p, size, dtype, 300, coef_rel=64 * U))
