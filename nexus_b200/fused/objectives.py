@@ -530,13 +530,39 @@ def _packed(t: torch.Tensor) -> torch.Tensor:
 
 
 def grad_square_sum(grads: Sequence[Optional[torch.Tensor]]) -> float:
-    """Sum of squares of all elements in FP64, on the host (one synchronisation): the square of the global gradient norm."""
-    grads, _ = _grad_list("grad_square_sum", list(grads), None)
-    if not _kernel_list(grads):
+    """Sum of squares of all elements in FP64, on the host (one synchronisation): the square of the global gradient norm.  Lists that the kernels do
+    not take (sparse tensors, tensors of several devices or of other types) are summed a tensor at a time."""
+    grads = [g for g in grads if g is not None]
+    if not _kernel_list(grads) or any(g.layout != torch.strided or g.device != grads[0].device for g in grads):
         return _square_sum_plain(grads)
     with _on(grads[0]):
         ts = [_packed(g) for g in grads if g.numel()]
         return float(O.grad_clip(O.grad_table(ts), ts[0].device, None)[0]) if ts else 0.0
+
+
+def clip_training_grads(grads: Sequence[torch.Tensor], max_norm: float) -> float:
+    """Clips the gradients of a training step in place by their global norm and returns the sum of their squares (one synchronisation); where that is
+    not finite they stay as they are.  Beside what `clip_grad_norm_` takes, gradients may be sparse, lie on several devices and share memory: such
+    lists are summed and scaled a tensor at a time."""
+    grads = list(grads)
+    table = _plain_table(grads, None)
+    if table is not None:
+        return float(_clip_table(table, grads, None, max_norm)[0])
+    sq = grad_square_sum(grads)
+    if math.isfinite(sq):
+        coef = min(1.0, max_norm / (math.sqrt(sq) + 1e-6))
+        if coef < 1.0:
+            with torch.no_grad():
+                for g in grads:
+                    g.mul_(coef)
+    return sq
+
+
+def _clip_table(table, grads, out, max_norm: float):
+    with _on(grads[0]):
+        norms = O.grad_clip(table, grads[0].device, max_norm)
+    torch.autograd.graph.increment_version(grads if out is None else out)
+    return norms
 
 
 def clip_grads(name: str, grads, max_norm: float, out=None):
@@ -547,10 +573,7 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
     out = out if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
     table = _plain_table(grads, out)
     if table is not None:
-        with _on(grads[0]):
-            norms = O.grad_clip(table, grads[0].device, max_norm)
-        torch.autograd.graph.increment_version(grads if out is None else out)
-        return norms
+        return _clip_table(table, grads, out, max_norm)
     grads, out = _grad_list(name, grads, out)
     if not grads:
         return torch.zeros((), dtype=torch.float64), torch.zeros((), dtype=torch.float32)

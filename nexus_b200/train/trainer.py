@@ -17,7 +17,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 import numpy as np
 import torch
 
-from ..fused.objectives import clip_grads, grad_square_sum
+from ..fused.objectives import clip_training_grads, grad_square_sum
 from ..loss import CrossEntropy
 from ..metrics import Accuracy
 from ..optim import SGD, AdamW
@@ -137,7 +137,7 @@ class Trainer:
             p.grad.mul_(inv)
         grads = [p.grad for p in params]
         if self.clip > 0:      # gradients whose norm is not finite stay as they are: the step is skipped below
-            sq = float(clip_grads("Trainer", grads, self.clip)[0])
+            sq = clip_training_grads(grads, self.clip)
         else:
             sq = grad_square_sum(grads)
         if not math.isfinite(sq):
