@@ -19,8 +19,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 _KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_KERNEL_SET = frozenset(_KERNEL_TYPES)
 _BYTES = (2, 4, 2)     # of the kernels' type codes
-_shape = attrgetter("shape")
+_shape, _dtype = attrgetter("shape"), attrgetter("dtype")
 _TARGET_TYPES = (torch.int32, torch.int64)
 O = None     # nexus_b200.ops._objectives, once a tensor on a GPU has been met
 
@@ -456,6 +457,9 @@ def _grad_list(name: str, grads, out):
             raise ValueError(f"{name}: takes dense floating-point tensors")
         if t.device != grads[0].device:
             raise ValueError(f"{name}: tensors on {t.device} and {grads[0].device}")
+    for g in grads:
+        if g.element_size() == 1:
+            raise ValueError(f"{name}: gradients of {g.dtype} cannot be scaled")
     if out is not None:
         for g, o in zip(grads, out):
             if g.shape != o.shape:
@@ -499,8 +503,10 @@ def _plain_table(grads, out):
             return None
         if out is not None and list(map(_shape, grads)) != list(map(_shape, out)):
             return None
+        if not _KERNEL_SET.issuperset(map(_dtype, every)):     # FP8 has a type code too
+            return None
         src, dst, counts, types = table = O.grad_table(grads, out)
-    except (AttributeError, KeyError, NotImplementedError, RuntimeError, TypeError):   # no tensors, or ones of other types, or without plain memory
+    except (AttributeError, NotImplementedError, RuntimeError, TypeError):   # no tensors, or ones without plain memory
         return None
     spans = [(at, n * _BYTES[t & 15]) for at, n, t in zip(src, counts, types)]
     if dst is not None:

@@ -56,3 +56,14 @@ def test_trainer_steps(sparse, clip):
     for a, b in zip(tr.model.parameters(), twin.parameters()):
         # AdamW divides the first steps' gradients by their own size: rounding of some 1e-6 of a gradient is as much of a step of 0.1
         assert float((a - b).abs().max()) < 1e-5
+
+
+def test_fp8_gradients_are_refused():
+    """A type that the library has codes for and the clipping does not take, first or behind others; an output may have it."""
+    a, b = torch.ones(8, device="cuda"), torch.ones(8, device="cuda").to(torch.float8_e4m3fn)
+    for call in (lambda: F.clip_grad_norm_([a, b], 1.0), lambda: F.clip_grad_norm_([b, a], 1.0), lambda: F.clip_grad_norm_([b], 1.0, out=[a])):
+        with pytest.raises(ValueError, match="float8"):
+            call()
+    assert torch.equal(a, torch.ones(8, device="cuda"))
+    assert float(F.clip_grad_norm_([2.0 * a], 1e3, out=[b])) == pytest.approx(32.0 ** 0.5) and bool((b.float() == 2.0).all())
+    assert F.grad_square_sum([a, b]) == 40.0
