@@ -1,8 +1,8 @@
 """Operators that fine-tune a language model on rewards and preferences: log-probabilities of given tokens, the clipped policy loss
 with KL and entropy terms, the preference loss over pairs, and the global gradient norm over many tensors with clipping.
 
-On CUDA logits (BF16, FP16, FP32) every operator runs hand-written sm_100a kernels (``csrc/cuda/token_objectives.cu``); elsewhere the
-same mathematics runs as plain PyTorch, which is also what the GPU tests compare against.  All of them are reached as
+On CUDA logits (BF16, FP16, FP32) every operator runs hand-written sm_100a kernels (``csrc/cuda/token_objectives.cu``); elsewhere, and for
+tensors that carry a forward-mode derivative, the same mathematics runs as plain PyTorch.  All of them are reached as
 ``fused.ops.<name>``, beside the cross-entropy.
 
 With x = logits / temperature over the vocabulary: logp_t = x_t - logsumexp(x), H = -sum p log p.  A target equal to `ignore_index`
@@ -16,6 +16,7 @@ from operator import attrgetter
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -77,6 +78,8 @@ def _check_values(name: str, what: str, t, shapes, device) -> torch.Tensor:
         raise ValueError(f"{name}: {what} on {t.device}, logits on {device}")
     if t.requires_grad:
         t = t.detach()
+    if _dual(t):
+        t = forward_ad.unpack_dual(t).primal
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
@@ -86,6 +89,16 @@ _HERE = contextlib.nullcontext()
 def _on(t: torch.Tensor):
     """Makes a tensor's device the current one, where it is not: the launches go to the current device's stream."""
     return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _dual(*ts: torch.Tensor) -> bool:
+    """Whether a tensor carries a forward-mode derivative, which the kernels would drop."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
+def _backward_only(name: str, t: torch.Tensor) -> None:
+    if _dual(t):
+        raise NotImplementedError(f"{name}: its gradient has no forward-mode derivative")
 
 
 def _kernels(t: torch.Tensor) -> bool:
@@ -137,6 +150,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
+        _backward_only("token_logprobs", dlogp)
         logits, targets, stats = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         with _on(logits):
@@ -152,7 +166,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: in
     """FP32 log-probability of ``targets`` [...] under ``softmax(logits / temperature)``, logits [..., V(+pad)]; zero where the target is
     `ignore_index`.  Differentiable (once) with respect to the logits; any row strides, the innermost one 1 (others are copied)."""
     V = _check_logits("token_logprobs", logits, targets, vocab, temperature)
-    if targets.numel() and _kernels(logits):
+    if targets.numel() and _kernels(logits) and not _dual(logits):
         if _wants(logits):
             return _TokenLogprobs.apply(logits, targets, V, ignore_index, float(temperature))
         return _token_forward(logits, targets, V, ignore_index, temperature)[2]
@@ -180,6 +194,7 @@ class _LinearLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogp):
+        _backward_only("linear_logprobs", dlogp)
         hidden, weight, t, block, weights = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         again = torch._C._autograd._get_current_graph_task_keep_graph()
@@ -217,7 +232,7 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
     if not 1 <= V <= weight.shape[0]:
         raise ValueError(f"{name}: vocab must be between 1 and {weight.shape[0]}, got {V}")
     d, n = hidden.shape[-1], targets.numel()
-    if n and d and d % 8 == 0 and hidden.dtype != torch.float32 and max(n, V) <= 1 << 30 and _kernels(hidden):
+    if n and d and d % 8 == 0 and hidden.dtype != torch.float32 and max(n, V) <= 1 << 30 and _kernels(hidden) and not _dual(hidden, weight):
         if _wants(hidden, weight):
             return _LinearLogprobs.apply(hidden, weight, targets, V, ignore_index, float(temperature), bool(recompute))
         return _linear_forward(hidden, weight, targets, V, ignore_index, temperature, False, False)[1]
@@ -253,6 +268,7 @@ class _PolicyLossHalf(torch.autograd.Function):
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 7
+        _backward_only("policy_loss", dloss)
         logits, targets, slopes = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         with _on(logits):
@@ -278,6 +294,7 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 7
+        _backward_only("policy_loss", dloss)
         (grad,) = ctx.saved_tensors
         # a graph that is kept may be walked again, and then needs the gradient as it was
         if torch._C._autograd._get_current_graph_task_keep_graph():
@@ -321,7 +338,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     old = _check_values(name, "old_logp", old_logp, [(B, T)], logits.device)
     adv = _check_values(name, "advantages", advantages, [(B, T), (B,)], logits.device)
     ref = None if ref_logp is None else _check_values(name, "ref_logp", ref_logp, [(B, T)], logits.device)
-    if targets.numel() and _kernels(logits):
+    if targets.numel() and _kernels(logits) and not _dual(logits):
         a = O.PolicyArgs(old.data_ptr(), None if ref is None else ref.data_ptr(), adv.data_ptr(), T if adv.dim() == 1 else 1, T, clip_low, clip_high,
                          kl_coef, entropy_coef, scale, O.KL[kl], O.MEAN[reduction], 0)
         if _wants(logits):
@@ -372,6 +389,7 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 7
+        _backward_only("preference_loss", dloss)
         logits, targets, kept = ctx.saved_tensors
         vocab, ignore_index, temperature = ctx.cfg
         with _on(logits):
@@ -405,7 +423,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optio
         raise ValueError(f"{name}: target_margin must be finite, and does not belong to the ipo loss")
     pairs = targets.shape[0] // 2
     ref = None if ref_logp is None else _check_values(name, "ref_logp", ref_logp, [(2 * pairs,)], logits.device)
-    if targets.numel() and _kernels(logits):
+    if targets.numel() and _kernels(logits) and not _dual(logits):
         options = dict(kind=kind, average=bool(average), beta=beta, smoothing=label_smoothing, target_margin=target_margin)
         if _wants(logits):
             return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, V, ignore_index, float(temperature), ref, options))
@@ -577,6 +595,8 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
         raise ValueError(f"{name}: max_norm must not be negative, got {max_norm}")
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     out = out if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    if forward_ad._current_level >= 0 and _dual(*(t for t in grads + (out or []) if isinstance(t, torch.Tensor))):
+        raise NotImplementedError(f"{name}: has no forward-mode derivative")
     table = _plain_table(grads, out)
     if table is not None:
         return _clip_table(table, grads, out, max_norm)

@@ -93,3 +93,56 @@ def test_preference_loss_at_low_temperatures(dtype, temperature, lo, hi):
     gw = slope * torch.tensor([-1.0, 1.0], device="cuda", dtype=torch.float64)[:, None, None] * (delta - p)
     size = torch.full((2, 64, 1), slope, dtype=torch.float64, device="cuda")
     close(x.grad, gw, grad_error(gw, p, size, dtype, 300, coef_rel=64 * U))
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+def dual_calls(dtype):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 5, 24, generator=g).to(dtype).cuda()
+    t = torch.randint(0, 24, (4, 5), generator=g).cuda()
+    t[0, :2] = -100
+    h, w = torch.randn(4, 5, 16, generator=g).to(dtype).cuda(), torch.randn(24, 16, generator=g).to(dtype).cuda()
+    old, adv = torch.full((4, 5), -3.0, device="cuda"), torch.ones(4, device="cuda")
+    return [(lambda v: F.token_logprobs(v, t), x), (lambda v: F.policy_loss(v, t, old, adv, entropy_coef=0.1).loss, x),
+            (lambda v: F.preference_loss(v, t).loss, x), (lambda v: F.linear_logprobs(v, w, t), h), (lambda v: F.linear_logprobs(h, v, t), w)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_forward_mode_derivatives(dtype):
+    """A tangent along v against the product of v with the gradient; values as without one."""
+    from torch.autograd import forward_ad
+    for call, x in dual_calls(dtype):
+        v = torch.randn(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).to(dtype)
+        leaf = x.clone().requires_grad_(True)
+        out = call(leaf)
+        up = torch.randn(out.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+        want = float((torch.autograd.grad(out, leaf, up)[0].double() * v.double()).sum())
+        with forward_ad.dual_level():
+            got = forward_ad.unpack_dual(call(forward_ad.make_dual(x, v)))
+            assert got.tangent is not None
+            tangent = float((got.tangent.double() * up.double()).sum())
+        _, by_func = torch.func.jvp(call, (x,), (v,))
+        # the sums have some hundred elements of order one, each rounded to the type
+        room = 4 * STEP[dtype] * x.numel() ** 0.5 + 1e-5
+        assert abs(tangent - want) < room and abs(float((by_func.double() * up.double()).sum()) - want) < room
+        assert torch.allclose(got.primal.detach(), out.detach(), atol=0.1 if dtype == BF16 else 1e-5)
+
+
+def test_forward_mode_derivatives_of_gradients_are_refused():
+    from torch.autograd import forward_ad
+    for call, x in dual_calls(F32)[:3]:
+        leaf = x.clone().requires_grad_(True)
+        with forward_ad.dual_level():
+            out = call(leaf)
+            up = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, up)
+
+
+def test_tangents_of_constants_are_dropped():
+    from torch.autograd import forward_ad
+    x, t = torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 3, dtype=torch.long, device="cuda")
+    with forward_ad.dual_level():
+        old = forward_ad.make_dual(torch.zeros(2, 3, device="cuda"), torch.ones(2, 3, device="cuda"))
+        for v in (x, x.double()):
+            assert forward_ad.unpack_dual(F.policy_loss(v, t, old, torch.ones(2, device="cuda")).loss).tangent is None

@@ -16,3 +16,21 @@ def test_fp8_gradients_are_refused():
     assert torch.equal(a, torch.ones(8))
     assert float(F.clip_grad_norm_([2.0 * a], 1e3, out=[b])) == pytest.approx(32.0 ** 0.5) and bool((b.float() == 2.0).all())
     assert F.grad_square_sum([a, b]) == 40.0
+
+
+def test_forward_mode_derivatives():
+    """Log-probabilities carry a tangent, constants of a loss none, and the clipping refuses it."""
+    from torch.autograd import forward_ad
+    g = torch.Generator().manual_seed(0)
+    x, v = torch.randn(2, 3, 8, generator=g), torch.randn(2, 3, 8, generator=g)
+    t = torch.randint(0, 8, (2, 3), generator=g)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, v)
+        got = forward_ad.unpack_dual(F.token_logprobs(d, t)).tangent
+        old = forward_ad.make_dual(torch.zeros(2, 3), torch.ones(2, 3))
+        assert forward_ad.unpack_dual(F.policy_loss(x, t, old, torch.ones(2)).loss).tangent is None
+        for grads, out in (([x, d], None), ([x], [d])):
+            with pytest.raises(NotImplementedError):
+                F.clip_grad_norm_(grads, 1.0, out=out)
+    want = v.gather(2, t[..., None])[..., 0] - (x.softmax(-1) * v).sum(-1)
+    assert torch.allclose(got, want, atol=1e-6)
