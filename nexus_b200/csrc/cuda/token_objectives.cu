@@ -330,7 +330,9 @@ using LongShape = Shape<512, 13, 1, true>;
 // where B would be too coarse (|x_t| or |B| above kFastLimit: at temperatures of 1e-8 the second from logits of 0.007 on; -inf, NaN), is done again
 // in the form with running maxima and the difference first; and so is, where t is multiplied, one where the finite value that stands for -inf (an
 // FP16 piece holds none below -65504) comes so near the target's logit, or is scaled down so far, that its weight is not zero.
-constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f;
+// Where a second pass writes the gradient its factors are divided by s, and are normal numbers (the row's weight being 2^-66 or more) only while s stays
+// below 2^60: t of 60 and more, targets of a log-probability below -41, are done again there.
+constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f, kFastSumDivides = 0x1p60f;
 // Stands for -inf (and all below it) where t is multiplied: the weight is zero either way, and zero times a finite product is zero.  Representable in
 // BF16; no lower than it must be, so that k (up to 1.5e8) and the entropy's factors keep the products finite.
 constexpr float kFloor = -998244352.0f;
@@ -794,7 +796,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         }
       };
       if (warp == 0) {
-        const bool careful = !(fabsf(xt) <= kFastLimit && fabsf(base) <= kFastLimit && st.y <= kFastSum && (!kPolicy || fmaf(PieceOf<T>::kLowest, k, -base) <= kNoWeight));
+        const bool careful = !(fabsf(xt) <= kFastLimit && fabsf(base) <= kFastLimit && st.y <= (second ? kFastSumDivides : kFastSum) &&
+                               (!kPolicy || fmaf(PieceOf<T>::kLowest, k, -base) <= kNoWeight));
         if (!careful) end_row(st, false);
         else if (lane == 0) sp->end.careful = 1;
         if (!kPolicy && !careful && lane == 0) sp->end.careful = 0;

@@ -146,3 +146,29 @@ def test_tangents_of_constants_are_dropped():
         old = forward_ad.make_dual(torch.zeros(2, 3, device="cuda"), torch.ones(2, 3, device="cuda"))
         for v in (x, x.double()):
             assert forward_ad.unpack_dual(F.policy_loss(v, t, old, torch.ones(2, device="cuda")).loss).tangent is None
+
+
+# ------------------------------------------------------------------------------------------------ targets far below the maximum
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("below", [40.0, 60.0, 75.0, 80.0, 83.0, 100.0])
+@pytest.mark.parametrize("ent", [0.0, 1e-3])
+def test_policy_gradient_of_unlikely_targets(dtype, below, ent):
+    """A weight per token of 1e-5 over a sum of exponentials up to e^100 times the target's own: the gradient keeps its digits."""
+    g = torch.Generator().manual_seed(int(below))
+    x = torch.randn(2, 6, 900, generator=g).to(dtype).cuda()
+    t = torch.randint(0, 400, (2, 6), generator=g).cuda()
+    x[..., 500:503] = torch.tensor([below, below - 1.0, below - 3.0], dtype=dtype)
+    x.scatter_(2, t[..., None], 0.0)
+    want = softmax64(x, 900, 1.0)
+    p, one = want.exp(), want.gather(2, t[..., None])[..., 0]
+    H = -(p * want).sum(-1, keepdim=True)
+    x.requires_grad_(True)
+    r = F.policy_loss(x, t, one.float(), torch.ones(2, device="cuda"), entropy_coef=ent, reduction="sum", scale=1e-5)
+    r.loss.backward()
+    close(r.logp, one, logp_error(one, 900))
+    delta = torch.nn.functional.one_hot(t, 900).double()
+    gw = 1e-5 * (-(delta - p) + ent * p * (want + H))
+    # the ratio is off by the errors of logp and of the old one's rounding; log p + H by two roundings of either
+    rel = 64 * U + float(logp_error(one, 900).max()) + U * (below + 20)
+    size = 1e-5 * (1.0 + ent * (H + 20.0))
+    close(x.grad, gw, grad_error(gw, p, size, dtype, 900, coef_rel=rel) + STEP[dtype] * gw.abs())
