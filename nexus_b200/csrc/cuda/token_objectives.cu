@@ -1053,9 +1053,11 @@ preference_kernel(const NxPreferenceArgs a, float* __restrict__ seq_logp, float*
         value = z < 1.0 ? 1.0 - z : (z == z ? 0.0 : z);
         slope = z < 1.0 ? -a.beta : 0.0;
       } else {
-        // -(1 - e) ln sig(z) - e ln sig(-z) = ln(1 + exp(-|z|)) + max(-z, 0) + e z
+        // -(1 - e) ln sig(z) - e ln sig(-z) = ln(1 + exp(-|z|)) + (e - 1 where z < 0, else e) z; z may be infinite (a sequence that cannot be)
         const double t = exp(-fabs(z)), sig = z >= 0.0 ? t / (1.0 + t) : 1.0 / (1.0 + t);  // sig = sigmoid(-z)
-        value = log1p(t) + (z < 0.0 ? -z : 0.0) + a.smoothing * z;
+        value = log1p(t);
+        if (z < 0.0) value += (a.smoothing - 1.0) * z;
+        else if (a.smoothing != 0.0f) value += a.smoothing * z;
         slope = a.beta * (a.smoothing - sig);
       }
     }

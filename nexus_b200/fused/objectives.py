@@ -436,7 +436,9 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optio
     h = ratio[:pairs] - ratio[pairs:]
     z = beta * h - target_margin
     if kind == "sigmoid":
-        each = -torch.nn.functional.logsigmoid(z) + label_smoothing * z
+        each = (label_smoothing - 1.0) * torch.nn.functional.logsigmoid(z)
+        if label_smoothing:      # of an infinite z, zero times the other side's logarithm is no number
+            each = each - label_smoothing * torch.nn.functional.logsigmoid(-z)
     elif kind == "hinge":
         each = (1.0 - z).clamp(min=0.0)
     else:

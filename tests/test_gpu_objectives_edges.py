@@ -172,3 +172,27 @@ def test_policy_gradient_of_unlikely_targets(dtype, below, ent):
     rel = 64 * U + float(logp_error(one, 900).max()) + U * (below + 20)
     size = 1e-5 * (1.0 + ent * (H + 20.0))
     close(x.grad, gw, grad_error(gw, p, size, dtype, 900, coef_rel=rel) + STEP[dtype] * gw.abs())
+
+
+@pytest.mark.parametrize("kind,smoothing", [("sigmoid", 0.0), ("sigmoid", 0.1), ("hinge", 0.0)])
+@pytest.mark.parametrize("side", [0, 1])
+def test_preference_of_a_sequence_that_cannot_be(kind, smoothing, side):
+    """A target whose logit is -inf in the chosen sequence (0) or in the rejected one (1): the loss is its limit, and the gradient finite."""
+    x = torch.zeros(4, 2, 4, device="cuda")
+    x[2 * side, 1, 0] = -math.inf        # of the first pair, which is rows 0 and 2
+    x.requires_grad_(True)
+    t = torch.zeros(4, 2, dtype=torch.long, device="cuda")
+    r = F.preference_loss(x, t, beta=0.5, kind=kind, label_smoothing=smoothing)
+    r.loss.backward()
+    other = math.log(2.0) if kind == "sigmoid" else 1.0
+    limit = {("sigmoid", 0): math.inf, ("sigmoid", 1): math.inf if smoothing else 0.0, ("hinge", 0): math.inf, ("hinge", 1): 0.0}[kind, side]
+    assert float(r.margin[0]) == (math.inf if side else -math.inf) and float(r.margin[1]) == 0.0
+    assert float(r.loss.detach()) == pytest.approx((limit + other) / 2)
+    slope = {"sigmoid": 0.5 * (smoothing - (0.0 if side else 1.0)), "hinge": 0.0 if side else -0.5}[kind] / 2
+    p = torch.softmax(x.detach().double(), -1)
+    want = torch.zeros_like(p)
+    want[..., 0] = 1.0
+    want = (want - p) * slope
+    want[2] = -want[2]
+    assert torch.allclose(x.grad[[0, 2]].double(), want[[0, 2]], atol=1e-6)
+    assert bool(torch.isfinite(x.grad).all())
