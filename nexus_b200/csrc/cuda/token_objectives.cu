@@ -287,8 +287,10 @@ __device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, const Pol
       o.kl = -d;
       slope = 1.0f;
     }
-    loss = fmaf(g.kl_coef, o.kl, loss);
-    c = fmaf(g.kl_coef, slope, c);
+    if (g.kl_coef != 0.0f) {  // an estimate that is only looked at may be infinite
+      loss = fmaf(g.kl_coef, o.kl, loss);
+      c = fmaf(g.kl_coef, slope, c);
+    }
   }
   if (g.entropy_coef != 0.0f) loss -= g.entropy_coef * entropy;
   o.loss = loss * in.weight;

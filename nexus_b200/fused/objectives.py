@@ -355,7 +355,10 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     if ref is not None:
         d = ref.to(lp.dtype).reshape(-1) - logp
         div = {"k1": -d, "k2": 0.5 * d * d, "k3": torch.expm1(d) - d}[kl]
-    per = torch.where(keep, kl_coef * div - gain - entropy_coef * ent, zero)
+    per = -gain
+    if kl_coef:               # an estimate that is only looked at may be infinite
+        per = per + kl_coef * div
+    per = torch.where(keep, per - entropy_coef * ent, zero)
     counts = keep.view(B, T).sum(-1)
     if reduction == "token":
         per = per / counts.sum().clamp(min=1)

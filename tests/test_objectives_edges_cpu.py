@@ -58,3 +58,21 @@ def test_preference_of_a_sequence_that_cannot_be(kind, smoothing, side):
     want[2] = -want[2]
     assert torch.allclose(x.grad[[0, 2]].double(), want[[0, 2]], atol=1e-6)
     assert bool(torch.isfinite(x.grad).all())
+
+
+@pytest.mark.parametrize("kl", ["k1", "k2", "k3"])
+def test_an_estimate_of_the_divergence_that_is_only_looked_at(kl):
+    """Without a KL term its estimate, which may overflow, is in neither the loss nor the gradient."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(2, 3, 8, generator=g)
+    t = torch.randint(0, 7, (2, 3), generator=g)
+    x[0, 0, 7] = 200.0                  # a target 200 below: exp(ref - logp) is beyond FP32
+    x.requires_grad_(True)
+    old = F.token_logprobs(x, t).detach()
+    ref = torch.full((2, 3), -1.0)
+    grads = []
+    for with_ref in (None, ref):
+        r = F.policy_loss(x, t, old, torch.ones(2), with_ref, kl=kl)
+        grads.append((r.loss.detach(), torch.autograd.grad(r.loss, x)[0]))
+    assert bool(torch.isfinite(grads[1][1]).all()) and float(r.kl[0, 0]) == (math.inf if kl == "k3" else pytest.approx(float(r.kl[0, 0])))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
