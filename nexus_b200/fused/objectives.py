@@ -347,7 +347,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     zero = torch.zeros((), dtype=lp.dtype, device=lp.device)
     p = lp.exp()
-    ent = torch.where(keep, -torch.where(p > 0, p * lp, zero).sum(-1), zero)
+    ent = torch.where(keep, -(p * torch.where(p > 0, lp, zero)).sum(-1), zero)     # the product outside: the gradient of 0 * -inf is no number
     old, adv = old.to(lp.dtype).reshape(-1), (adv if adv.dim() == 2 else adv[:, None].expand(B, T)).to(lp.dtype).reshape(-1)
     ratio = torch.exp(logp - old)
     gain = torch.minimum(ratio * adv, ratio.clamp(1.0 - clip_low, 1.0 + clip_high) * adv)

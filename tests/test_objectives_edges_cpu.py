@@ -76,3 +76,20 @@ def test_an_estimate_of_the_divergence_that_is_only_looked_at(kl):
         grads.append((r.loss.detach(), torch.autograd.grad(r.loss, x)[0]))
     assert bool(torch.isfinite(grads[1][1]).all()) and float(r.kl[0, 0]) == (math.inf if kl == "k3" else pytest.approx(float(r.kl[0, 0])))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("ent", [0.0, 0.05])
+def test_masked_vocabulary(ent):
+    """Entries of -inf have no weight and no gradient in the policy loss: as the vocabulary without them."""
+    g = torch.Generator().manual_seed(3)
+    short = torch.randn(2, 4, 9, dtype=torch.float64, generator=g, requires_grad=True)
+    t = torch.randint(0, 9, (2, 4), generator=g)
+    t[1, 3] = -100
+    x = torch.cat([short.detach(), torch.full((2, 4, 5), -math.inf, dtype=torch.float64)], -1).requires_grad_(True)
+    old, adv = torch.full((2, 4), -2.0), torch.tensor([1.0, -0.5])
+    results = []
+    for v in (short, x):
+        r = F.policy_loss(v, t, old, adv, entropy_coef=ent)
+        results.append((r.loss.detach(), r.entropy, torch.autograd.grad(r.loss, v)[0]))
+    (a, ea, ga), (b, eb, gb) = results
+    assert torch.allclose(a, b) and torch.allclose(ea, eb) and torch.allclose(ga, gb[..., :9]) and bool((gb[..., 9:] == 0).all())
