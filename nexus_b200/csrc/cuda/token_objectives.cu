@@ -267,7 +267,8 @@ __device__ __forceinline__ PolicyIn policy_in(const NxPolicyArgs& g, const doubl
 }
 __device__ __forceinline__ PolicyRow policy_row(const NxPolicyArgs& g, const PolicyIn& in, float logp, float entropy) {
   PolicyRow o;
-  const float ratio = expf(logp - in.old);
+  float ratio = expf(logp - in.old);
+  if (in.adv == 0.0f && ratio == INFINITY) ratio = 1.0f;  // beyond FP32, and counted zero times
   const float free = ratio * in.adv, bound = fminf(fmaxf(ratio, 1.0f - g.clip_low), 1.0f + g.clip_high) * in.adv;
   // the unclipped term where it is the smaller one, or they are equal, or it is no number
   const bool follows = !(free > bound);

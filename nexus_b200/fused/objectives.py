@@ -349,7 +349,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     p = lp.exp()
     ent = torch.where(keep, -(p * torch.where(p > 0, lp, zero)).sum(-1), zero)     # the product outside: the gradient of 0 * -inf is no number
     old, adv = old.to(lp.dtype).reshape(-1), (adv if adv.dim() == 2 else adv[:, None].expand(B, T)).to(lp.dtype).reshape(-1)
-    ratio = torch.exp(logp - old)
+    moved = logp - old
+    ratio = torch.exp(torch.where((adv == 0) & torch.isinf(torch.exp(moved.detach())), zero, moved))     # beyond the type, and counted zero times
     gain = torch.minimum(ratio * adv, ratio.clamp(1.0 - clip_low, 1.0 + clip_high) * adv)
     div = torch.zeros_like(logp)
     if ref is not None:

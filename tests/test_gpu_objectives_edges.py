@@ -214,3 +214,15 @@ def test_an_estimate_of_the_divergence_that_is_only_looked_at(kl):
         grads.append((r.loss.detach(), torch.autograd.grad(r.loss, x)[0]))
     assert bool(torch.isfinite(grads[1][1]).all()) and float(r.kl[0, 0]) == (math.inf if kl == "k3" else pytest.approx(float(r.kl[0, 0])))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_advantages_of_zero_beside_ratios_beyond_fp32():
+    x = torch.zeros(2, 2, 8, device="cuda", requires_grad=True)
+    t = torch.zeros(2, 2, dtype=torch.long, device="cuda")
+    old = torch.full((2, 2), -100.0, device="cuda")                     # exp(100 - ln 8)
+    r = F.policy_loss(x, t, old, torch.zeros(2, device="cuda"))
+    r.loss.backward()
+    assert float(r.loss.detach()) == 0.0 and bool((x.grad == 0).all())
+    old[0, 0] = math.nan
+    assert math.isnan(float(F.policy_loss(x, t, old, torch.zeros(2, device="cuda")).loss.detach()))
+    assert math.isinf(float(F.policy_loss(x, t, torch.full_like(old, -100.0), -torch.ones(2, device="cuda")).loss.detach()))

@@ -93,3 +93,15 @@ def test_masked_vocabulary(ent):
         results.append((r.loss.detach(), r.entropy, torch.autograd.grad(r.loss, v)[0]))
     (a, ea, ga), (b, eb, gb) = results
     assert torch.allclose(a, b) and torch.allclose(ea, eb) and torch.allclose(ga, gb[..., :9]) and bool((gb[..., 9:] == 0).all())
+
+
+def test_advantages_of_zero_beside_ratios_beyond_fp32():
+    x = torch.zeros(2, 2, 8, requires_grad=True)
+    t = torch.zeros(2, 2, dtype=torch.long)
+    old = torch.full((2, 2), -100.0)                     # exp(100 - ln 8)
+    r = F.policy_loss(x, t, old, torch.zeros(2))
+    r.loss.backward()
+    assert float(r.loss.detach()) == 0.0 and bool((x.grad == 0).all())
+    old[0, 0] = math.nan
+    assert math.isnan(float(F.policy_loss(x, t, old, torch.zeros(2)).loss.detach()))
+    assert math.isinf(float(F.policy_loss(x, t, torch.full_like(old, -100.0), -torch.ones(2)).loss.detach()))
