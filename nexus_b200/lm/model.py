@@ -366,19 +366,27 @@ class LanguageModel(nn.Module):
     def _logit_scale(self) -> float:
         return self.config.mup_base_width / self.config.d_model if self.config.init == "mup" else 1.0
 
-    def token_logprobs(self, tokens: torch.Tensor, mask: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+    def token_logprobs(self, tokens: torch.Tensor, mask: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                       through_logits: bool = False) -> torch.Tensor:
         """FP32 log-probabilities [B, T] of the next tokens: entry t is that of ``tokens[:, t + 1]`` (zero at the last position and for
-        tokens whose ``mask`` is false: prompts, padding).  The logits are never in memory (`fused.ops.linear_logprobs`): what scores the
-        samples of an older policy or of a reference model, under ``torch.no_grad``, and what other objectives differentiate."""
+        tokens whose ``mask`` is false: prompts, padding).
+
+        By default from the hidden states and the head's weight (`fused.ops.linear_logprobs`): with BF16 or FP16 activations the logits are never in
+        memory and are rounded nowhere.  ``through_logits``: from `logits`, rounded to the activations' type as `policy_loss` and `preference_loss`
+        take them.  Scores that those losses compare with their own (``old_logp``, ``ref_logp``) want this: a BF16 logit between 16 and 32 is rounded
+        by up to 0.0625, and otherwise the ratio of an unchanged policy is off from 1 by as much."""
+        targets = self._next_targets(tokens, mask)
+        if through_logits:
+            return F_.token_logprobs(self.logits(tokens), targets, temperature=temperature, vocab=self.config.vocab_size)
         h = self.hidden(tokens)
         w = self.wte if self.lm_head is None else self.lm_head
-        return F_.linear_logprobs(h, w.to(h.dtype) if w.dtype != h.dtype else w, self._next_targets(tokens, mask),
-                                  temperature=temperature / self._logit_scale(), vocab=self.config.vocab_size)
+        return F_.linear_logprobs(h, w.to(h.dtype) if w.dtype != h.dtype else w, targets, temperature=temperature / self._logit_scale(),
+                                  vocab=self.config.vocab_size)
 
     def policy_loss(self, tokens: torch.Tensor, mask: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
                     ref_logp: Optional[torch.Tensor] = None, **options) -> "F_.PolicyLoss":
         """`fused.ops.policy_loss` of sampled sequences [B, T]; ``mask`` is true on the tokens that were sampled, ``old_logp`` and ``ref_logp``
-        are as `token_logprobs` returns them, advantages [B] or [B, T] (of the token that an entry predicts).  The router losses of MoE layers
+        are as `token_logprobs` returns them (``through_logits``), advantages [B] or [B, T] (of the token that an entry predicts).  The router losses of MoE layers
         are added to the loss."""
         r = F_.policy_loss(self.logits(tokens), self._next_targets(tokens, mask), old_logp, advantages, ref_logp, vocab=self.config.vocab_size,
                            **options)
@@ -386,7 +394,7 @@ class LanguageModel(nn.Module):
 
     def preference_loss(self, tokens: torch.Tensor, mask: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, **options) -> "F_.PreferenceLoss":
         """`fused.ops.preference_loss` of pairs of sequences [2 P, T], the chosen ones first; ``mask`` is true on the answers' tokens, ``ref_logp``
-        [2 P] the sums (with ``average`` the means) of the reference model's `token_logprobs`."""
+        [2 P] the sums (with ``average`` the means) of the reference model's `token_logprobs` (``through_logits``)."""
         r = F_.preference_loss(self.logits(tokens), self._next_targets(tokens, mask), ref_logp, vocab=self.config.vocab_size, **options)
         return r._replace(loss=r.loss + self.aux_loss()) if self.config.moe_experts > 0 else r
 
