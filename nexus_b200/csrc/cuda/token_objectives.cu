@@ -449,15 +449,16 @@ struct RowInfo {
 // What the row's end makes of its sums, for every worker's second pass.
 struct RowEnd {
   float c, c1, es, eb;   // g = 2^t (es t + eb), without an entropy term 2^t c1; c more at the target
-  int32_t careful;
+  int32_t careful;       // or kStop: a wait has run out, nothing more is written
   float m, log2_s, slope, off;  // careful: g = 2^((v - m) k - log2_s) (slope (v - m) + off)
 };
+constexpr int kStop = 2;
 constexpr int kAhead = 4;
 template <typename S>
 struct RingSpace {
   RowInfo info[kAhead];
   RowEnd end;
-  float4 warps[S::kWorkers / 32];    // (m, s, h) of each warp
+  float4 warps[S::kWorkers / 32];    // (m, s, h) of each warp, and whether one of its waits has run out
   float4 blocks[2][kMaxCuts];        // of each block of the cluster, in turns
   uint64_t full[S::kSlots], empty[S::kSlots], told[kAhead], heard[kAhead];
   uint64_t arrived;                  // counts the blocks that have put theirs in
@@ -493,11 +494,13 @@ __device__ __forceinline__ void join_lanes(float4& v, float k) {
   }
 }
 
-// Joins all threads' and blocks' sums of a row; the first warp gets them.
+// Joins all threads' and blocks' sums of a row; the first warp gets them.  The last component is not zero where a wait of any thread or block has run
+// out (`fine` is what this thread knows of it), so that all of them stop at the same row.
 template <bool kMaxima, typename S>
-__device__ __forceinline__ float4 join_all(float4 v, float k, RingSpace<S>* sp, int rank, int cuts, int& turn) {
+__device__ __forceinline__ float4 join_all(float4 v, float k, RingSpace<S>* sp, int rank, int cuts, int& turn, bool& fine) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   join_lanes<kMaxima, 32>(v, k);
+  v.w = __all_sync(0xffffffffu, fine) ? 0.0f : 1.0f;
   if (lane == 0) sp->warps[warp] = v;
   workers_sync<S>();
   const int side = turn & 1;
@@ -505,6 +508,7 @@ __device__ __forceinline__ float4 join_all(float4 v, float k, RingSpace<S>* sp, 
   if (warp != 0) return v;
   v = sp->warps[lane & (S::kWorkers / 32 - 1)];
   join_lanes<kMaxima, S::kWorkers / 32>(v, k);
+  v.w = __any_sync(0xffffffffu, v.w != 0.0f) ? 1.0f : 0.0f;
   if (cuts > 1) {
     if (lane < cuts) {  // a lane per block of the cluster
       const uint32_t to = mapa_shared(smem_u32(&sp->blocks[side][rank]), lane);
@@ -528,10 +532,11 @@ __device__ __forceinline__ float4 join_all(float4 v, float k, RingSpace<S>* sp, 
         }
       }
     }
-    __syncwarp();
+    if (!__all_sync(0xffffffffu, done != 0)) fine = false;
     v = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
     if ((lane & (kMaxCuts - 1)) < cuts) v = sp->blocks[side][lane & (kMaxCuts - 1)];
     join_lanes<kMaxima, kMaxCuts>(v, k);
+    v.w = !fine || __any_sync(0xffffffffu, v.w != 0.0f) ? 1.0f : 0.0f;
   }
   return v;
 }
@@ -663,15 +668,22 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int slot = 0, turn = 0, seat = 0;
     uint32_t phase = 0, seat_phase = 0;
-    bool fine = true;
+    bool fine = true, stopped = false;  // a wait of this thread has not run out; one of any has, and all warps have left at the same row
     auto wait = [&](uint64_t* bar, uint32_t ph) { fine = mbar_wait_bounded(bar, ph, abort_flag) && fine; };
     auto release = [&](int s) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sp->empty[s]);
     };
+    auto stop = [&] {  // the first warp, between the two barriers of a join
+      if (lane == 0) {
+        sp->end.careful = kStop;
+        *abort_flag = 1;
+      }
+    };
     const Pair kk = pair_of(k, k);
     for (uint64_t row = first; row < rows; row += step) {
       wait(&sp->told[seat], seat_phase);
+      if (!__all_sync(0xffffffffu, fine)) break;  // nothing is known of this row; the others hear of it in their next join or behind the loop
       const int32_t tg = sp->info[seat].target;
       const int64_t at = sp->info[seat].at;
       const float xt = sp->info[seat].x;
@@ -754,7 +766,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
       float s0, s1, h0, h1;
       halves(on.s, s0, s1);
       halves(on.h, h0, h1);
-      float4 st = join_all<false, S>(make_float4(0.0f, s0 + s1, h0 + h1, 0.0f), k, sp, rank, cuts, turn);
+      float4 st = join_all<false, S>(make_float4(0.0f, s0 + s1, h0 + h1, 0.0f), k, sp, rank, cuts, turn, fine);
       // The first warp ends the row and tells the others how its gradient comes.  `m`, `sum` and `h` relative to it where done with maxima.
       auto end_row = [&](const float4& v, bool careful) {
         RowEnd e{};
@@ -801,11 +813,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
       if (warp == 0) {
         const bool careful = !(fabsf(xt) <= kFastLimit && fabsf(base) <= kFastLimit && st.y <= (second ? kFastSumDivides : kFastSum) &&
                                (!kPolicy || fmaf(PieceOf<T>::kLowest, k, -base) <= kNoWeight));
-        if (!careful) end_row(st, false);
+        if (st.w != 0.0f) stop();
+        else if (!careful) end_row(st, false);
         else if (lane == 0) sp->end.careful = 1;
-        if (!kPolicy && !careful && lane == 0) sp->end.careful = 0;
+        if (!kPolicy && st.w == 0.0f && !careful && lane == 0) sp->end.careful = 0;
       }
       workers_sync<S>();
+      if (sp->end.careful == kStop) {
+        stopped = true;
+        break;
+      }
       if (sp->end.careful) {  // the same in every block of the cluster; from memory, with maxima and the difference first
         Online on2;
         const T* body = p + r.head + static_cast<int64_t>(lo) * VN;
@@ -818,9 +835,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
           const float v[1] = {ev};
           on2.absorb(v, k);
         }
-        st = join_all<true, S>(make_float4(on2.m, on2.s, on2.h, 0.0f), k, sp, rank, cuts, turn);
-        if (warp == 0) end_row(st, true);
+        st = join_all<true, S>(make_float4(on2.m, on2.s, on2.h, 0.0f), k, sp, rank, cuts, turn, fine);
+        if (warp == 0) {
+          if (st.w != 0.0f) stop();
+          else end_row(st, true);
+        }
         workers_sync<S>();
+        if (sp->end.careful == kStop) {
+          stopped = true;
+          break;
+        }
       }
       if constexpr (second) {
         const RowEnd e = sp->end;
@@ -873,7 +897,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
               c = (d < slots ? d : d - slots) * kSlotPieces;
               const uint4* data = reinterpret_cast<const uint4*>(ring_smem + slot * kSlotBytes);
               if (d >= slots) wait(&sp->full[slot], phase);
-              if (c + kSlotPieces <= n) {
+              if (!fine) {  // not there
+              } else if (c + kSlotPieces <= n) {
                 uint4 q[kPer];
 #pragma unroll
                 for (int u = 0; u < kPer; ++u) q[u] = data[tid + u * kWorkers];
@@ -905,6 +930,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const N
         }
         for (int w = a.vocab + rank * kWorkers + tid; w < a.width; w += cuts * kWorkers) Num<T>::store(gr + w, 0.0f);
       }
+    }
+    if (!stopped) {  // the barriers of one more join: a warp that has left early meets the others here, or here those that are in a row
+      const bool all = __all_sync(0xffffffffu, fine);
+      if (lane == 0) sp->warps[warp].w = all ? 0.0f : 1.0f;
+      workers_sync<S>();
+      if (warp == 0 && __any_sync(0xffffffffu, sp->warps[lane & (kWorkers / 32 - 1)].w != 0.0f)) stop();
+      workers_sync<S>();
     }
     if (!fine) atomicCAS(o.status, 0, kStatusTimeoutEpilogue);
   }
