@@ -44,7 +44,7 @@ class PreferenceLoss(NamedTuple):
     margin: torch.Tensor
 
 
-def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature: float) -> int:
+def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature: float, ignore_index: int) -> int:
     if not logits.is_floating_point() or logits.dim() < 1:
         raise ValueError(f"{name}: logits must be a floating-point tensor [..., vocabulary]")
     shape = logits.shape
@@ -55,6 +55,7 @@ def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature:
     if targets.device != logits.device:
         raise ValueError(f"{name}: targets on {targets.device}, logits on {logits.device}")
     _check_temperature(name, temperature)
+    _check_ignored(name, ignore_index)
     V = shape[-1] if vocab is None else int(vocab)
     if not 1 <= V <= shape[-1]:
         raise ValueError(f"{name}: vocab must be between 1 and {shape[-1]}, got {V}")
@@ -66,6 +67,11 @@ def _check_logits(name: str, logits, targets, vocab: Optional[int], temperature:
 def _check_temperature(name: str, temperature: float) -> None:
     if not 1e-8 <= temperature <= 1e8:     # its inverse times a logit is an FP32 number, and -inf stays far below every logit
         raise ValueError(f"{name}: temperature must be between 1e-8 and 1e8, got {temperature}")
+
+
+def _check_ignored(name: str, ignore_index: int) -> None:
+    if not -2 ** 63 <= ignore_index < 2 ** 63:     # the kernels would take it modulo 2^64
+        raise ValueError(f"{name}: ignore_index must be a 64-bit integer, got {ignore_index}")
 
 
 def _check_values(name: str, what: str, t, shapes, device) -> torch.Tensor:
@@ -165,7 +171,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: in
                    vocab: Optional[int] = None) -> torch.Tensor:
     """FP32 log-probability of ``targets`` [...] under ``softmax(logits / temperature)``, logits [..., V(+pad)]; zero where the target is
     `ignore_index`.  Differentiable (once) with respect to the logits; any row strides, the innermost one 1 (others are copied)."""
-    V = _check_logits("token_logprobs", logits, targets, vocab, temperature)
+    V = _check_logits("token_logprobs", logits, targets, vocab, temperature, ignore_index)
     if targets.numel() and _kernels(logits) and not _dual(logits):
         if _wants(logits):
             return _TokenLogprobs.apply(logits, targets, V, ignore_index, float(temperature))
@@ -228,6 +234,7 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"{name}: targets {tuple(targets.shape)} do not match hidden {tuple(hidden.shape)}")
     _check_temperature(name, temperature)
+    _check_ignored(name, ignore_index)
     V = weight.shape[0] if vocab is None else int(vocab)
     if not 1 <= V <= weight.shape[0]:
         raise ValueError(f"{name}: vocab must be between 1 and {weight.shape[0]}, got {V}")
@@ -320,7 +327,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
     multiplied afterwards, so the factor of an accumulated micro-batch is better given as ``scale``.  With FP16 logits it is made in the
     backward pass, with a second read of them: a loss scale must be in it before it is rounded."""
     name = "policy_loss"
-    V = _check_logits(name, logits, targets, vocab, temperature)
+    V = _check_logits(name, logits, targets, vocab, temperature, ignore_index)
     if targets.dim() != 2:
         raise ValueError(f"{name}: logits must be [B, T, V] and targets [B, T]")
     B, T = targets.shape
@@ -414,7 +421,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logp: Optio
     ``"sigmoid"``: -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z); ``"hinge"``: max(0, 1 - z); ``"ipo"``:
     (h - 1 / (2 beta))^2.  The loss is the mean over the pairs."""
     name = "preference_loss"
-    V = _check_logits(name, logits, targets, vocab, temperature)
+    V = _check_logits(name, logits, targets, vocab, temperature, ignore_index)
     if targets.dim() != 2 or targets.shape[0] < 2 or targets.shape[0] % 2:
         raise ValueError(f"{name}: logits must be [2 P, T, V] and targets [2 P, T] with P >= 1 chosen sequences before P rejected ones")
     if kind not in ("sigmoid", "hinge", "ipo"):

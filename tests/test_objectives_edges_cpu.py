@@ -105,3 +105,13 @@ def test_advantages_of_zero_beside_ratios_beyond_fp32():
     old[0, 0] = math.nan
     assert math.isnan(float(F.policy_loss(x, t, old, torch.zeros(2)).loss.detach()))
     assert math.isinf(float(F.policy_loss(x, t, torch.full_like(old, -100.0), -torch.ones(2)).loss.detach()))
+
+
+def test_refuses_an_ignored_index_beyond_64_bits():
+    x, t, z = torch.zeros(2, 3, 8), torch.ones(2, 3, dtype=torch.long), torch.zeros(2, 3)
+    for index in (2 ** 64 + 1, 2 ** 63, -2 ** 63 - 1):
+        for call in (lambda: F.token_logprobs(x, t, ignore_index=index), lambda: F.linear_logprobs(x, torch.zeros(5, 8), t, ignore_index=index),
+                     lambda: F.policy_loss(x, t, z, z, ignore_index=index), lambda: F.preference_loss(x, t, ignore_index=index)):
+            with pytest.raises(ValueError, match="ignore_index"):
+                call()
+    assert bool((F.token_logprobs(x, t, ignore_index=2 ** 63 - 1) != 0).all())
