@@ -652,7 +652,9 @@ def clip_grads(name: str, grads, max_norm: float, out=None):
         coef = min(1.0, max_norm / (norm + 1e-6)) if math.isfinite(norm) else 1.0
         for i, g in enumerate(full):
             if outs is not None:
-                outs[i].copy_(g if coef == 1.0 else g * coef)
+                if coef != 1.0:      # the product in a type that holds both (FP8: of the gradient)
+                    g = (g if outs[i].element_size() == 1 else g.to(torch.promote_types(g.dtype, outs[i].dtype))) * coef
+                outs[i].copy_(g)
             elif coef != 1.0:
                 g.mul_(coef)
         return torch.tensor(sq, dtype=torch.float64), torch.tensor(norm, dtype=torch.float32, device=full[0].device)

@@ -67,3 +67,5 @@ def test_fp8_gradients_are_refused():
     assert torch.equal(a, torch.ones(8, device="cuda"))
     assert float(F.clip_grad_norm_([2.0 * a], 1e3, out=[b])) == pytest.approx(32.0 ** 0.5) and bool((b.float() == 2.0).all())
     assert F.grad_square_sum([a, b]) == 40.0
+    F.clip_grad_norm_([a], 8.0 ** 0.5 / 2, out=[b])
+    assert bool((b.float() == 0.5).all())

@@ -16,6 +16,8 @@ def test_fp8_gradients_are_refused():
     assert torch.equal(a, torch.ones(8))
     assert float(F.clip_grad_norm_([2.0 * a], 1e3, out=[b])) == pytest.approx(32.0 ** 0.5) and bool((b.float() == 2.0).all())
     assert F.grad_square_sum([a, b]) == 40.0
+    F.clip_grad_norm_([a], 8.0 ** 0.5 / 2, out=[b])
+    assert bool((b.float() == 0.5).all())
 
 
 def test_forward_mode_derivatives():
@@ -115,3 +117,14 @@ def test_refuses_an_ignored_index_beyond_64_bits():
             with pytest.raises(ValueError, match="ignore_index"):
                 call()
     assert bool((F.token_logprobs(x, t, ignore_index=2 ** 63 - 1) != 0).all())
+
+
+@pytest.mark.parametrize("src,dst", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.bfloat16, torch.float16), (torch.float32, torch.float64)])
+def test_clipped_values_of_a_wider_type_are_rounded_once(src, dst):
+    g = torch.randn(500, generator=torch.Generator().manual_seed(0)).to(src)
+    out = torch.empty(500, dtype=dst)
+    F.clip_grad_norm_([g], 1.0, out=[out])
+    want = g.double() / (g.double().norm() + 1e-6)
+    step = {torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24, torch.float64: 2.0 ** -53}[dst]
+    # the factor as FP32 or FP64, the product, the type it goes to; half a subnormal step of FP16
+    assert bool(((out.double() - want).abs() <= (2 * max(step, 2.0 ** -53) + 2.0 ** -24 * (dst != torch.float64) + 2.0 ** -51) * want.abs() + 2.0 ** -25 * (dst == torch.float16)).all())
