@@ -214,11 +214,16 @@ class _LinearLogprobs(torch.autograd.Function):
 def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,
                     vocab: Optional[int] = None, recompute: bool = False) -> torch.Tensor:
     """`token_logprobs` of the logits ``hidden @ weight.T`` without the logits in memory: hidden [..., d], weight [V(+pad), d] of one type,
-    targets [...].  Differentiable (once) with respect to both.  Where a gradient is wanted, d is 512 or more and there are at most 2^29
-    logits (of at most 65536 tokens), their exponentials are held in 16 bits (1 GiB at most) until the backward pass turns them into the
-    logits' gradient in place; else, or with ``recompute``, nothing is held and the backward pass makes the logits again (a third more products), their gradient of at most 2^29 logits
-    (or of 256 rows) at a time.  The kernels take BF16 and FP16 with d a multiple of 8 (logits in FP32, rounded nowhere; their gradient
-    rounded to the type for its products); other types and sizes go through the logits.  Under autocast the operands are cast as a linear layer's are."""
+    targets [...].  Differentiable (once) with respect to both.
+
+    Where a gradient is wanted, d is 512 or more and there are at most 2^29 logits (of at most 65536 tokens), their exponentials are held in
+    16 bits (1 GiB at most) until the backward pass turns them into the logits' gradient in place.  Else, or with ``recompute``, nothing is held
+    and the backward pass makes the logits again (a third more products), their gradient of at most 2^29 logits (or of 256 rows) at a time.
+
+    The kernels take BF16 and FP16 with d a multiple of 8.  Log-probabilities come from logits in FP32 that are rounded nowhere.  The logits'
+    gradient is rounded to the operands' type for its products, once with ``recompute``; from held exponentials twice, the exponential itself and
+    its product with the row's coefficient.  FP32 and other widths go through the logits of a linear layer.  Under autocast the operands are cast
+    as a linear layer's are."""
     name = "linear_logprobs"
     if hidden.is_cuda and torch.is_autocast_enabled("cuda") and hidden.is_floating_point() and weight.is_floating_point():
         dtype = torch.get_autocast_dtype("cuda")
