@@ -4,8 +4,8 @@
 // arguments, so nothing is uploaded and a captured graph carries its own.  A block walks over pieces of kPiece elements, whatever tensors they
 // belong to.  The second kernel's blocks each add up the first one's partial sums, in the same order, instead of a launch in between.
 // Bound by bytes: every gradient is read twice and written once; the second pass walks backwards, so that it begins with what the first one
-// left in L2.  8 x [4096, 4096] FP32: norm 82 us (6.5 TB/s), both passes to other memory 293 us (5.5 TB/s of two reads and a write); in place with a norm
-// that is small enough 107.  Other shapes of blocks (256, 1024 threads; two or four pieces in flight) and stores past L2 were no faster.
+// left in L2.  8 x [4096, 4096] FP32: norm 82 us (6.5 TB/s), both passes to other memory 293 us (5.5 TB/s of two reads and a write); in place with
+// a norm that is small enough 107.  Other shapes of blocks (256, 1024 threads; two or four pieces in flight) and stores past L2 were no faster.
 #include "common.cuh"
 #include "nx_api_objectives.h"
 #include "row_vec.cuh"
@@ -213,7 +213,8 @@ extern "C" int nx_grad_clip(const NxGradTable* g, double max_norm, int clip, dou
       !(max_norm >= 0.0))
     return -1;
   for (int64_t i = 0; i < g->tensors; ++i)
-    if (g->src[i] == nullptr || g->count[i] < 1 || (g->type[i] & 15) > NX_F16 || (g->type[i] >> 4) > NX_F16 || (g->dst != nullptr && g->dst[i] == nullptr))
+    if (g->src[i] == nullptr || g->count[i] < 1 || (g->type[i] & 15) > NX_F16 || (g->type[i] >> 4) > NX_F16 ||
+        (g->dst != nullptr && g->dst[i] == nullptr))
       return -1;
   return run<kTableMax>(g, max_norm, clip, partial, out, static_cast<cudaStream_t>(stream));
 }

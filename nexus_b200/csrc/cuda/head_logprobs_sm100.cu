@@ -10,9 +10,9 @@
 //   grad    otherwise h W^T again, whose epilogue turns the logits into G in 16 bits: one product more, and G of a bounded number of rows is
 //           all that is ever in memory
 //   dh, dW  G W and G^T h
-// Bound by the tensor cores: 2048 x 2048 x 32000 BF16 at 86 (statistics, exponentials written) and 87 % (dh) of their pipe, 180 us each, 1.49 PFLOP/s; at
-// 5376 x 4096 x 32000 1.05 ms for each of the three products, 1.33 PFLOP/s (to 1.43 in other runs), under
-// the power cap.
+// Bound by the tensor cores: 2048 x 2048 x 32000 BF16 at 86 (statistics, exponentials written) and 87 % (dh) of their pipe, 180 us each, 1.49
+// PFLOP/s; at 5376 x 4096 x 32000 1.05 ms for each of the three products, 1.33 PFLOP/s (to 1.43 in other runs), under the power cap.  The
+// statistics' form spills 40 bytes stored, 56 loaded (168 registers, which ten warps leave it); the others nothing.
 // Rows whose target does not count are left out before the first product: the others are brought together in order (their number stays on the
 // device and bounds every loop), so that prompts and padding cost no tensor-core time.  A tile is 256 rows: without a gradient, up to that
 // many rows stay where they are (with one they would put 0 * h of a row that does not count into dW, and h may hold anything there).
@@ -83,7 +83,8 @@ struct Extent {
   int slices, per;          // input gradient: pieces of the vocabulary, and blocks of a piece
 };
 // Pieces of `blocks` 64-deep blocks for each of `tiles` tiles, so that the CTA pairs finish together: rounds times (blocks of a piece and six for
-// handing a tile over).  Chosen here, from the number of rows that count: by all rows, 380 of 609 kept 48 of the 74 pairs busy (156 us; now 130 to 141).
+// handing a tile over).  Chosen here, from the number of rows that count: by all rows, 380 of 609 kept 48 of the 74 pairs busy (156 us; now 130
+// to 141).
 __device__ __forceinline__ void cut(Extent& e, int tiles, int blocks, int most) {
   int best = 0x7fffffff;
   e.slices = 1;
@@ -573,7 +574,8 @@ head_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 // Scoring beside decoding: the time is that of reading the weight once.  The weight's rows are the tall operand here: every SM takes one run of
 // the vocabulary, in groups of 32 rows so that the runs differ by at most one group (with 256 x 256 tiles 50257 rows were 197 tiles for 74 pairs,
 // three rounds for 2.7), and a lane of the epilogue keeps maximum and sum of one row of a tile for every token, over all tiles of the run; lanes
-// meet once, at its end.  8 x 50257 x 1600 BF16: 35 us (4.6 TB/s of weights), 256 x 256 tiles 44.
+// meet once, at its end.  8 x 50257 x 1600 BF16: 35 us (4.6 TB/s of weights), 256 x 256 tiles 44.  The form for 64 tokens keeps 192 values per lane
+// and spills (255 registers; 148 bytes stored, 164 loaded): 50 us with L2 flushed, where 32 tokens take 46 and a plain read of the weight 37.
 constexpr int kFewRows = 64, kFewThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2..5: a quarter of the 128 lanes each
 constexpr int kGroupBytes = 32 * kBK * 2, kFewAccumulators = 4;
 template <int NT>
@@ -1093,7 +1095,8 @@ int launch_few(const NxHeadArgs* a, const Params& p, int blocks, cudaStream_t st
 }
 template <bool BF>
 int launch_few(const NxHeadArgs* a, const Params& p, int blocks, cudaStream_t st) {
-  return a->rows <= 16 ? launch_few<16, BF>(a, p, blocks, st) : a->rows <= 32 ? launch_few<32, BF>(a, p, blocks, st) : launch_few<64, BF>(a, p, blocks, st);
+  if (a->rows <= 16) return launch_few<16, BF>(a, p, blocks, st);
+  return a->rows <= 32 ? launch_few<32, BF>(a, p, blocks, st) : launch_few<64, BF>(a, p, blocks, st);
 }
 
 // K-major operand of [rows][k], or MN-major of [k][mn]; 128-byte swizzle
@@ -1196,7 +1199,8 @@ extern "C" int nx_head_logprobs(const NxHeadArgs* a, float* logp, float* tlogit,
 }
 
 extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, nx_stream_t stream) {
-  if (!args_ok(a) || a->index == nullptr || g == nullptr || g->coef == nullptr || g->logit_grad == nullptr || g->chunk < kTile || g->chunk % kTile != 0 ||
+  if (!args_ok(a) || a->index == nullptr || g == nullptr || g->coef == nullptr || g->logit_grad == nullptr || g->chunk < kTile ||
+      g->chunk % kTile != 0 ||
       g->ld_logit_grad < a->vocab || g->ld_logit_grad % 64 != 0 || (reinterpret_cast<uintptr_t>(g->logit_grad) & 15) != 0 ||
       (a->dtype == NX_F16 && g->scale == nullptr) || g->slices < 1 || (g->slices > 1 && g->slice_sums == nullptr) ||
       (reinterpret_cast<uintptr_t>(g->d_hidden) & 15) != 0 || (reinterpret_cast<uintptr_t>(g->d_weight) & 15) != 0 ||
@@ -1216,7 +1220,8 @@ extern "C" int nx_head_logprobs_grad(const NxHeadArgs* a, const NxHeadGrad* g, n
   const bool sums = g->d_weight != nullptr && g->chunk < a->rows;  // several launches add up in FP32
   CUtensorMap w_k, w_mn, g_k, g_mn, g_out, dw_out;
   const int64_t ldg = g->ld_logit_grad;
-  if ((rc = map_k(&w_k, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0 || (rc = map_mn(&w_mn, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0 ||
+  if ((rc = map_k(&w_k, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0 ||
+      (rc = map_mn(&w_mn, a, a->weight, a->width, a->vocab, a->ld_weight)) != 0 ||
       (rc = map_k(&g_k, a, g->logit_grad, a->vocab, g->chunk, ldg)) != 0 || (rc = map_mn(&g_mn, a, g->logit_grad, a->vocab, g->chunk, ldg)) != 0 ||
       (rc = map_store(&g_out, a, g->logit_grad, a->vocab, g->chunk, ldg)) != 0)
     return rc;

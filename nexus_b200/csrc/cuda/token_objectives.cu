@@ -333,8 +333,8 @@ using LongShape = Shape<512, 13, 1, true>;
 // where B would be too coarse (|x_t| or |B| above kFastLimit: at temperatures of 1e-8 the second from logits of 0.007 on; -inf, NaN), is done again
 // in the form with running maxima and the difference first; and so is, where t is multiplied, one where the finite value that stands for -inf (an
 // FP16 piece holds none below -65504) comes so near the target's logit, or is scaled down so far, that its weight is not zero.
-// Where a second pass writes the gradient its factors are divided by s, and are normal numbers (the row's weight being 2^-66 or more) only while s stays
-// below 2^60: t of 60 and more, targets of a log-probability below -41, are done again there.
+// Where a second pass writes the gradient its factors are divided by s, and are normal numbers (the row's weight being 2^-66 or more) only while
+// s stays below 2^60: t of 60 and more, targets of a log-probability below -41, are done again there.
 constexpr float kFastLimit = 1.0e6f, kFastSum = 1.3e36f, kFastSumDivides = 0x1p60f;
 // Stands for -inf (and all below it) where t is multiplied: the weight is zero either way, and zero times a finite product is zero.  Representable in
 // BF16; no lower than it must be, so that k (up to 1.5e8) and the entropy's factors keep the products finite.
@@ -558,7 +558,8 @@ struct RingOut {
 };
 
 template <typename T, bool kPolicy, typename S>
-__global__ void __launch_bounds__(S::kThreads, S::kResident) ring_kernel(const NxTokenRows a, const NxPolicyArgs g, const RingOut o, T* __restrict__ grad) {
+__global__ void __launch_bounds__(S::kThreads, S::kResident)
+ring_kernel(const NxTokenRows a, const NxPolicyArgs g, const RingOut o, T* __restrict__ grad) {
   constexpr int kWorkers = S::kWorkers, kSlots = S::kSlots;
   constexpr int VN = RowVec<T>::kN, kPer = kSlotPieces / kWorkers;
   extern __shared__ __align__(128) uint8_t ring_smem[];
@@ -1174,7 +1175,8 @@ extern "C" int nx_policy_loss(const NxTokenRows* a, const NxPolicyArgs* g, doubl
                               float* entropy, float* row_loss, float* loss, void* grad, NxPolicySlope* slopes, int* status, nx_stream_t stream) {
   if (!rows_ok(a) || a->rows == 0 || g == nullptr || (reinterpret_cast<uintptr_t>(slopes) & 3) != 0 ||
       totals == nullptr || (reinterpret_cast<uintptr_t>(totals) & 7) != 0 || counts == nullptr || loss == nullptr || status == nullptr ||
-      g->adv_per < 1 || g->adv_per > 0x7fffffff || g->seq_len < 1 || g->seq_len > 0x7fffffff || a->rows % g->seq_len != 0 || (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
+      g->adv_per < 1 || g->adv_per > 0x7fffffff || g->seq_len < 1 || g->seq_len > 0x7fffffff || a->rows % g->seq_len != 0 ||
+      (g->write_grad && (grad == nullptr || !same_lines(a->logits, grad))))
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   NX_PDL(token_count_kernel, kJoinBlocks, kJoinThreads, 0, st, a->targets, a->targets_wide, g->mean != NX_MEAN_NONE ? a->rows / g->seq_len : 0,

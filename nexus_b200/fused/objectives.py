@@ -354,7 +354,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logp: torch.Ten
         a = O.PolicyArgs(old.data_ptr(), None if ref is None else ref.data_ptr(), adv.data_ptr(), T if adv.dim() == 1 else 1, T, clip_low, clip_high,
                          kl_coef, entropy_coef, scale, O.KL[kl], O.MEAN[reduction], 0)
         if _wants(logits):
-            return PolicyLoss(*(_PolicyLossHalf if logits.dtype == torch.float16 else _PolicyLoss).apply(logits, targets, V, ignore_index, float(temperature), old, a))
+            form = _PolicyLossHalf if logits.dtype == torch.float16 else _PolicyLoss
+            return PolicyLoss(*form.apply(logits, targets, V, ignore_index, float(temperature), old, a))
         return PolicyLoss(*_policy_forward(logits, targets, V, ignore_index, temperature, old, a, False)[0])
     keep, lp, logp = _token_parts(logits, targets, ignore_index, temperature, V)
     zero = torch.zeros((), dtype=lp.dtype, device=lp.device)
@@ -535,7 +536,9 @@ def _plain_table(grads, out):
     own.  None for every other list, wrong ones among them."""
     every = grads if out is None else grads + out
     try:
-        if not every or not _kernels(every[0]) or len(set(map(torch.Tensor.get_device, every))) != 1 or not all(map(torch.Tensor.is_contiguous, every)):
+        if not every or not _kernels(every[0]) or len(set(map(torch.Tensor.get_device, every))) != 1:
+            return None
+        if not all(map(torch.Tensor.is_contiguous, every)):
             return None
         if out is not None and list(map(_shape, grads)) != list(map(_shape, out)):
             return None

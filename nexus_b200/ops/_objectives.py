@@ -140,8 +140,8 @@ def policy_loss(rows: TokenRows, args: PolicyArgs, like: torch.Tensor, grad, slo
     at = scratch.data_ptr()
     args.write_grad = grad is not None
     _call("nx_policy_loss", C.byref(rows), C.byref(args), at, at + 24, logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
-          at + 24 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(), None if slopes is None else slopes.data_ptr(),
-          K.status_word(dev).data_ptr())
+          at + 24 + 4 * (n // args.seq_len), loss.data_ptr(), None if grad is None else grad.data_ptr(),
+          None if slopes is None else slopes.data_ptr(), K.status_word(dev).data_ptr())
     return loss, logp, kl, entropy
 
 
@@ -305,8 +305,8 @@ def head_logprobs_grad(hidden, weight, targets, vocab: int, ignore_index: int, i
     if want_weight and weight.shape[0] > vocab:
         dw[vocab:].zero_()
     a = _head_args(hidden, weight, targets, base + index, moved, base + stats, part, weights, vocab, ignore_index, inv_temp)
-    g = HeadGrad(coef.data_ptr(), weights.data_ptr() if grad_at is None else at + grad_at, chunk, ld, at + scale, None if dh is None else dh.data_ptr(),
-                 None if dw is None else dw.data_ptr(), None if slice_sums is None else at + slice_sums,
+    g = HeadGrad(coef.data_ptr(), weights.data_ptr() if grad_at is None else at + grad_at, chunk, ld, at + scale,
+                 None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr(), None if slice_sums is None else at + slice_sums,
                  None if weight_sums is None else at + weight_sums, slices, 0)
     _call("nx_head_logprobs_grad", C.byref(a), C.byref(g))
     return dh, dw
