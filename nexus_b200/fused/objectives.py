@@ -308,10 +308,10 @@ class _PolicyLoss(torch.autograd.Function):
             return (None,) * 7
         _backward_only("policy_loss", dloss)
         (grad,) = ctx.saved_tensors
-        # a graph that is kept may be walked again, and then needs the gradient as it was
-        if torch._C._autograd._get_current_graph_task_keep_graph():
-            return ((grad.float() * dloss.float()).to(grad.dtype), *(None,) * 6)
         with _on(grad):
+            # a graph that is kept may be walked again, and then needs the gradient as it was
+            if torch._C._autograd._get_current_graph_task_keep_graph():
+                grad = grad.clone()
             O.scale_unless_one_(grad, dloss.float())
         return (grad, *(None,) * 6)
 

@@ -226,3 +226,23 @@ def test_advantages_of_zero_beside_ratios_beyond_fp32():
     old[0, 0] = math.nan
     assert math.isnan(float(F.policy_loss(x, t, old, torch.zeros(2, device="cuda")).loss.detach()))
     assert math.isinf(float(F.policy_loss(x, t, torch.full_like(old, -100.0), -torch.ones(2, device="cuda")).loss.detach()))
+
+
+@pytest.mark.parametrize("form", ["whole", "view"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_kept_graph_costs_one_copy_of_the_gradient(dtype, form):
+    full = torch.randn(2, 65, 8200, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(dtype)
+    x = (full if form == "whole" else full[:, 1:, :8100]).detach().requires_grad_(True)
+    t = torch.randint(0, 8100, x.shape[:2], device="cuda")
+    old, adv = torch.full(x.shape[:2], -9.0, device="cuda"), torch.tensor([1.0, -2.0], device="cuda")
+    loss = F.policy_loss(x, t, old, adv, entropy_coef=0.01).loss
+    up = torch.tensor(0.3, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    (a,) = torch.autograd.grad(loss, x, up, retain_graph=True)
+    assert torch.cuda.max_memory_allocated() - before < 1.1 * full.numel() * full.element_size() + (1 << 21)
+    (b,) = torch.autograd.grad(loss, x, up, retain_graph=True)
+    (c,) = torch.autograd.grad(loss, x, retain_graph=True)
+    (d,) = torch.autograd.grad(loss, x, up)
+    assert torch.equal(a, b) and torch.equal(a, d) and torch.equal(a, (c.float() * up).to(dtype))
